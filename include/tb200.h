@@ -43,6 +43,12 @@ extern "C" {
 #define TB200_DT_BF16 2
 #define TB200_DT_F8E4M3 3
 
+/* Gate functions f of the gated feed-forward block. */
+#define TB200_ACT_SILU      0  /* g / (1 + exp(-g))                                            */
+#define TB200_ACT_GELU      1  /* g * (1 + erf(g / sqrt(2))) / 2                               */
+#define TB200_ACT_GELU_TANH 2  /* g * (1 + tanh(sqrt(2 / pi) * (g + 0.044715 g^3))) / 2        */
+#define TB200_ACT_RELU      3  /* max(g, 0), derivative 0 at 0                                 */
+
 int         tb200_abi_version(void);
 /* Message of the calling thread's most recent failing call ("" if none). */
 const char* tb200_last_error(void);
@@ -230,6 +236,50 @@ int    tb200_gemm_w4a16_static(const void* a, const void* wp, const void* scales
  */
 int tb200_allgather_cols(const void* local, int64_t ld_local, void* const* out_ptrs, int world, int rank,
                          int64_t m, int64_t n_local, int64_t elem_bytes, int64_t ldo, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Gated feed-forward block with its activations kept in 8 bits (new operators `act_checkpoint_fp8`,
+ * `act_restore_fp8`, `ffn_gated`, `ffn_gated_bwd`; no counterpart in the reference).
+ *
+ * 8-bit form of a [rows, cols] activation: e4m3 codes [rows, cols], contiguous, and one fp32 scale per 1 x 128
+ * block of a row, [rows, ceil(cols / 128)] (the last block of a row may be short).  The scale is the smallest
+ * power of two 2^e, e >= -126, with amax <= 448 * 2^e, 1 for a block without a non-zero finite value; a code is
+ * the e4m3 number nearest to x / scale (ties to even).  Infinities and NaN are stored as NaN and do not enter
+ * amax.  Where cols is a multiple of 128 the pair also serves as `a`, `sa` of tb200_gemm_fp8_blockscaled.
+ * rows / m = 0 is a valid call: nothing is launched (the weights' gradients are set to zero).
+ * ------------------------------------------------------------------------------------------- */
+
+/* Codes and scales of x (dtype F32, F16 or BF16), rows ldx elements apart.  Any width, stride and alignment;
+ * rows on 16-byte boundaries with cols a multiple of 8 are the faster path. */
+int tb200_act_checkpoint_fp8(const void* x, void* q, float* scales, int64_t rows, int64_t cols, int64_t ldx,
+                             int dtype, void* stream);
+/* out[r, c] = code * scale in `dtype` (F32, F16 or BF16), [rows, cols] contiguous.  A product beyond the type's
+ * largest finite value becomes that value (an amax close to it may have been rounded up). */
+int tb200_act_restore_fp8(const void* q, const float* scales, void* out, int64_t rows, int64_t cols, int dtype,
+                          void* stream);
+/*
+ * h = f(x Wg^T) * (x Wu^T) in one kernel: x [m, k] with rows ldx elements apart, wg and wu [f, k], h [m, f], all of
+ * dtype F16 or BF16; fp32 accumulation, one rounding at the end.
+ *   gq, gs, uq, us   all NULL, or the 8-bit forms of g = x Wg^T and u = x Wu^T ([m, f]; taken from the fp32 sums),
+ *                    which the backward pass reads
+ *   act              TB200_ACT_*
+ * k and ldx must be multiples of 8, x, wg and wu 16-byte aligned; any m and f.
+ */
+int tb200_ffn_gated(const void* x, const void* wg, const void* wu, void* h, void* gq, float* gs, void* uq, float* us,
+                    int64_t m, int64_t f, int64_t k, int64_t ldx, int act, int dtype, void* stream);
+/* Bytes of scratch tb200_ffn_gated_bwd needs (256-byte aligned); x_codes: nonzero when x is passed in 8 bits. */
+size_t tb200_ffn_gated_bwd_workspace_bytes(int64_t m, int64_t f, int64_t k, int x_codes);
+/*
+ * Gradients of that block from dh [m, f] and the 8-bit forms of g and u:
+ *   dg = dh * u * f'(g), du = dh * f(g), rounded to dtype (a value beyond fp16's range becomes infinite there)
+ *   dx = dg Wg + du Wu [m, k],  dWg = dg^T x [f, k],  dWu = du^T x [f, k], of dtype, written (not accumulated)
+ * x is the block's input: of dtype with rows ldx elements apart (xs NULL), or its e4m3 codes with scales xs.
+ * k and ldx must be multiples of 8; wg, wu, dx, dwg, dwu (and x unless in 8 bits) 16-byte aligned; any m and f.
+ */
+int tb200_ffn_gated_bwd(const void* dh, const void* wg, const void* wu, const void* x, const float* xs,
+                        const void* gq, const float* gs, const void* uq, const float* us, void* dx, void* dwg, void* dwu,
+                        int64_t m, int64_t f, int64_t k, int64_t ldx, int act, int dtype, void* workspace,
+                        size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Device status word.  Every wait inside the GEMM kernels (mbarrier, TMEM hand-off) is bounded;

@@ -25,7 +25,7 @@ from tilebench_b200.core.timer import DEFAULT_REPEAT, DEFAULT_WARMUP, report_ben
 from tilebench_b200.core.verifier import config_tolerance, verify
 from tilebench_b200.data.tensors import SEED0, expand_cases, get_generator, infer_problem_size
 from tilebench_b200.hardware import detect_arch
-from tilebench_b200.paths import list_operators, operator_config
+from tilebench_b200.paths import list_layer_operators, list_operators, operator_config, operator_package
 
 HAS_CUDA = torch.cuda.is_available()
 DEFAULT_ENABLED_BACKENDS = GPU_BACKENDS
@@ -70,11 +70,12 @@ def run_benchmark_suite(operator_name, benchmark_overrides=None, enabled_backend
         config = yaml.safe_load(f)
 
     enabled = set(DEFAULT_ENABLED_BACKENDS if enabled_backends is None else canonical_backends(enabled_backends))
-    impl_torch = importlib.import_module(f"{OPERATOR_PACKAGE}.{operator_name}.impl_torch")
+    package = operator_package(operator_name) if operator_name in list_layer_operators() else f"{OPERATOR_PACKAGE}.{operator_name}"
+    impl_torch = importlib.import_module(f"{package}.impl_torch")
     impl_cuda = None
     if "cuda" in enabled:
         try:
-            impl_cuda = importlib.import_module(f"{OPERATOR_PACKAGE}.{operator_name}.impl_cuda")
+            impl_cuda = importlib.import_module(f"{package}.impl_cuda")
         except ImportError as e:
             print(f"  cuda import skipped: {e}")
     else:
@@ -100,7 +101,8 @@ def run_benchmark_suite(operator_name, benchmark_overrides=None, enabled_backend
             if idx < 0 or idx >= len(cases):
                 raise ValueError(f"case index {idx} out of range for {len(cases)} generated cases")
         cases = [cases[i] for i in case_indices]
-    op_index = list_operators().index(operator_name) if operator_name in list_operators() else 0
+    known = list_operators() + list_layer_operators()
+    op_index = known.index(operator_name) if operator_name in known else 0
 
     def _bench(fn, args, kw=None):
         return report_benchmark(fn, args, kwargs=kw or {}, warmup=warmup, repeat=repeat,

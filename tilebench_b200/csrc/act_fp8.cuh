@@ -1,0 +1,129 @@
+// The 8-bit form of an activation and the gate functions of the feed-forward block, shared by the kernels that save,
+// restore and use activation checkpoints.
+//
+// A 1 x 128 block of a row is stored as e4m3 codes and one power-of-two scale: the smallest 2^e (e >= -126) with
+// amax <= 448 * 2^e.  e4m3 carries its own exponent, so a finer scale would not make a code more precise; a power of
+// two makes x / s and code * s exact, so every code is the correctly rounded one whatever order the work is done in,
+// and restoring to bf16 or fp32 rounds nothing.  Infinities and NaN do not enter amax and are stored as NaN.
+#pragma once
+
+#include "common.cuh"
+
+#include <cuda_fp8.h>
+#include <float.h>
+
+namespace tb200 {
+
+constexpr int kActBlock = 128;
+
+#ifdef __CUDACC__
+
+__device__ __forceinline__ float act_size(float v) {            // |v|, 0 for infinities and NaN
+    const float a = fabsf(v);
+    return a <= FLT_MAX ? a : 0.0f;
+}
+// (scale, 1 / scale) of a block: both are powers of two within the normal range, so both are exact.
+__device__ __forceinline__ float2 act_scale(float amax) {
+    const uint32_t b = __float_as_uint(amax);
+    int e = static_cast<int>(b >> 23) - 8 + ((b & 0x7FFFFFu) > 0x600000u ? 1 : 0);      // 448 = 1.75 * 2^8
+    e = amax > 0.0f ? max(e, 1) : 127;
+    return make_float2(__uint_as_float(static_cast<uint32_t>(e) << 23), __uint_as_float(static_cast<uint32_t>(254 - e) << 23));
+}
+// The hardware conversion saturates, so what is not finite is made NaN first (finite values are at most 448 here).
+__device__ __forceinline__ float act_scaled(float v, float inv) {
+    const float y = v * inv;
+    return fabsf(y) <= 448.0f ? y : __int_as_float(0x7FC00000);
+}
+__device__ __forceinline__ uint32_t act_codes2(float a, float b) {
+    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ uint32_t act_codes4(float a, float b, float c, float d, float inv) {
+    return act_codes2(act_scaled(a, inv), act_scaled(b, inv)) | (act_codes2(act_scaled(c, inv), act_scaled(d, inv)) << 16);
+}
+__device__ __forceinline__ float2 act_values2(uint32_t codes) { // two codes in the low half, as numbers (exact)
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes), __NV_E4M3);
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+// code * scale, held within +-top: a block whose amax is close to the type's largest value may round up beyond it.
+__device__ __forceinline__ float act_restored(float code, float s, float top) {
+    const float v = code * s;
+    return fabsf(v) > top ? copysignf(top, v) : v;              // a NaN code stays NaN
+}
+
+template <typename T> struct ActType;
+template <> struct ActType<float> {
+    static constexpr float kTop = FLT_MAX;
+    static __device__ __forceinline__ float load(float v) { return v; }
+    static __device__ __forceinline__ float store(float v) { return v; }
+};
+template <> struct ActType<__half> {
+    static constexpr float kTop = 65504.0f;
+    static __device__ __forceinline__ float load(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ __half store(float v) { return __float2half_rn(v); }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+};
+template <> struct ActType<__nv_bfloat16> {
+    static constexpr float kTop = 3.38953138925153547590470800371487866880e+38f;
+    static __device__ __forceinline__ float load(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ __nv_bfloat16 store(float v) { return __float2bfloat16_rn(v); }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t w) {
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+    }
+};
+
+// ---- gate functions: f(g), and f'(g) ---------------------------------------------------------------------------
+// All in fp32.  The fast exponential and divide are off by some 2^-21 of the value, far below the 2^-9 (bf16) or
+// 2^-12 (fp16) of the rounding that follows.  The error-function and tanh forms are written so that nothing cancels
+// for large negative g: erfc instead of 1 + erf, and (1 + tanh z) / 2 as the logistic function of 2 z.
+__device__ __forceinline__ float gate_logistic(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+
+constexpr float kSqrtHalf = 0.70710678118654752440f;
+constexpr float kInvSqrt2Pi = 0.39894228040143267794f;
+constexpr float kTanhA = 0.79788456080286535588f;               // sqrt(2 / pi)
+constexpr float kTanhB = 0.044715f;
+
+template <int ACT>
+__device__ __forceinline__ float gate_value(float g) {
+    if constexpr (ACT == TB200_ACT_SILU) {
+        return g * gate_logistic(g);
+    } else if constexpr (ACT == TB200_ACT_GELU) {
+        return 0.5f * g * erfcf(-g * kSqrtHalf);
+    } else if constexpr (ACT == TB200_ACT_GELU_TANH) {
+        return g * gate_logistic(2.0f * kTanhA * (g + kTanhB * g * g * g));
+    } else {
+        return g <= 0.0f ? 0.0f : g;                            // NaN stays NaN
+    }
+}
+// f(g) and f'(g) together
+template <int ACT>
+__device__ __forceinline__ float2 gate_both(float g) {
+    if constexpr (ACT == TB200_ACT_SILU) {
+        const float s = gate_logistic(g);
+        return make_float2(g * s, s * (1.0f + g * (1.0f - s)));
+    } else if constexpr (ACT == TB200_ACT_GELU) {
+        const float p = 0.5f * erfcf(-g * kSqrtHalf);
+        return make_float2(g * p, p + g * kInvSqrt2Pi * __expf(-0.5f * g * g));
+    } else if constexpr (ACT == TB200_ACT_GELU_TANH) {
+        const float s = gate_logistic(2.0f * kTanhA * (g + kTanhB * g * g * g));
+        return make_float2(g * s, s + 2.0f * g * s * (1.0f - s) * kTanhA * (1.0f + 3.0f * kTanhB * g * g));
+    } else {
+        return make_float2(g <= 0.0f ? 0.0f : g, g > 0.0f ? 1.0f : 0.0f);
+    }
+}
+#endif  // __CUDACC__
+
+// ---- launchers shared between the files of the feed-forward block ----------------------------------------------
+// The products of the backward pass's two intermediates: dg = dh * u * f'(g), du = dh * f(g), row pitch ldg.
+int launch_gated_act_bwd(const void* dh, const void* gq, const float* gs, const void* uq, const float* us, void* dg, void* du,
+                         int64_t m, int64_t f, int64_t ldg, int act, int dtype, cudaStream_t st);
+int launch_act_restore(const void* q, const float* scales, void* out, int dtype, int64_t rows, int64_t cols, cudaStream_t st);
+
+}  // namespace tb200

@@ -219,6 +219,118 @@ void quantize_int4_group(const torch::Tensor& x, torch::Tensor& wp, torch::Tenso
              "tb200_quantize_int4_group");
 }
 
+// ---- gated feed-forward block with 8-bit activation checkpoints ----
+void check_same_device(const torch::Tensor& t, const char* name, const torch::Tensor& first) {
+    TORCH_CHECK(t.is_cuda() && t.device() == first.device(), name, " must be on ", first.device().str(), ", is on ", t.device().str());
+}
+// codes [rows, cols] and scales [rows, ceil(cols / 128)] of one activation
+void check_codes(const torch::Tensor& q, const torch::Tensor& s, const char* name, int64_t rows, int64_t cols, const torch::Tensor& first) {
+    check_cuda(q, name, torch::kFloat8_e4m3fn);
+    check_cuda(s, "scales", torch::kFloat32);
+    check_same_device(q, name, first);
+    check_same_device(s, "scales", first);
+    // numbers go through to_string: this object and libstdc++ each hold the stream's number formatting, and mixing them crashes
+    TORCH_CHECK(q.dim() == 2 && q.size(0) == rows && q.size(1) == cols, name, " must be [", std::to_string(rows), ", ", std::to_string(cols), "]");
+    TORCH_CHECK(s.dim() == 2 && s.size(0) == rows && s.size(1) == (cols + 127) / 128, "the scales of ", name, " must be [", std::to_string(rows),
+                ", ", std::to_string((cols + 127) / 128), "]");
+}
+void check_rows(const torch::Tensor& t, const char* name) {
+    TORCH_CHECK(t.is_cuda() && t.dim() == 2, name, " must be a CUDA matrix");
+    TORCH_CHECK(t.size(1) <= 1 || t.stride(1) == 1, name, " must have unit column stride");
+}
+
+void act_checkpoint_fp8(const torch::Tensor& x, torch::Tensor& q, torch::Tensor& scales) {
+    check_rows(x, "x");
+    check_codes(q, scales, "q", x.size(0), x.size(1), x);
+    c10::cuda::CUDAGuard guard(x.device());
+    check_rc(tb200_act_checkpoint_fp8(x.data_ptr(), q.data_ptr(), scales.data_ptr<float>(), x.size(0), x.size(1), x.stride(0),
+                                      dt_code(x.scalar_type()), stream_of(x)),
+             "tb200_act_checkpoint_fp8");
+}
+
+void act_restore_fp8(const torch::Tensor& q, const torch::Tensor& scales, torch::Tensor& out) {
+    TORCH_CHECK(q.is_cuda() && q.dim() == 2, "q must be a CUDA matrix");
+    check_codes(q, scales, "q", q.size(0), q.size(1), q);
+    check_same_device(out, "out", q);
+    TORCH_CHECK(out.is_contiguous() && out.sizes() == q.sizes(), "out must be contiguous and match q's shape");
+    c10::cuda::CUDAGuard guard(q.device());
+    check_rc(tb200_act_restore_fp8(q.data_ptr(), scales.data_ptr<float>(), out.data_ptr(), q.size(0), q.size(1), dt_code(out.scalar_type()),
+                                   stream_of(q)),
+             "tb200_act_restore_fp8");
+}
+
+// x [m, k], wg and wu [f, k]; returns the dtype code
+int check_block(const torch::Tensor& first, const torch::Tensor& wg, const torch::Tensor& wu) {
+    const auto dt = wg.scalar_type();
+    check_cuda(wg, "wg", dt);
+    check_cuda(wu, "wu", dt);
+    check_same_device(wg, "wg", first);
+    check_same_device(wu, "wu", first);
+    TORCH_CHECK(wg.dim() == 2 && wu.sizes() == wg.sizes(), "wg and wu must be [f, k]");
+    return dt_code(dt);
+}
+
+void ffn_gated(const torch::Tensor& x, const torch::Tensor& wg, const torch::Tensor& wu, torch::Tensor& h, int64_t act,
+               const c10::optional<torch::Tensor>& gq, const c10::optional<torch::Tensor>& gs, const c10::optional<torch::Tensor>& uq,
+               const c10::optional<torch::Tensor>& us) {
+    check_rows(x, "x");
+    const int dt = check_block(x, wg, wu);
+    TORCH_CHECK(x.scalar_type() == wg.scalar_type(), "x has dtype ", x.scalar_type(), ", expected the weights' ", wg.scalar_type());
+    const int64_t m = x.size(0), k = x.size(1), f = wg.size(0);
+    TORCH_CHECK(wg.size(1) == k, "x [m,k], wg [f,k]");
+    check_cuda(h, "h", wg.scalar_type());
+    check_same_device(h, "h", x);
+    TORCH_CHECK(h.dim() == 2 && h.size(0) == m && h.size(1) == f, "h must be [m, f]");
+    const int given = gq.has_value() + gs.has_value() + uq.has_value() + us.has_value();
+    TORCH_CHECK(given == 0 || given == 4, "gq, gs, uq, us are given together or not at all");
+    if (given) {
+        check_codes(*gq, *gs, "gq", m, f, x);
+        check_codes(*uq, *us, "uq", m, f, x);
+    }
+    c10::cuda::CUDAGuard guard(x.device());
+    check_rc(tb200_ffn_gated(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), h.data_ptr(), given ? gq->data_ptr() : nullptr,
+                             given ? gs->data_ptr<float>() : nullptr, given ? uq->data_ptr() : nullptr, given ? us->data_ptr<float>() : nullptr,
+                             m, f, k, x.stride(0), static_cast<int>(act), dt, stream_of(x)),
+             "tb200_ffn_gated");
+}
+
+int64_t ffn_gated_bwd_workspace_bytes(int64_t m, int64_t f, int64_t k, bool x_codes) {
+    return static_cast<int64_t>(tb200_ffn_gated_bwd_workspace_bytes(m, f, k, x_codes ? 1 : 0));
+}
+
+void ffn_gated_bwd(const torch::Tensor& dh, const torch::Tensor& wg, const torch::Tensor& wu, const torch::Tensor& x,
+                   const c10::optional<torch::Tensor>& xs, const torch::Tensor& gq, const torch::Tensor& gs, const torch::Tensor& uq,
+                   const torch::Tensor& us, torch::Tensor& dx, torch::Tensor& dwg, torch::Tensor& dwu, int64_t act, torch::Tensor& workspace) {
+    TORCH_CHECK(dh.is_cuda() && dh.dim() == 2, "dh must be a CUDA matrix");
+    const int dt = check_block(dh, wg, wu);
+    const int64_t m = dh.size(0), f = wg.size(0), k = wg.size(1);
+    check_cuda(dh, "dh", wg.scalar_type());
+    TORCH_CHECK(dh.size(1) == f, "dh [m,f], wg [f,k]");
+    check_codes(gq, gs, "gq", m, f, dh);
+    check_codes(uq, us, "uq", m, f, dh);
+    if (xs.has_value()) {
+        check_codes(x, *xs, "x", m, k, dh);
+    } else {
+        check_rows(x, "x");
+        check_same_device(x, "x", dh);
+        TORCH_CHECK(x.scalar_type() == wg.scalar_type(), "x has dtype ", x.scalar_type(), ", expected the weights' ", wg.scalar_type(), ", or e4m3 codes with scales");
+        TORCH_CHECK(x.size(0) == m && x.size(1) == k, "x must be [m, k]");
+    }
+    for (const torch::Tensor* t : {&dx, &dwg, &dwu, &workspace}) check_same_device(*t, "outputs and workspace", dh);
+    check_cuda(dx, "dx", wg.scalar_type());
+    check_cuda(dwg, "dwg", wg.scalar_type());
+    check_cuda(dwu, "dwu", wg.scalar_type());
+    TORCH_CHECK(dx.dim() == 2 && dx.size(0) == m && dx.size(1) == k, "dx must be [m, k]");
+    TORCH_CHECK(dwg.sizes() == wg.sizes() && dwu.sizes() == wg.sizes(), "dwg and dwu must be [f, k]");
+    TORCH_CHECK(workspace.is_contiguous(), "workspace must be contiguous");
+    c10::cuda::CUDAGuard guard(dh.device());
+    check_rc(tb200_ffn_gated_bwd(dh.data_ptr(), wg.data_ptr(), wu.data_ptr(), x.data_ptr(), xs.has_value() ? xs->data_ptr<float>() : nullptr,
+                                 gq.data_ptr(), gs.data_ptr<float>(), uq.data_ptr(), us.data_ptr<float>(), dx.data_ptr(), dwg.data_ptr(),
+                                 dwu.data_ptr(), m, f, k, x.stride(0), static_cast<int>(act), dt, workspace.data_ptr(),
+                                 static_cast<size_t>(workspace.numel()) * workspace.element_size(), stream_of(dh)),
+             "tb200_ffn_gated_bwd");
+}
+
 py::tuple device_status() {
     int code = 0, detail = 0;
     check_rc(tb200_device_status(&code, &detail), "tb200_device_status");
@@ -247,6 +359,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("matmul_int8_packed2", &matmul_int8_packed2);
     m.def("matmul_plain", &matmul_plain);
     m.def("quantize_int4_group", &quantize_int4_group);
+    m.def("act_checkpoint_fp8", &act_checkpoint_fp8);
+    m.def("act_restore_fp8", &act_restore_fp8);
+    m.def("ffn_gated", &ffn_gated);
+    m.def("ffn_gated_bwd_workspace_bytes", &ffn_gated_bwd_workspace_bytes);
+    m.def("ffn_gated_bwd", &ffn_gated_bwd);
     m.def("device_status", &device_status);
     m.def("clear_device_status", &clear_device_status);
 }

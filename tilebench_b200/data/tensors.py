@@ -197,7 +197,86 @@ def generate_matmul_fp32_fp16_fp8_inputs(M, N, K, dtype=torch.float32, device=DE
     return (a.to(device), b.to(device))
 
 
+# ---- gated feed-forward block with 8-bit activation checkpoints ----------------------------------
+
+ACT_BLOCK = 128
+
+
+def checkpoint_fp8(x: torch.Tensor):
+    """8-bit form of a [rows, cols] activation: e4m3 codes and one power-of-two fp32 scale per 1 x 128 block of a
+    row (the last block may be short).  The scale is the smallest 2^e, e >= -126, with amax <= 448 * 2^e, 1 for a
+    block without a non-zero finite value; infinities and NaN are stored as NaN and do not enter amax."""
+    rows, cols = x.shape
+    blocks = -(-cols // ACT_BLOCK)
+    xb = torch.nn.functional.pad(x.to(torch.float32), (0, blocks * ACT_BLOCK - cols)).view(rows, blocks, ACT_BLOCK)
+    amax = torch.where(torch.isfinite(xb), xb.abs(), torch.zeros_like(xb)).amax(dim=2)
+    part, power = torch.frexp(amax)                                   # amax = part * 2^power, 448 = 0.875 * 2^9
+    e = (power + (part > 0.875).to(power.dtype) - 9).clamp(min=-126)
+    e = torch.where(amax > 0, e, torch.zeros_like(e)).to(torch.int32)
+    scale, inverse = ((e + 127) << 23).view(torch.float32), ((127 - e) << 23).view(torch.float32)
+    codes = (xb * inverse[:, :, None]).to(torch.float8_e4m3fn).view(rows, blocks * ACT_BLOCK)[:, :cols]
+    return codes.contiguous(), scale
+
+
+def restore_fp8(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """code * scale in `dtype`; a product beyond the type's largest finite value becomes that value."""
+    y = codes.to(torch.float32) * scale.repeat_interleave(ACT_BLOCK, dim=1)[:, :codes.shape[1]]
+    top = torch.finfo(dtype).max
+    return y.clamp(-top, top).to(dtype)
+
+
+def gate(g: torch.Tensor, act: str):
+    """f(g) and f'(g) of the gated feed-forward block's gate."""
+    if act == "silu":
+        s = torch.sigmoid(g)
+        return g * s, s * (1 + g * (1 - s))
+    if act == "gelu":
+        p = 0.5 * torch.erfc(-g * math.sqrt(0.5))
+        return g * p, p + g * torch.exp(-0.5 * g * g) / math.sqrt(2 * math.pi)
+    if act == "gelu_tanh":
+        s = torch.sigmoid(2 * math.sqrt(2 / math.pi) * (g + 0.044715 * g ** 3))
+        return g * s, s + 2 * g * s * (1 - s) * math.sqrt(2 / math.pi) * (1 + 3 * 0.044715 * g ** 2)
+    if act == "relu":
+        return g.clamp(min=0), (g > 0).to(g.dtype)
+    raise ValueError(f"unknown activation {act!r}; choose from silu, gelu, gelu_tanh, relu")
+
+
+def generate_act_checkpoint_fp8_inputs(rows, cols, dtype=torch.bfloat16, device=DEFAULT_DEVICE, seed=SEED0 + 11000, **kwargs):
+    """Standard normal rows of very different size (log-normal factor), with some channels 30 times larger."""
+    g = _gen(seed)
+    x = torch.randn(rows, cols, generator=g) * torch.exp(torch.randn(rows, 1, generator=g))
+    x[:, ::257] *= 30
+    return (x.to(dtype).to(device),)
+
+
+def generate_act_restore_fp8_inputs(rows, cols, dtype=torch.bfloat16, device=DEFAULT_DEVICE, seed=SEED0 + 12000, **kwargs):
+    (x,) = generate_act_checkpoint_fp8_inputs(rows, cols, dtype=dtype, device="cpu", seed=seed)
+    q, s = checkpoint_fp8(x)
+    return (q.to(device), s.to(device), dtype)
+
+
+def generate_ffn_gated_inputs(M, K, F, ACT="silu", dtype=torch.bfloat16, device=DEFAULT_DEVICE, seed=SEED0 + 13000, **kwargs):
+    """x standard normal, weights scaled by K**-0.5 so that both projections stay O(1)."""
+    g = _gen(seed)
+    x = torch.randn(M, K, generator=g).to(dtype)
+    wg, wu = ((torch.randn(F, K, generator=g) * K ** -0.5).to(dtype) for _ in range(2))
+    return (x.to(device), wg.to(device), wu.to(device), ACT)
+
+
+def generate_ffn_gated_bwd_inputs(M, K, F, ACT="silu", dtype=torch.bfloat16, device=DEFAULT_DEVICE, seed=SEED0 + 14000, **kwargs):
+    """dh scaled by M**-0.5 so that the weights' gradients stay O(1); x, g and u in 8 bits."""
+    x, wg, wu, act = generate_ffn_gated_inputs(M, K, F, ACT, dtype=dtype, device="cpu", seed=seed)
+    g = _gen(seed + 1)
+    dh = (torch.randn(M, F, generator=g) * max(M, 1) ** -0.5).to(dtype)
+    held = [t for _ in range(2) for t in checkpoint_fp8(torch.randn(M, F, generator=g))]
+    return (dh.to(device), wg.to(device), wu.to(device), *(t.to(device) for t in (*checkpoint_fp8(x), *held)), act)
+
+
 GENERATORS = {
+    "act_checkpoint_fp8": generate_act_checkpoint_fp8_inputs,
+    "act_restore_fp8": generate_act_restore_fp8_inputs,
+    "ffn_gated": generate_ffn_gated_inputs,
+    "ffn_gated_bwd": generate_ffn_gated_bwd_inputs,
     "dequant_int4_group": generate_dequant_int4_group_inputs,
     "dequant_int8_channel": generate_dequant_int8_channel_inputs,
     "gemm_w4a16": generate_gemm_w4a16_inputs,
@@ -238,6 +317,10 @@ def infer_problem_size(operator_name, params):
         return int(p["N"]) * int(p["K"])
     if operator_name == "weight_dequant":
         return int(p["M"]) * int(p.get("N") or p["M"])
+    if operator_name in ("act_checkpoint_fp8", "act_restore_fp8"):
+        return int(p["rows"]) * int(p["cols"])
+    if operator_name in ("ffn_gated", "ffn_gated_bwd"):
+        return int(p["M"]) * int(p["F"])
     if operator_name in ("matmul_int8", "matmul_fp32_fp16_fp8"):
         return 2 * int(p["M"]) * int(p["N"]) * int(p["K"])       # the reference sizes GEMMs by FLOPs (tensors.py:703-704)
     return 1

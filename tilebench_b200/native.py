@@ -24,9 +24,13 @@ ABI_SYMBOLS = (
     "tb200_gemm_w4a16_static_scratch_bytes", "tb200_gemm_w4a16_static", "tb200_gemm_w4a16_gather",
     "tb200_quantize_fp8_block", "tb200_matmul_int8_packed2", "tb200_matmul_plain", "tb200_quantize_int4_group",
     "tb200_allgather_cols", "tb200_selftest_bounded_wait",
+    "tb200_act_checkpoint_fp8", "tb200_act_restore_fp8", "tb200_ffn_gated", "tb200_ffn_gated_bwd_workspace_bytes",
+    "tb200_ffn_gated_bwd",
 )
 
 DT_F32, DT_F16, DT_BF16, DT_F8E4M3 = 0, 1, 2, 3
+#: Gate functions of the gated feed-forward block by name -> TB200_ACT_* code.
+ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
 
 _ext = None
 _capi = None
@@ -103,6 +107,16 @@ def capi() -> ctypes.CDLL:
     lib.tb200_allgather_cols.restype = ci
     lib.tb200_selftest_bounded_wait.argtypes = [i64, vp]
     lib.tb200_selftest_bounded_wait.restype = ci
+    lib.tb200_act_checkpoint_fp8.argtypes = [vp, vp, vp, i64, i64, i64, ci, vp]
+    lib.tb200_act_checkpoint_fp8.restype = ci
+    lib.tb200_act_restore_fp8.argtypes = [vp, vp, vp, i64, i64, ci, vp]
+    lib.tb200_act_restore_fp8.restype = ci
+    lib.tb200_ffn_gated.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, ci, ci, vp]
+    lib.tb200_ffn_gated.restype = ci
+    lib.tb200_ffn_gated_bwd_workspace_bytes.argtypes = [i64, i64, i64, ci]
+    lib.tb200_ffn_gated_bwd_workspace_bytes.restype = sz
+    lib.tb200_ffn_gated_bwd.argtypes = [vp] * 12 + [i64, i64, i64, i64, ci, ci, vp, sz, vp]
+    lib.tb200_ffn_gated_bwd.restype = ci
     lib.tb200_device_status.argtypes = [ctypes.POINTER(ci), ctypes.POINTER(ci)]
     lib.tb200_clear_device_status.argtypes = []
     for name in ("tb200_dequant_int4_group", "tb200_dequant_int8_rowwise", "tb200_weight_dequant_block",
@@ -115,6 +129,14 @@ def capi() -> ctypes.CDLL:
 
 def last_error() -> str:
     return capi().tb200_last_error().decode()
+
+
+def activation(name: str) -> int:
+    """The C ABI's code of a gate function; ValueError for an unknown name."""
+    try:
+        return ACTIVATIONS[name]
+    except KeyError:
+        raise ValueError(f"unknown activation {name!r}; choose from {', '.join(ACTIVATIONS)}") from None
 
 
 def require_b200() -> None:

@@ -25,7 +25,7 @@ import yaml
 from tilebench_b200 import provenance
 from tilebench_b200.backends import MODES, backend_tag, parse_backends
 from tilebench_b200.core.metrics import compute_derived, load_peak_config
-from tilebench_b200.paths import list_operators, operator_config, results_csv_dir, results_logs_dir
+from tilebench_b200.paths import list_layer_operators, list_operators, operator_config, results_csv_dir, results_logs_dir
 
 _BACKEND_LABEL = {"cuda": "CUDA"}
 _SPEEDUP_CODE = {"cuda": "cu"}
@@ -117,7 +117,7 @@ def write_outputs(gpu: str, operator: str, mode: str, active, results, prov, out
 def main(argv=None) -> int:
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     ap.add_argument("--gpu", default="B200", help="result namespace results/<gpu>/ and peak table data/peak_performance/<gpu>.json")
-    ap.add_argument("--operator", required=True, choices=list_operators())
+    ap.add_argument("--operator", required=True, choices=list_operators() + list_layer_operators())
     ap.add_argument("--tile-language", default=None, help="comma-separated backends (cuda); torch always runs")
     ap.add_argument("--warmup", type=int)
     ap.add_argument("--repeat", type=int)
