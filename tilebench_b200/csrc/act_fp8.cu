@@ -3,249 +3,529 @@
 // by HBM: saving moves size + 1 bytes per element, restoring 1 + size, the backward step 4 in and 4 out.
 #include "act_fp8.cuh"
 
+#include <limits.h>
+
 namespace tb200 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kSeg = 1024;                      // columns that a warp of the staged kernels takes at a time
-constexpr int kSegBlocks = kSeg / kActBlock;
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* __restrict__ p, float (&v)[8]) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-        const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+__device__ __forceinline__ void load32(const void* p, uint32_t (&r)[8]) {        // 32 bytes, read once
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "l"(p));
+}
+__device__ __forceinline__ void store32(void* p, const uint32_t (&r)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+                 "r"(r[6]), "r"(r[7]) : "memory");
+}
+
+// N words of memory <-> the 4 N / sizeof(T) numbers that they hold
+template <typename T, int N>
+__device__ __forceinline__ void numbers(const uint32_t (&w)[N], float (&v)[4 * N / sizeof(T)]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < N; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            v[i] = __uint_as_float(w[i]);
+        } else {
             const float2 f = ActType<T>::unpack(w[i]);
             v[2 * i] = f.x;
             v[2 * i + 1] = f.y;
         }
     }
 }
-
-// Saving, rows on 16-byte boundaries.  Half a warp per block, 8 elements per lane; U pairs of blocks per warp are in
-// flight at once.  A short last block is handled by leaving lanes out (cols is a multiple of 8).
-template <typename T, int U>
-__global__ void __launch_bounds__(kThreads) k_save(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales,
-                                                   uint32_t total, uint32_t nblk, int64_t cols, int64_t ldx) {
-    const int lane = threadIdx.x & 31, sub = lane & 15;
-    const uint32_t warps = gridDim.x * (kThreads / 32);
-    const uint32_t groups = (total + 2 * U - 1) / (2 * U);
-    for (uint32_t g = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); g < groups; g += warps) {
-        float v[U][8];
-        int64_t at[U];                          // offset of the lane's codes, -1 where it has none
+template <typename T, int N>
+__device__ __forceinline__ void words(const float (&v)[4 * N / sizeof(T)], uint32_t (&w)[N]) {
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-            const uint32_t blk = g * (2 * U) + 2 * j + (lane >> 4);
-            const uint32_t row = blk / nblk, col = (blk - row * nblk) * kActBlock + sub * 8;
-            at[j] = blk < total && col < cols ? static_cast<int64_t>(row) * cols + col : -1;
-            if (at[j] >= 0) {
-                load8(x + static_cast<int64_t>(row) * ldx + col, v[j]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[j][i] = 0.0f;
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-            float amax = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) amax = fmaxf(amax, act_size(v[j][i]));
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-            const float2 s = act_scale(amax);
-            if (at[j] >= 0) {
-                uint2 o;
-                o.x = act_codes4(v[j][0], v[j][1], v[j][2], v[j][3], s.y);
-                o.y = act_codes4(v[j][4], v[j][5], v[j][6], v[j][7], s.y);
-                *reinterpret_cast<uint2*>(q + at[j]) = o;
-                if (sub == 0) scales[g * (2 * U) + 2 * j + (lane >> 4)] = s.x;
-            }
-        }
+    for (int i = 0; i < N; ++i) {
+        if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v[i]);
+        else w[i] = ActType<T>::pack(v[2 * i], v[2 * i + 1]);
     }
 }
-
-// Moves n elements between global memory at any alignment and a shared buffer that has the same address modulo 16:
-// single elements up to the first 16-byte boundary and behind the last one, 16-byte pieces between.
-template <typename T>
-__device__ __forceinline__ T* same_offset(uint8_t* buf, const T* global) { return reinterpret_cast<T*>(buf + (reinterpret_cast<uintptr_t>(global) & 15)); }
-template <typename T, typename Dst, typename Src>
-__device__ __forceinline__ void copy_any(Dst* dst, const Src* src, int n, int lane) {
-    constexpr int V = 16 / sizeof(T);
-    const int head = min(n, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / sizeof(T)));
-    const int vecs = (n - head) / V, tail0 = head + vecs * V;
-    if (lane < head) dst[lane] = src[lane];
-    for (int i = lane; i < vecs; i += 32) *reinterpret_cast<uint4*>(dst + head + i * V) = *reinterpret_cast<const uint4*>(src + head + i * V);
-    if (tail0 + lane < n) dst[tail0 + lane] = src[tail0 + lane];
-}
-
-// Saving, any width, stride and alignment: a warp stages up to 1024 columns of a row in shared memory, so that global
-// memory sees 16-byte accesses although a row may begin at any byte.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) k_save_any(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales,
-                                                       int64_t segments, uint32_t nseg, uint32_t nblk, int64_t cols, int64_t ldx) {
-    __shared__ __align__(16) uint8_t xs[kThreads / 32][kSeg * sizeof(T) + 16];
-    __shared__ __align__(16) uint8_t qs[kThreads / 32][kSeg + 16];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int64_t s = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + warp; s < segments; s += static_cast<int64_t>(gridDim.x) * (kThreads / 32)) {
-        const int64_t row = s / nseg;
-        const int64_t col = (s - row * nseg) * kSeg;
-        const int n = static_cast<int>(min(static_cast<int64_t>(kSeg), cols - col));
-        const T* src = x + row * ldx + col;
-        uint8_t* dst = q + row * cols + col;
-        T* xb = same_offset(xs[warp], src);
-        uint8_t* qb = same_offset(qs[warp], dst);
-        copy_any<T>(xb, src, n, lane);
-        __syncwarp();
-#pragma unroll 2
-        for (int b = 0; b * kActBlock < n; ++b) {
-            float v[4], amax = 0.0f;
+// The scale of a block whose E numbers per lane lie in 128 / E neighbouring lanes, and the lane's codes.
+template <int E>
+__device__ __forceinline__ float encode(const float (&v)[E], uint32_t (&codes)[E / 4]) {
+    float amax = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int i = b * kActBlock + j * 32 + lane;
-                v[j] = i < n ? ActType<T>::load(xb[i]) : 0.0f;
-                amax = fmaxf(amax, act_size(v[j]));
-            }
+    for (int i = 0; i < E; ++i) amax = fmaxf(amax, fabsf(v[i]));
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-            const float2 sc = act_scale(amax);
+    for (int o = kActBlock / E / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const bool infinite = amax > FLT_MAX;                        // the same in all lanes of the block
+    if (__any_sync(0xffffffffu, infinite)) {
+        float size = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int i = b * kActBlock + j * 32 + lane;
-                if (i < n) qb[i] = static_cast<uint8_t>(act_codes2(act_scaled(v[j], sc.y), 0.0f) & 0xFFu);
-            }
-            if (lane == 0) scales[row * nblk + col / kActBlock + b] = sc.x;
-        }
-        __syncwarp();
-        copy_any<uint8_t>(dst, qb, n, lane);
-        __syncwarp();
+        for (int i = 0; i < E; ++i) size = fmaxf(size, act_size(v[i]));
+#pragma unroll
+        for (int o = kActBlock / E / 2; o > 0; o >>= 1) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, o));
+        amax = size;
     }
-}
-
-// 16 codes -> 16 values of T, 16-byte stores
-template <typename T>
-__device__ __forceinline__ void restore16(T* __restrict__ out, const uint4& c, float s) {
-    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-    float v[16];
+    const float2 s = act_scale(amax);
+    if (infinite) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 a = act_values2(w[i] & 0xFFFFu), b = act_values2(w[i] >> 16);
-        v[4 * i] = act_restored(a.x, s, ActType<T>::kTop);
-        v[4 * i + 1] = act_restored(a.y, s, ActType<T>::kTop);
-        v[4 * i + 2] = act_restored(b.x, s, ActType<T>::kTop);
-        v[4 * i + 3] = act_restored(b.y, s, ActType<T>::kTop);
-    }
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(out)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        for (int i = 0; i < E / 4; ++i) codes[i] = act_codes4_checked(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], s.y);
     } else {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            reinterpret_cast<uint4*>(out)[i] = make_uint4(ActType<T>::pack(v[8 * i], v[8 * i + 1]), ActType<T>::pack(v[8 * i + 2], v[8 * i + 3]),
-                                                          ActType<T>::pack(v[8 * i + 4], v[8 * i + 5]), ActType<T>::pack(v[8 * i + 6], v[8 * i + 7]));
+        for (int i = 0; i < E / 4; ++i) codes[i] = act_codes4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], s.y);
+    }
+    return s.x;
+}
+template <int E>
+__device__ __forceinline__ void decode(const uint32_t (&codes)[E / 4], float s, float top, float (&v)[E]) {
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i) {
+        const float2 a = act_values2(codes[i] & 0xFFFFu), b = act_values2(codes[i] >> 16);
+        v[4 * i] = a.x * s;
+        v[4 * i + 1] = a.y * s;
+        v[4 * i + 2] = b.x * s;
+        v[4 * i + 3] = b.y * s;
+    }
+    if (act_may_exceed(s, top)) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] = act_held(v[i], top);
     }
 }
 
-// Restoring, widths that are multiples of 16: 16 codes per lane, U independent loads in flight.
-template <typename T, int U>
-__global__ void __launch_bounds__(kThreads) k_restore(const uint4* __restrict__ q, const float* __restrict__ scales, T* __restrict__ out,
-                                                      int64_t total, uint32_t per_row, uint32_t nblk) {
-    const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
-    for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i0 < total; i0 += U * step) {
-        uint4 c[U];
-        float s[U];
+// ---- rows on 32-byte boundaries: one 32-byte piece of x per lane and access ------------------------------------
+
+// Saving.  E numbers (32 bytes) per lane, 128 / E lanes per block, U pieces in flight.  per_row: pieces per row; a row
+// ends inside a block where cols is not a multiple of 128 (lanes past it hold zeros).  FLAT: rows are whole blocks and
+// adjacent, so the piece's number is its place.
+template <typename T, int U, bool FLAT>
+__global__ void __launch_bounds__(kThreads) k_save(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales,
+                                                   uint32_t blocks, uint32_t nblk, int64_t cols, int64_t ldx) {
+    constexpr int E = 32 / sizeof(T), kLanes = kActBlock / E;
+    const uint64_t total = static_cast<uint64_t>(blocks) * kLanes, step = static_cast<uint64_t>(gridDim.x) * kThreads;
+    for (uint64_t i0 = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x; i0 - (threadIdx.x & 31) < total; i0 += U * step) {
+        uint32_t w[U][8];
+        int64_t at[U];                                           // place of the lane's codes, -1 where it has none
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            const int64_t i = i0 + j * step;
+            const uint64_t i = i0 + j * step;
+            at[j] = -1;
             if (i < total) {
-                c[j] = __ldcs(q + i);
-                const int64_t row = i / per_row;
-                s[j] = __ldg(scales + row * nblk + static_cast<uint32_t>(i - row * per_row) / 8);
+                if constexpr (FLAT) {
+                    at[j] = static_cast<int64_t>(i) * E;
+                    load32(x + at[j], w[j]);
+                } else {
+                    const uint32_t blk = static_cast<uint32_t>(i / kLanes), row = blk / nblk;
+                    const int64_t col = static_cast<int64_t>(blk - row * nblk) * kActBlock + (i % kLanes) * E;
+                    if (col < cols) {
+                        at[j] = static_cast<int64_t>(row) * cols + col;
+                        load32(x + static_cast<int64_t>(row) * ldx + col, w[j]);
+                    }
+                }
+            }
+            if (at[j] < 0) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[j][e] = 0;
             }
         }
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            const int64_t i = i0 + j * step;
-            if (i < total) restore16(out + 16 * i, c[j], s[j]);
+            const uint64_t i = i0 + j * step;
+            float v[E];
+            uint32_t c[E / 4];
+            numbers<T, 8>(w[j], v);
+            const float s = encode<E>(v, c);
+            if (at[j] >= 0) {
+                if constexpr (E == 16) *reinterpret_cast<uint4*>(q + at[j]) = make_uint4(c[0], c[1], c[2], c[3]);
+                else *reinterpret_cast<uint2*>(q + at[j]) = make_uint2(c[0], c[1]);
+                if (i % kLanes == 0) scales[i / kLanes] = s;
+            }
         }
     }
 }
 
+// Restoring: E codes per lane make one 32-byte piece.
+template <typename T, int U, bool FLAT>
+__global__ void __launch_bounds__(kThreads) k_restore(const uint8_t* __restrict__ q, const float* __restrict__ scales, T* __restrict__ out,
+                                                      uint32_t blocks, uint32_t nblk, int64_t cols) {
+    constexpr int E = 32 / sizeof(T), kLanes = kActBlock / E;
+    const uint64_t total = static_cast<uint64_t>(blocks) * kLanes, step = static_cast<uint64_t>(gridDim.x) * kThreads;
+    for (uint64_t i0 = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x; i0 < total; i0 += U * step) {
+        uint32_t c[U][E / 4];
+        float s[U];
+        int64_t at[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const uint64_t i = i0 + j * step;
+            at[j] = -1;
+            if (i < total) {
+                const uint32_t blk = static_cast<uint32_t>(i / kLanes);
+                if constexpr (FLAT) {
+                    at[j] = static_cast<int64_t>(i) * E;
+                } else {
+                    const uint32_t row = blk / nblk;
+                    const int64_t col = static_cast<int64_t>(blk - row * nblk) * kActBlock + (i % kLanes) * E;
+                    if (col < cols) at[j] = static_cast<int64_t>(row) * cols + col;
+                }
+                if (at[j] >= 0) {
+                    if constexpr (E == 16) {
+                        const uint4 p = __ldcs(reinterpret_cast<const uint4*>(q + at[j]));
+                        c[j][0] = p.x; c[j][1] = p.y; c[j][2] = p.z; c[j][3] = p.w;
+                    } else {
+                        const uint2 p = __ldcs(reinterpret_cast<const uint2*>(q + at[j]));
+                        c[j][0] = p.x; c[j][1] = p.y;
+                    }
+                    s[j] = __ldg(scales + blk);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            if (at[j] >= 0) {
+                float v[E];
+                uint32_t w[8];
+                decode<E>(c[j], s[j], ActType<T>::kTop, v);
+                words<T, 8>(v, w);
+                store32(out + at[j], w);
+            }
+        }
+    }
+}
+
+// ---- any width, stride and alignment ---------------------------------------------------------------------------
+// A warp walks a span of one row in parts of 32 pieces of 4 N bytes, piece l in lane l.  Memory is accessed in aligned
+// pieces; where the row begins at another offset, a lane's piece is a window over its own aligned piece and the next
+// lane's (loads; lane 31 takes lane 0's of the part that follows, which is already there), or an aligned piece is a window over
+// the previous lane's codes and its own (stores).  Loads that reach outside the tensor and stores that reach outside
+// the span are made byte by byte.
+
+// The piece at byte `off` behind base (base + off is aligned); bytes outside [lo, hi) come as zeros.
+template <int N>
+__device__ __forceinline__ void load_piece(const uint8_t* base, int off, int lo, int hi, uint32_t (&r)[N]) {
+    if (off >= lo && off + 4 * N <= hi) {
+        if constexpr (N == 4) {
+            const uint4 v = __ldcs(reinterpret_cast<const uint4*>(base + off));
+            r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
+        } else if constexpr (N == 2) {
+            const uint2 v = __ldcs(reinterpret_cast<const uint2*>(base + off));
+            r[0] = v.x; r[1] = v.y;
+        } else {
+            r[0] = __ldcs(reinterpret_cast<const uint32_t*>(base + off));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) r[i] = 0;
+        if (off + 4 * N > lo && off < hi) {
+#pragma unroll 1
+            for (int i = max(0, lo - off); i < 4 * N && off + i < hi; ++i) {
+                const uint32_t byte = static_cast<uint32_t>(base[off + i]) << (8 * (i & 3));
+#pragma unroll
+                for (int w = 0; w < N; ++w) r[w] |= i / 4 == w ? byte : 0;
+            }
+        }
+    }
+}
+// One row's bytes [at, at + bytes) in parts, kAhead of them on the way.  The tensor is [begin, end).
+template <int N>
+struct Stream {
+    static constexpr int kAhead = 2, kPart = 32 * 4 * N;
+    const uint8_t* base;
+    int off, lo, hi, stop, mis;
+    uint32_t held[kAhead + 1][N];
+    __device__ __forceinline__ Stream(const uint8_t* at, int64_t bytes, const uint8_t* begin, const uint8_t* end, int lane) {
+        mis = static_cast<int>(reinterpret_cast<uintptr_t>(at) & (4 * N - 1));
+        base = at - mis;
+        off = lane * 4 * N;
+        lo = at - begin >= 4 * N ? 0 : max(0, mis - static_cast<int>(at - begin));
+        stop = mis + static_cast<int>(bytes);
+        hi = end - at >= bytes + 4 * N ? stop + 4 * N : mis + static_cast<int>(end - at);
+#pragma unroll
+        for (int j = 0; j <= kAhead; ++j) load(j, j);
+    }
+    __device__ __forceinline__ void load(int j, int part) {
+        const int o = off + part * kPart;
+        load_piece<N>(base, o, o < stop ? lo : INT_MAX, hi, held[j]);
+    }
+    // The lane's piece of the current part; fetches the part kAhead + 1 further on and moves on by one.
+    __device__ __forceinline__ void next(int lane, uint32_t (&r)[N]) {
+        if (mis == 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) r[i] = held[0][i];
+        } else {
+            uint32_t a[2 * N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                a[i] = held[0][i];
+                a[N + i] = __shfl_sync(0xffffffffu, lane == 0 ? held[1][i] : held[0][i], (lane + 1) & 31);
+            }
+            // words [mis / 4, mis / 4 + N], then mis % 4 bytes on
+#pragma unroll
+            for (int step = N / 2; step > 0; step >>= 1) {
+                const bool by = (mis & (4 * step)) != 0;
+#pragma unroll
+                for (int i = 0; i < N + step; ++i) a[i] = by ? a[i + step < 2 * N ? i + step : i] : a[i];
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) r[i] = __funnelshift_r(a[i], a[i + 1], (mis & 3) * 8);
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+            for (int i = 0; i < N; ++i) held[j][i] = held[j + 1][i];
+        load(kAhead, kAhead + 1);
+        off += kPart;
+    }
+};
+template <int N>
+__device__ __forceinline__ void store_piece(uint8_t* base, int off, int lo, int hi, const uint32_t (&r)[N]) {
+    if (off >= lo && off + 4 * N <= hi) {
+        if constexpr (N == 2) *reinterpret_cast<uint2*>(base + off) = make_uint2(r[0], r[1]);
+        else *reinterpret_cast<uint32_t*>(base + off) = r[0];
+    } else if (off + 4 * N > lo && off < hi) {
+#pragma unroll 1
+        for (int i = max(0, lo - off); i < 4 * N && off + i < hi; ++i)
+            base[off + i] = static_cast<uint8_t>((N == 1 || i < 4 ? r[0] : r[N - 1]) >> (8 * (i & 3)));
+    }
+}
+// The last `mis` bytes of one piece followed by the first of the next; N is 1 or 2, mis in [1, 4 N).
+template <int N>
+__device__ __forceinline__ void join_before(const uint32_t (&before)[N], const uint32_t (&r)[N], int mis, uint32_t (&out)[N]) {
+    static_assert(N == 1 || N == 2, "codes of 4 or 8 numbers");
+    const uint32_t sh = (mis & 3) * 8;
+    if constexpr (N == 1) {
+        out[0] = __funnelshift_l(before[0], r[0], sh);
+    } else {
+        const bool word = mis >= 4;
+        const uint32_t b0 = word ? before[0] : before[1], b1 = word ? before[1] : r[0], b2 = word ? r[0] : r[1];
+        out[0] = __funnelshift_l(b0, b1, sh);
+        out[1] = __funnelshift_l(b1, b2, sh);
+    }
+}
+template <typename T> struct Part {
+    static constexpr int E = 16 / sizeof(T);                     // numbers per lane
+    static constexpr int kCols = 32 * E;
+    static constexpr int kLanes = kActBlock / E;                 // lanes per block
+};
+
+// spans: warps' shares of the rows, per_row of them in a row, `width` columns each (a multiple of the part).
+template <typename T>
+__global__ void __launch_bounds__(kThreads) k_save_any(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales,
+                                                       int64_t spans, uint32_t per_row, int width, uint32_t nblk, int64_t rows, int64_t cols,
+                                                       int64_t ldx) {
+    constexpr int E = Part<T>::E, N = E / 4, kLanes = Part<T>::kLanes, kCols = Part<T>::kCols;
+    const int lane = threadIdx.x & 31;
+    const uint8_t *begin = reinterpret_cast<const uint8_t*>(x), *end = reinterpret_cast<const uint8_t*>(x + (rows - 1) * ldx + cols);
+    for (int64_t s = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); s < spans; s += static_cast<int64_t>(gridDim.x) * (kThreads / 32)) {
+        const int64_t row = s / per_row, first = (s - row * per_row) * width;
+        const int n = static_cast<int>(min(static_cast<int64_t>(width), cols - first));
+        Stream<4> in(reinterpret_cast<const uint8_t*>(x + row * ldx + first), static_cast<int64_t>(n) * sizeof(T), begin, end, lane);
+        uint8_t* const to = q + row * cols + first;
+        float* const sc = scales + row * nblk + first / kActBlock;
+        const int mis = static_cast<int>(reinterpret_cast<uintptr_t>(to) & (4 * N - 1));
+        uint32_t before[N] = {};                                 // lane 31's codes of the part before
+        int part = 0;
+#pragma unroll 1
+        for (int col = 0; col < n; col += kCols, ++part) {
+            uint32_t r[4], c[N], b[N], out[N];
+            float v[E];
+            in.next(lane, r);
+            numbers<T, 4>(r, v);
+            const int at = col + lane * E;                       // the lane's first column in the span
+            if (at + E > n) {
+#pragma unroll
+                for (int i = 0; i < E; ++i) v[i] = at + i < n ? v[i] : 0.0f;
+            }
+            const float scale = encode<E>(v, c);
+            if (lane % kLanes == 0 && at < n) sc[at / kActBlock] = scale;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                b[i] = __shfl_sync(0xffffffffu, lane == 31 ? before[i] : c[i], (lane + 31) & 31);
+                before[i] = c[i];
+            }
+            if (mis != 0) {
+                join_before<N>(b, c, mis, out);
+                store_piece<N>(to - mis, at, mis, mis + n, out);
+            } else {
+                store_piece<N>(to, at, 0, n, c);
+            }
+        }
+        if (mis != 0 && lane == 31) {                            // the last lane's codes that belong to the piece behind it
+            uint32_t zero[N] = {}, out[N];
+            join_before<N>(before, zero, mis, out);
+            store_piece<N>(to - mis, part * kCols, mis, mis + n, out);
+        }
+    }
+}
+
+// Restoring, any width of at least 16 columns, q on 16-byte and out on 32-byte boundaries: codes and numbers are both without gaps
+// between rows, so pieces of 16 (8 for fp32) are taken across the ends of rows and blocks.  At most two ends lie inside a piece (those
+// of a whole block and of a last one that is shorter than a piece); each code takes the scale of its side.
+template <typename T, int U>
+__global__ void __launch_bounds__(kThreads) k_restore_across(const uint8_t* __restrict__ q, const float* __restrict__ scales, T* __restrict__ out,
+                                                             int64_t total, uint32_t nblk, int64_t cols) {
+    constexpr int E = 32 / sizeof(T);
+    // a warp takes U * 32 neighbouring pieces at a time: their first place is divided once, the lanes' by 32-bit steps
+    constexpr int kWarpCols = U * 32 * E;
+    const int lane = threadIdx.x & 31;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / 32) * kWarpCols;
+    for (int64_t w0 = (static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5)) * kWarpCols; w0 < total; w0 += step) {
+        const int64_t row0 = w0 / cols;
+        const uint32_t col0 = static_cast<uint32_t>(w0 - row0 * cols), width = static_cast<uint32_t>(cols);
+        const float* sc = scales + row0 * nblk;
+        uint32_t c[U][E / 4];
+        float s0[U], s1[U], s2[U];
+        uint32_t cut[U], cut2[U];                                // codes from here on take s1, and s2
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int64_t at = w0 + (j * 32 + lane) * E;
+            if (at >= total) continue;
+            load_piece<E / 4>(q + at, 0, 0, static_cast<int>(min(total - at, static_cast<int64_t>(E))), c[j]);
+            uint32_t col = col0 + (j * 32 + lane) * E, row = 0;
+            if (col >= width) {
+                row = width >= kWarpCols ? 1 : col / width;      // 1: col0 < width, and the warp's share is no wider
+                col -= row * width;
+            }
+            const float* p = sc + static_cast<int64_t>(row) * nblk + col / kActBlock;
+            const uint32_t end = min(width, (col / kActBlock + 1) * kActBlock);                   // of the block
+            cut[j] = min(end - col, static_cast<uint32_t>(E));
+            cut2[j] = end < width ? min(width - col, static_cast<uint32_t>(E)) : E;
+            s0[j] = __ldg(p);                                    // scales have no gaps either
+            s1[j] = cut[j] < E && at + cut[j] < total ? __ldg(p + 1) : s0[j];
+            s2[j] = cut2[j] < E && at + cut2[j] < total ? __ldg(p + 2) : s1[j];
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int64_t at = w0 + (j * 32 + lane) * E;
+            if (at >= total) continue;
+            float v[E];
+            uint32_t w[8];
+            decode<E>(c[j], 1.0f, FLT_MAX, v);
+            if (cut[j] == E) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] *= s0[j];
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] *= e < cut[j] ? s0[j] : e < cut2[j] ? s1[j] : s2[j];
+            }
+            if (act_may_exceed(fmaxf(s0[j], fmaxf(s1[j], s2[j])), ActType<T>::kTop)) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = act_held(v[e], ActType<T>::kTop);
+            }
+            words<T, 8>(v, w);
+            if (at + E <= total) store32(out + at, w);
+            else {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (at + e < total) out[at + e] = ActType<T>::store(v[e]);
+            }
+        }
+    }
+}
+
+// Restoring at any alignment and width, one number per thread.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_restore_any(const uint8_t* __restrict__ q, const float* __restrict__ scales, T* __restrict__ out,
-                                                          int64_t segments, uint32_t nseg, uint32_t nblk, int64_t cols) {
-    __shared__ __align__(16) uint8_t ys[kThreads / 32][kSeg * sizeof(T) + 16];
-    __shared__ __align__(16) uint8_t qs[kThreads / 32][kSeg + 16];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int64_t s = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + warp; s < segments; s += static_cast<int64_t>(gridDim.x) * (kThreads / 32)) {
-        const int64_t row = s / nseg;
-        const int64_t col = (s - row * nseg) * kSeg;
-        const int n = static_cast<int>(min(static_cast<int64_t>(kSeg), cols - col));
-        const uint8_t* src = q + row * cols + col;
-        T* dst = out + row * cols + col;
-        uint8_t* qb = same_offset(qs[warp], src);
-        T* yb = same_offset(ys[warp], dst);
-        copy_any<uint8_t>(qb, src, n, lane);
-        __syncwarp();
-        for (int b = 0; b * kActBlock < n; ++b) {
-            const float sc = __ldg(scales + row * nblk + col / kActBlock + b);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int i = b * kActBlock + j * 32 + lane;
-                if (i < n) yb[i] = ActType<T>::store(act_restored(act_values2(qb[i]).x, sc, ActType<T>::kTop));
-            }
-        }
-        __syncwarp();
-        copy_any<T>(dst, yb, n, lane);
-        __syncwarp();
+                                                          int64_t total, uint32_t nblk, int64_t cols) {
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * kThreads) {
+        const int64_t row = i / cols;
+        out[i] = ActType<T>::store(act_held(act_values2(q[i]).x * scales[row * nblk + (i - row * cols) / kActBlock], ActType<T>::kTop));
     }
 }
 
-// dg = dh * u * f'(g), du = dh * f(g); 8 elements per thread, rows of multiples of 8.
+// dg = dh * u * f'(g), du = dh * f(g) for 8 numbers of a lane.
 template <typename T, int ACT>
+__device__ __forceinline__ void gated_bwd8(const uint32_t (&d)[4], const uint32_t (&cg)[2], const uint32_t (&cu)[2], float sg, float su,
+                                           uint4& dg, uint4& du) {
+    float e[8], g[8], u[8];
+    uint32_t og[4], ou[4];
+    numbers<T, 4>(d, e);
+    decode<8>(cg, sg, FLT_MAX, g);
+    decode<8>(cu, su, FLT_MAX, u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float2 a = gate_both<ACT>(g[i]);
+        g[i] = e[i] * u[i] * a.y;
+        u[i] = e[i] * a.x;
+    }
+    words<T, 4>(g, og);
+    words<T, 4>(u, ou);
+    dg = make_uint4(og[0], og[1], og[2], og[3]);
+    du = make_uint4(ou[0], ou[1], ou[2], ou[3]);
+}
+
+// Widths that are multiples of 8, 16-byte boundaries: 8 numbers per thread.
+template <typename T, int ACT, int U>
 __global__ void __launch_bounds__(kThreads) k_gated_bwd(const uint4* __restrict__ dh, const uint2* __restrict__ gq, const float* __restrict__ gs,
                                                         const uint2* __restrict__ uq, const float* __restrict__ us, uint4* __restrict__ dg,
-                                                        uint4* __restrict__ du, int64_t total, uint32_t per_row, uint32_t nblk) {
-    const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total; i += step) {
-        const int64_t row = i / per_row;
-        const int64_t blk = row * nblk + static_cast<uint32_t>(i - row * per_row) / 16;
-        const uint4 d = __ldcs(dh + i);
-        const uint2 cg = __ldcs(gq + i), cu = __ldcs(uq + i);
-        const float sg = __ldg(gs + blk), su = __ldg(us + blk);
-        const uint32_t dw[4] = {d.x, d.y, d.z, d.w};
-        uint32_t og[4], ou[4];
+                                                        uint4* __restrict__ du, uint32_t total, uint32_t per_row, uint32_t nblk) {
+    const uint32_t step = gridDim.x * kThreads;
+    for (uint64_t i0 = blockIdx.x * kThreads + threadIdx.x; i0 < total; i0 += U * step) {
+        uint4 d[U];
+        uint2 cg[U], cu[U];
+        float sg[U], su[U];
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            const uint32_t hg = (p < 2 ? cg.x : cg.y) >> (16 * (p & 1)) & 0xFFFFu, hu = (p < 2 ? cu.x : cu.y) >> (16 * (p & 1)) & 0xFFFFu;
-            const float2 g = act_values2(hg), u = act_values2(hu), e = ActType<T>::unpack(dw[p]);
-            const float2 a = gate_both<ACT>(act_restored(g.x, sg, FLT_MAX)), b = gate_both<ACT>(act_restored(g.y, sg, FLT_MAX));
-            og[p] = ActType<T>::pack(e.x * act_restored(u.x, su, FLT_MAX) * a.y, e.y * act_restored(u.y, su, FLT_MAX) * b.y);
-            ou[p] = ActType<T>::pack(e.x * a.x, e.y * b.x);
+        for (int j = 0; j < U; ++j) {
+            const uint64_t i = i0 + j * step;
+            if (i < total) {
+                const uint32_t row = static_cast<uint32_t>(i) / per_row, blk = row * nblk + (static_cast<uint32_t>(i) - row * per_row) / 16;
+                d[j] = __ldcs(dh + i);
+                cg[j] = __ldcs(gq + i);
+                cu[j] = __ldcs(uq + i);
+                sg[j] = __ldg(gs + blk);
+                su[j] = __ldg(us + blk);
+            }
         }
-        dg[i] = make_uint4(og[0], og[1], og[2], og[3]);
-        du[i] = make_uint4(ou[0], ou[1], ou[2], ou[3]);
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const uint64_t i = i0 + j * step;
+            if (i < total) {
+                const uint32_t dw[4] = {d[j].x, d[j].y, d[j].z, d[j].w}, gw[2] = {cg[j].x, cg[j].y}, uw[2] = {cu[j].x, cu[j].y};
+                uint4 a, b;
+                gated_bwd8<T, ACT>(dw, gw, uw, sg[j], su[j], a, b);
+                dg[i] = a;
+                du[i] = b;
+            }
+        }
     }
 }
 
-// The same for any width: single elements, neighbouring lanes on neighbouring columns.
+// The same for any width and alignment of dh and the codes; dg and du have rows on 16-byte boundaries, ldg >= f a multiple of 8.
 template <typename T, int ACT>
 __global__ void __launch_bounds__(kThreads) k_gated_bwd_any(const T* __restrict__ dh, const uint8_t* __restrict__ gq, const float* __restrict__ gs,
                                                             const uint8_t* __restrict__ uq, const float* __restrict__ us, T* __restrict__ dg,
-                                                            T* __restrict__ du, int64_t total, int64_t f, int64_t ldg, uint32_t nblk) {
-    const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total; i += step) {
-        const int64_t row = i / f, col = i - row * f, blk = row * nblk + col / kActBlock;
-        const float g = act_restored(act_values2(gq[i]).x, gs[blk], FLT_MAX), u = act_restored(act_values2(uq[i]).x, us[blk], FLT_MAX);
-        const float e = ActType<T>::load(dh[i]);
-        const float2 a = gate_both<ACT>(g);
-        dg[row * ldg + col] = ActType<T>::store(e * u * a.y);
-        du[row * ldg + col] = ActType<T>::store(e * a.x);
+                                                            T* __restrict__ du, int64_t spans, uint32_t per_row, int width, int64_t m, int64_t f,
+                                                            int64_t ldg, uint32_t nblk) {
+    constexpr int E = Part<T>::E, kCols = Part<T>::kCols;
+    const int lane = threadIdx.x & 31;
+    const int64_t total = m * f;
+    for (int64_t s = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); s < spans; s += static_cast<int64_t>(gridDim.x) * (kThreads / 32)) {
+        const int64_t row = s / per_row, first = (s - row * per_row) * width, at0 = row * f + first;
+        const int n = static_cast<int>(min(static_cast<int64_t>(width), f - first));
+        Stream<4> in(reinterpret_cast<const uint8_t*>(dh + at0), static_cast<int64_t>(n) * sizeof(T), reinterpret_cast<const uint8_t*>(dh),
+                     reinterpret_cast<const uint8_t*>(dh + total), lane);
+        Stream<2> ing(gq + at0, n, gq, gq + total, lane), inu(uq + at0, n, uq, uq + total, lane);
+        const int64_t blk = row * nblk + first / kActBlock;
+        T *const to_g = dg + row * ldg + first, *const to_u = du + row * ldg + first;
+#pragma unroll 1
+        for (int col = 0; col < n; col += kCols) {
+            uint32_t d[4], cg[2], cu[2];
+            const int at = col + lane * E;
+            const bool here = at < n;
+            const float sg = here ? __ldg(gs + blk + at / kActBlock) : 0.0f, su = here ? __ldg(us + blk + at / kActBlock) : 0.0f;
+            in.next(lane, d);
+            ing.next(lane, cg);
+            inu.next(lane, cu);
+            if (here) {
+                uint4 a, b;
+                gated_bwd8<T, ACT>(d, cg, cu, sg, su, a, b);
+                *reinterpret_cast<uint4*>(to_g + at) = a;        // the row's padding takes what is behind its last column
+                *reinterpret_cast<uint4*>(to_u + at) = b;
+            }
+        }
     }
+}
+
+// How k_save_any and k_gated_bwd_any share out their rows: long spans have fewer ragged ends, many spans keep all SMs busy, so the
+// longest spans that still leave every SM 32 warps, and at least two parts each.
+struct Spans { int64_t count; uint32_t per_row; int width; };
+Spans spans_of(int64_t rows, int64_t cols, int part) {
+    const int64_t parts = (cols + part - 1) / part, enough = static_cast<int64_t>(num_sms()) * 32;
+    int64_t per_row = (enough + rows - 1) / rows;
+    if (per_row > (parts + 1) / 2) per_row = (parts + 1) / 2;
+    const int64_t each = (parts + per_row - 1) / per_row;
+    per_row = (parts + each - 1) / each;
+    return {rows * per_row, static_cast<uint32_t>(per_row), static_cast<int>(each * part)};
 }
 
 int capped(int64_t ctas, int per_sm) {
@@ -253,17 +533,24 @@ int capped(int64_t ctas, int per_sm) {
     return static_cast<int>(ctas < 1 ? 1 : ctas < cap ? ctas : cap);
 }
 
+constexpr uint64_t aligned_to(uintptr_t bytes, const void* p, uintptr_t pitch_bytes) {
+    return ((reinterpret_cast<uintptr_t>(p) | pitch_bytes) & (bytes - 1)) == 0;
+}
+
 template <typename T>
 int launch_save(const T* x, uint8_t* q, float* scales, int64_t rows, int64_t cols, int64_t ldx, cudaStream_t st) {
+    constexpr int E = 32 / sizeof(T), U = 4;
     const uint32_t nblk = static_cast<uint32_t>((cols + kActBlock - 1) / kActBlock);
-    const bool vec = cols % 8 == 0 && aligned16(x) && (ldx * sizeof(T)) % 16 == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0;
-    if (vec) {
-        const uint32_t total = static_cast<uint32_t>(rows * nblk);
-        constexpr int U = 4;
-        k_save<T, U><<<capped((total + 16 * U - 1) / (16 * U), 8), kThreads, 0, st>>>(x, q, scales, total, nblk, cols, ldx);
+    if (cols % E == 0 && aligned_to(32, x, rows > 1 ? ldx * sizeof(T) : 0) && aligned_to(E, q, 0)) {
+        const uint32_t blocks = static_cast<uint32_t>(rows * nblk);
+        const int grid = capped((static_cast<int64_t>(blocks) * (kActBlock / E) + kThreads * U - 1) / (kThreads * U), 8);
+        if (cols % kActBlock == 0 && (ldx == cols || rows == 1))
+            k_save<T, U, true><<<grid, kThreads, 0, st>>>(x, q, scales, blocks, nblk, cols, ldx);
+        else
+            k_save<T, U, false><<<grid, kThreads, 0, st>>>(x, q, scales, blocks, nblk, cols, ldx);
     } else {
-        const uint32_t nseg = static_cast<uint32_t>((cols + kSeg - 1) / kSeg);
-        k_save_any<T><<<capped((rows * nseg + 7) / 8, 8), kThreads, 0, st>>>(x, q, scales, rows * nseg, nseg, nblk, cols, ldx);
+        const Spans sp = spans_of(rows, cols, Part<T>::kCols);
+        k_save_any<T><<<capped((sp.count + 7) / 8, 8), kThreads, 0, st>>>(x, q, scales, sp.count, sp.per_row, sp.width, nblk, rows, cols, ldx);
     }
     TB200_CUDA_TRY(cudaGetLastError());
     return TB200_OK;
@@ -271,15 +558,19 @@ int launch_save(const T* x, uint8_t* q, float* scales, int64_t rows, int64_t col
 
 template <typename T>
 int launch_restore(const uint8_t* q, const float* scales, T* out, int64_t rows, int64_t cols, cudaStream_t st) {
+    constexpr int E = 32 / sizeof(T), U = 4;
     const uint32_t nblk = static_cast<uint32_t>((cols + kActBlock - 1) / kActBlock);
-    if (cols % 16 == 0 && aligned16(q) && aligned16(out)) {
-        const int64_t total = rows * (cols / 16);
-        constexpr int U = 4;
-        k_restore<T, U><<<capped((total + kThreads * U - 1) / (kThreads * U), 8), kThreads, 0, st>>>(
-            reinterpret_cast<const uint4*>(q), scales, out, total, static_cast<uint32_t>(cols / 16), nblk);
+    if (cols % E == 0 && aligned_to(E, q, 0) && aligned_to(32, out, 0)) {
+        const uint32_t blocks = static_cast<uint32_t>(rows * nblk);
+        const int grid = capped((static_cast<int64_t>(blocks) * (kActBlock / E) + kThreads * U - 1) / (kThreads * U), 8);
+        if (cols % kActBlock == 0) k_restore<T, U, true><<<grid, kThreads, 0, st>>>(q, scales, out, blocks, nblk, cols);
+        else k_restore<T, U, false><<<grid, kThreads, 0, st>>>(q, scales, out, blocks, nblk, cols);
+    } else if (cols >= 16 && aligned_to(16, q, 0) && aligned_to(32, out, 0)) {
+        const int64_t total = rows * cols;
+        k_restore_across<T, U><<<capped((total + kThreads * E * U - 1) / (kThreads * E * U), 8), kThreads, 0, st>>>(q, scales, out, total, nblk, cols);
     } else {
-        const uint32_t nseg = static_cast<uint32_t>((cols + kSeg - 1) / kSeg);
-        k_restore_any<T><<<capped((rows * nseg + 7) / 8, 8), kThreads, 0, st>>>(q, scales, out, rows * nseg, nseg, nblk, cols);
+        const int64_t total = rows * cols;
+        k_restore_any<T><<<capped((total + kThreads - 1) / kThreads, 8), kThreads, 0, st>>>(q, scales, out, total, nblk, cols);
     }
     TB200_CUDA_TRY(cudaGetLastError());
     return TB200_OK;
@@ -289,16 +580,17 @@ template <typename T, int ACT>
 int launch_gated(const void* dh, const void* gq, const float* gs, const void* uq, const float* us, void* dg, void* du, int64_t m, int64_t f,
                  int64_t ldg, cudaStream_t st) {
     const uint32_t nblk = static_cast<uint32_t>((f + kActBlock - 1) / kActBlock);
-    const bool vec = f % 8 == 0 && ldg == f && aligned16(dh) && (reinterpret_cast<uintptr_t>(gq) & 7) == 0 && (reinterpret_cast<uintptr_t>(uq) & 7) == 0;
-    if (vec) {
+    if (f % 8 == 0 && aligned_to(16, dh, 0) && aligned_to(8, gq, 0) && aligned_to(8, uq, 0) && m * (f / 8) <= 0xFFFFFFFFll) {
         const int64_t total = m * (f / 8);
-        k_gated_bwd<T, ACT><<<capped((total + kThreads - 1) / kThreads, 8), kThreads, 0, st>>>(
+        constexpr int U = 2;
+        k_gated_bwd<T, ACT, U><<<capped((total + kThreads * U - 1) / (kThreads * U), 8), kThreads, 0, st>>>(
             static_cast<const uint4*>(dh), static_cast<const uint2*>(gq), gs, static_cast<const uint2*>(uq), us, static_cast<uint4*>(dg),
-            static_cast<uint4*>(du), total, static_cast<uint32_t>(f / 8), nblk);
+            static_cast<uint4*>(du), static_cast<uint32_t>(total), static_cast<uint32_t>(f / 8), nblk);
     } else {
-        k_gated_bwd_any<T, ACT><<<capped((m * f + kThreads - 1) / kThreads, 8), kThreads, 0, st>>>(
+        const Spans sp = spans_of(m, f, Part<T>::kCols);
+        k_gated_bwd_any<T, ACT><<<capped((sp.count + 7) / 8, 8), kThreads, 0, st>>>(
             static_cast<const T*>(dh), static_cast<const uint8_t*>(gq), gs, static_cast<const uint8_t*>(uq), us, static_cast<T*>(dg),
-            static_cast<T*>(du), m * f, f, ldg, nblk);
+            static_cast<T*>(du), sp.count, sp.per_row, sp.width, m, f, ldg, nblk);
     }
     TB200_CUDA_TRY(cudaGetLastError());
     return TB200_OK;

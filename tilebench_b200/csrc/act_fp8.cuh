@@ -18,7 +18,9 @@ constexpr int kActBlock = 128;
 
 #ifdef __CUDACC__
 
-__device__ __forceinline__ float act_size(float v) {            // |v|, 0 for infinities and NaN
+// |v|, 0 for infinities and NaN.  fmaxf passes over NaN by itself, so a block's amax is first taken as the plain
+// maximum of |v|, and only a block where that is infinite is looked at again with act_size.
+__device__ __forceinline__ float act_size(float v) {
     const float a = fabsf(v);
     return a <= FLT_MAX ? a : 0.0f;
 }
@@ -29,7 +31,8 @@ __device__ __forceinline__ float2 act_scale(float amax) {
     e = amax > 0.0f ? max(e, 1) : 127;
     return make_float2(__uint_as_float(static_cast<uint32_t>(e) << 23), __uint_as_float(static_cast<uint32_t>(254 - e) << 23));
 }
-// The hardware conversion saturates, so what is not finite is made NaN first (finite values are at most 448 here).
+// Codes of numbers times 1 / scale.  The hardware conversion makes NaN of NaN but saturates infinities, so a block that
+// holds any goes through act_scaled first (finite values are at most 448 here).
 __device__ __forceinline__ float act_scaled(float v, float inv) {
     const float y = v * inv;
     return fabsf(y) <= 448.0f ? y : __int_as_float(0x7FC00000);
@@ -38,16 +41,20 @@ __device__ __forceinline__ uint32_t act_codes2(float a, float b) {
     return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
 __device__ __forceinline__ uint32_t act_codes4(float a, float b, float c, float d, float inv) {
+    return act_codes2(a * inv, b * inv) | (act_codes2(c * inv, d * inv) << 16);
+}
+__device__ __forceinline__ uint32_t act_codes4_checked(float a, float b, float c, float d, float inv) {
     return act_codes2(act_scaled(a, inv), act_scaled(b, inv)) | (act_codes2(act_scaled(c, inv), act_scaled(d, inv)) << 16);
 }
 __device__ __forceinline__ float2 act_values2(uint32_t codes) { // two codes in the low half, as numbers (exact)
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes), __NV_E4M3);
     return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
-// code * scale, held within +-top: a block whose amax is close to the type's largest value may round up beyond it.
-__device__ __forceinline__ float act_restored(float code, float s, float top) {
-    const float v = code * s;
-    return fabsf(v) > top ? copysignf(top, v) : v;              // a NaN code stays NaN
+// code * scale, held within +-top: a block whose amax is close to the type's largest value may round up beyond it,
+// which takes a scale above top / 448.
+__device__ __forceinline__ bool act_may_exceed(float s, float top) { return s > top * (1.0f / 448.0f) * 0.999f; }
+__device__ __forceinline__ float act_held(float v, float top) {
+    return fabsf(v) > top ? copysignf(top, v) : v;              // NaN stays NaN
 }
 
 template <typename T> struct ActType;

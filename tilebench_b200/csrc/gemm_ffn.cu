@@ -17,6 +17,7 @@
 // Every mbarrier wait is bounded and reports through g_status.
 #include "act_fp8.cuh"
 
+#include <cmath>
 #include <cstring>
 
 namespace tb200 {
@@ -28,11 +29,12 @@ constexpr int kStages = 6;
 constexpr int kOperandBytes = kHalf * 128;
 constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kAtomBytes = kBK * 128;            // MN-major: one box of 64 contraction rows x 64 columns
-constexpr int kStagingBytes = 32 * 256;          // per epilogue warp: 32 rows x 128 16-bit columns
+constexpr int kEpiWarps = 8;                     // two per quarter of the tensor memory's lanes
+constexpr int kStagingBytes = 32 * 128;          // per epilogue warp: 32 rows of 128 bytes
 constexpr int kBarBytes = 256;
-constexpr int kSmemBytes = kStages * kStageBytes + 4 * kStagingBytes + kBarBytes + 1024;
+constexpr int kSmemBytes = kStages * kStageBytes + kEpiWarps * kStagingBytes + kBarBytes + 1024;
 constexpr int kTmemCols = 512;
-constexpr int kThreads = 256;
+constexpr int kThreads = 128 + 32 * kEpiWarps;   // TMA, MMA, two idle warps, epilogue
 constexpr int kGroupM = 8;                       // tiles are walked in bands of 8 x 256 rows, so that B's tiles stay in L2
 
 enum FfnKind : int { FK_FWD = 0, FK_DX = 1, FK_DW = 2 };
@@ -43,7 +45,10 @@ struct FfnMaps {
 };
 struct FfnArgs {
     void* out[2];                                // forward: h, -      dx: dx, -      dw: dWg, dWu
+    float* sums;                                 // dx in shares: [splits, rows, cols] partial sums
     int rows, cols, depth;                       // of one result, and of one product's contraction
+    int splits;                                  // dx: shares of the contraction
+    int w;                                       // forward: hidden units per tile (128 with checkpoints)
     int64_t ldo;                                 // row pitch of the result, in elements
     uint8_t* codes[2];                           // forward with checkpoints: codes of g and u, [rows, cols]
     float* scales[2];                            // and their scales, [rows, ceil(cols / 128)]
@@ -64,35 +69,59 @@ __device__ __forceinline__ void mma_pair_if(uint32_t issue, uint32_t d_tmem, uin
                  "r"(idesc), "r"(accumulate), "r"(issue) : "memory");
 }
 
-// ---- epilogue helpers --------------------------------------------------------------------------------------------
-// A warp collects 32 rows of 256 bytes in shared memory, 16-byte piece c of row r at place c ^ (r & 15) (free of bank
-// conflicts both ways), and writes them out with neighbouring lanes on neighbouring bytes.
-__device__ __forceinline__ uint4* staged(uint8_t* buf, int row, int piece) {
-    return reinterpret_cast<uint4*>(buf + row * 256 + ((piece ^ (row & 15)) << 4));
+__device__ __forceinline__ void mma_if(uint32_t issue, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc),
+                 "r"(idesc), "r"(accumulate), "r"(issue) : "memory");
 }
-// Pieces [first, first + count) of every row are `count` * 16 bytes of row r of dst; rows and columns beyond the valid
-// ones are left out.  T: the element.  Rows that do not lie on 16-byte boundaries are written element by element.
-template <typename T>
-__device__ __forceinline__ void flush(uint8_t* buf, int first, int count, T* __restrict__ dst, int64_t pitch, int rows, int cols, int lane) {
-    constexpr int V = 16 / sizeof(T);
-    if (rows > 32) rows = 32;
-    const bool vec = (reinterpret_cast<uintptr_t>(dst) & 15) == 0 && (pitch * sizeof(T)) % 16 == 0;
-    if (vec) {
-        const int per = 32 / count, sub = lane / count, piece = lane % count;
-        for (int r = sub; r < rows; r += per) {
-            const uint4 v = *staged(buf, r, first + piece);
-            T* p = dst + r * pitch + piece * V;
-            if (piece * V + V <= cols) {
-                *reinterpret_cast<uint4*>(p) = v;
+
+// ---- epilogue helpers --------------------------------------------------------------------------------------------
+// A warp collects 32 rows of 128 bytes in shared memory, 16-byte piece c of row r at place c ^ (r & 7) (free of bank
+// conflicts both ways), and writes them out with neighbouring lanes on neighbouring bytes.
+__device__ __forceinline__ uint8_t* staged(uint8_t* buf, int row, int piece) { return buf + row * 128 + ((piece ^ (row & 7)) << 4); }
+
+// Pieces [first, first + COUNT) of each row go to row r of dst; rows and columns beyond the valid ones are left out.
+// T: the element.  Rows that begin on 16-byte boundaries take 16-byte stores as they are.  Others (f is odd, say) take
+// 16-byte stores too, of five words shifted into place, between single elements at either end of the row.
+template <typename T, int COUNT>
+__device__ __forceinline__ void flush(uint8_t* buf, int first, T* __restrict__ dst, int64_t pitch, int rows, int cols, int lane) {
+    constexpr int kPer = 32 / COUNT, kSize = sizeof(T);
+    const int bytes = min(cols, COUNT * 16 / kSize) * kSize, sub = lane / COUNT, c = lane % COUNT;
+    rows = min(rows, 32);
+    if (bytes <= 0) return;
+    if (((reinterpret_cast<uintptr_t>(dst) | static_cast<uintptr_t>(pitch * kSize)) & 15) == 0) {
+#pragma unroll 4
+        for (int r = sub; r < rows; r += kPer) {
+            const uint8_t* src = staged(buf, r, first + c);
+            T* p = dst + r * pitch + c * (16 / kSize);
+            if (16 * c + 16 <= bytes) {
+                *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(src);
             } else {
-                const T* e = reinterpret_cast<const T*>(staged(buf, r, first + piece));
-                for (int i = 0; i < cols - piece * V; ++i) p[i] = e[i];
+                for (int i = 0; 16 * c + i * kSize < bytes; ++i) p[i] = reinterpret_cast<const T*>(src)[i];
             }
         }
     } else {
-        for (int r = 0; r < rows; ++r)
-            for (int c = lane; c < count * V && c < cols; c += 32)
-                dst[r * pitch + c] = reinterpret_cast<const T*>(staged(buf, r, first + c / V))[c % V];
+#pragma unroll 2
+        for (int r = sub; r < rows; r += kPer) {
+            uint8_t* p = reinterpret_cast<uint8_t*>(dst + r * pitch);
+            const int head = min(bytes, static_cast<int>(-reinterpret_cast<uintptr_t>(p) & 15)), tail = (bytes - head) & 15;
+            const int at = head + 16 * c;
+            if (at + 16 <= bytes) {
+                uint32_t w[5];
+#pragma unroll
+                for (int i = 0; i < 5; ++i) {
+                    const int word = min(at / 4 + i, 4 * COUNT - 1);        // the fifth is not used where it would lie behind the row
+                    w[i] = *reinterpret_cast<const uint32_t*>(staged(buf, r, first + word / 4) + (word & 3) * 4);
+                }
+                const uint32_t sh = (at & 3) * 8;
+                *reinterpret_cast<uint4*>(p + at) = make_uint4(__funnelshift_r(w[0], w[1], sh), __funnelshift_r(w[1], w[2], sh),
+                                                               __funnelshift_r(w[2], w[3], sh), __funnelshift_r(w[3], w[4], sh));
+            }
+            for (int e = c; e * kSize < head + tail; e += COUNT) {
+                const int b = e * kSize < head ? e * kSize : bytes - tail + e * kSize - head;
+                *reinterpret_cast<T*>(p + b) = *reinterpret_cast<const T*>(staged(buf, r, first + b / 16) + (b & 15));
+            }
+        }
     }
 }
 
@@ -100,27 +129,32 @@ template <typename T>
 __device__ __forceinline__ void stage32(uint8_t* buf, int row, int piece0, const float (&v)[32]) {      // 32 columns: 4 pieces
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-        *staged(buf, row, piece0 + q) = make_uint4(ActType<T>::pack(v[8 * q], v[8 * q + 1]), ActType<T>::pack(v[8 * q + 2], v[8 * q + 3]),
-                                                   ActType<T>::pack(v[8 * q + 4], v[8 * q + 5]), ActType<T>::pack(v[8 * q + 6], v[8 * q + 7]));
+        *reinterpret_cast<uint4*>(staged(buf, row, piece0 + q)) = make_uint4(ActType<T>::pack(v[8 * q], v[8 * q + 1]), ActType<T>::pack(v[8 * q + 2], v[8 * q + 3]),
+                                                                             ActType<T>::pack(v[8 * q + 4], v[8 * q + 5]), ActType<T>::pack(v[8 * q + 6], v[8 * q + 7]));
 }
-__device__ __forceinline__ void stage_codes32(uint8_t* buf, int row, int piece0, const uint32_t (&v)[32], float inv) {  // 2 pieces
+__device__ __forceinline__ void stage_codes32(uint8_t* buf, int row, int piece0, const uint32_t (&v)[32], float inv, bool checked) {  // 2 pieces
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int i = 16 * q + 4 * e;
-            w[e] = act_codes4(__uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]), inv);
+            const float a = __uint_as_float(v[i]), b = __uint_as_float(v[i + 1]), c = __uint_as_float(v[i + 2]), d = __uint_as_float(v[i + 3]);
+            w[e] = checked ? act_codes4_checked(a, b, c, d, inv) : act_codes4(a, b, c, d, inv);
         }
-        *staged(buf, row, piece0 + q) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(staged(buf, row, piece0 + q)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
+__device__ __forceinline__ void pair_of_warps_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
 template <int ACT>
 __device__ __forceinline__ void gated32(const uint32_t (&g)[32], const uint32_t (&u)[32], float (&h)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) h[i] = gate_value<ACT>(__uint_as_float(g[i])) * __uint_as_float(u[i]);
 }
+
+// First step of share i of n.
+__device__ __forceinline__ int share_at(int steps, int i, int n) { return static_cast<int>(static_cast<int64_t>(steps) * i / n); }
 
 struct Tile { int m, n; };
 __device__ __forceinline__ Tile tile_at(int t, int tiles_m, int tiles_n) {
@@ -135,14 +169,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs p) {
     constexpr int S = kStages;
     constexpr bool kAMn = KIND == FK_DW, kBMn = KIND != FK_FWD;
-    constexpr int kTileCols = KIND == FK_FWD ? 128 : 256;       // columns of the result that a tile covers
+    const int tile_cols = KIND == FK_FWD ? p.w : 2 * kHalf;     // columns of the result that a tile covers
+    const int b_bytes = KIND == FK_FWD ? p.w * 128 : kOperandBytes;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* staging = smem + S * kStageBytes;
-    uint64_t* bar_full = reinterpret_cast<uint64_t*>(staging + 4 * kStagingBytes);
+    uint64_t* bar_full = reinterpret_cast<uint64_t*>(staging + kEpiWarps * kStagingBytes);
     uint64_t* bar_empty = bar_full + S;
     uint64_t* bar_afull = bar_empty + S;          // [2] accumulator complete
-    uint64_t* bar_aempty = bar_afull + 2;         // [2] accumulator read (4 epilogue warps in each CTA)
+    uint64_t* bar_aempty = bar_afull + 2;         // [2] accumulator read (the epilogue warps of both CTAs)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_aempty + 2);
 
     const int warp = threadIdx.x >> 5;
@@ -151,11 +186,12 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
     const int pair = blockIdx.x >> 1;
     const int npairs = gridDim.x >> 1;
     const int KB = (p.depth + kBK - 1) / kBK;                   // stages of one product
-    const int steps = KIND == FK_DX ? 2 * KB : KB;
+    const int steps = KIND == FK_DX ? 2 * KB : KB;              // of a tile; dx: dg Wg, then du Wu
     const int tm1 = (p.rows + 2 * kHalf - 1) / (2 * kHalf);
     const int tiles_m = KIND == FK_DW ? 2 * tm1 : tm1;          // dw: the tiles of dWg, then those of dWu
-    const int tiles_n = (p.cols + kTileCols - 1) / kTileCols;
+    const int tiles_n = (p.cols + tile_cols - 1) / tile_cols;
     const int tiles = tiles_m * tiles_n;
+    const int items = KIND == FK_DX ? tiles * p.splits : tiles; // dx: item i is share i / tiles of tile i % tiles
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
@@ -164,7 +200,7 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&bar_afull[b], 1);
-            mbar_init(&bar_aempty[b], 8);
+            mbar_init(&bar_aempty[b], 2 * kEpiWarps);
         }
         mbar_fence_init();
         tma_prefetch_desc(&maps.a[0]);
@@ -187,15 +223,17 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
         if (lane == 0) {
             uint32_t s = 0, ph = 1;
             bool ok = true;
-            for (int t = pair; t < tiles && ok; t += npairs) {
-                const Tile tc = tile_at(t, tiles_m, tiles_n);
+            for (int t = pair; t < items && ok; t += npairs) {
+                const int share = KIND == FK_DX ? t / tiles : 0;
+                const Tile tc = tile_at(t - share * tiles, tiles_m, tiles_n);
                 const int sel = KIND == FK_DW && tc.m >= tm1 ? 1 : 0;
                 const int a_row = (tc.m - sel * tm1) * 2 * kHalf + rank * kHalf;
-                const int b_col = KIND == FK_FWD ? tc.n * kHalf : tc.n * 2 * kHalf + rank * kHalf;
-                for (int st = 0; st < steps; ++st) {
+                const int b_col = KIND == FK_FWD ? tc.n * tile_cols : tc.n * 2 * kHalf + rank * kHalf;
+                const int st0 = KIND == FK_DX ? share_at(steps, share, p.splits) : 0, st1 = KIND == FK_DX ? share_at(steps, share + 1, p.splits) : steps;
+                for (int st = st0; st < st1; ++st) {
                     if (!mbar_wait(&bar_empty[s], ph, ST_WAIT_SMEM_EMPTY, st)) { ok = false; break; }
                     uint8_t* stage = smem + s * kStageBytes;
-                    if (rank == 0) mbar_expect_tx(&bar_full[s], 2 * kStageBytes);               // both CTAs' bytes
+                    if (rank == 0) mbar_expect_tx(&bar_full[s], 2 * (kOperandBytes + b_bytes));  // both CTAs' bytes
                     const int prod = KIND == FK_DX && st >= KB ? 1 : 0;
                     const int k0 = (st - prod * KB) * kBK;
                     if constexpr (kAMn) {
@@ -222,7 +260,7 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
     } else if (warp == 1 && rank == 0) {
         // ---------------- MMA issuer (leader only; the whole warp walks the loop, lane 0 issues by predication) ------
         constexpr uint32_t fmt = sizeof(T) == 2 && ActType<T>::kTop > 1e6f ? 1u : 0u;            // 1 = bf16, 0 = fp16
-        constexpr uint32_t idesc = umma_idesc(fmt, fmt, 2 * kHalf, 2 * kHalf) | (kAMn ? 1u << 15 : 0u) | (kBMn ? 1u << 16 : 0u);
+        const uint32_t idesc = umma_idesc(fmt, fmt, 2 * kHalf, KIND == FK_FWD ? 2 * tile_cols : 2 * kHalf) | (kAMn ? 1u << 15 : 0u) | (kBMn ? 1u << 16 : 0u);
         constexpr uint32_t kStageDesc = kStageBytes >> 4;
         // 16 of the 64 contraction elements per MMA: 32 bytes along a K-major row, 16 rows of an MN-major box
         constexpr uint64_t a_step = kAMn ? 16 * 128 / 16 : 2, b_step = kBMn ? 16 * 128 / 16 : 2;
@@ -232,12 +270,14 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
         uint32_t s = 0, ph = 0, cnt = 0;
         bool ready = false;
         bool ok = true;
-        for (int t = pair; t < tiles && ok; t += npairs, ++cnt) {
+        for (int t = pair; t < items && ok; t += npairs, ++cnt) {
             const uint32_t acc = cnt & 1;
             if (!mbar_wait(&bar_aempty[acc], ((cnt >> 1) & 1) ^ 1, ST_WAIT_TMEM_EMPTY, t)) { ok = false; break; }
             tc_fence_after();
             const uint32_t d_tmem = tmem_base + acc * 256;
-            for (int st = 0; st < steps; ++st) {
+            const int share = KIND == FK_DX ? t / tiles : 0;
+            const int n = KIND == FK_DX ? share_at(steps, share + 1, p.splits) - share_at(steps, share, p.splits) : steps;
+            for (int st = 0; st < n; ++st) {
                 if (!ready && !mbar_wait(&bar_full[s], ph, ST_WAIT_SMEM_FULL, st)) { ok = false; break; }
                 tc_fence_after();
                 const uint64_t a_desc = a_desc0 + s * kStageDesc;
@@ -253,41 +293,46 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
             if (ok && leader) tc_commit_pair(&bar_afull[acc], 0x3);
         }
     } else if (warp >= 4) {
-        // ---------------- epilogue (both CTAs; each owns 128 rows of the tile, each warp 32 of them) ----------------
-        const int ew = warp - 4;
-        uint8_t* buf = staging + ew * kStagingBytes;
+        // ---------------- epilogue (both CTAs; each owns 128 rows of the tile, each warp 32 rows of one half of the columns) ----
+        const int ew = (warp - 4) & 3, half = (warp - 4) >> 2;
+        uint8_t* buf = staging + (warp - 4) * kStagingBytes;
         const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(ew * 32) << 16);
         uint32_t cnt = 0;
         bool ok = true;
-        for (int t = pair; t < tiles && ok; t += npairs, ++cnt) {
-            const Tile tc = tile_at(t, tiles_m, tiles_n);
+        for (int t = pair; t < items; t += npairs, ++cnt) {
+            const int share = KIND == FK_DX ? t / tiles : 0;
+            const Tile tc = tile_at(t - share * tiles, tiles_m, tiles_n);
             const int sel = KIND == FK_DW && tc.m >= tm1 ? 1 : 0;
             const uint32_t acc = cnt & 1;
             const int row0 = (tc.m - sel * tm1) * 2 * kHalf + rank * kHalf + ew * 32;             // the warp's first row
             const int rows = p.rows - row0;                                                       // valid rows (may be <= 0)
-            const int col0 = tc.n * kTileCols, cols = p.cols - col0;
             const uint32_t t_acc = t_lane + acc * 256;
-            if (!mbar_wait(&bar_afull[acc], (cnt >> 1) & 1, ST_WAIT_TMEM_FULL, t)) { ok = false; break; }
+            // a wait that gave up ends the waiting, not the walk: the warps meet at barriers below
+            ok = ok && mbar_wait(&bar_afull[acc], (cnt >> 1) & 1, ST_WAIT_TMEM_FULL, t);
             tc_fence_after();
-            T* dst = static_cast<T*>(p.out[sel]) + static_cast<int64_t>(row0) * p.ldo + col0;
+            auto release = [&] {                                                                  // the warp has read its part of the accumulator
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_leader(&bar_aempty[acc]);
+            };
             if constexpr (KIND == FK_FWD) {
+                // columns [at, at + n) of the tile, n <= 64; what is read beyond them belongs to nobody and is not stored
+                const int split = (tile_cols / 2 + 7) / 8 * 8, at = half * split, n = half == 0 ? split : tile_cols - split;
+                const int col0 = tc.n * tile_cols + at, cols = min(n, p.cols - col0);
+                const uint32_t t_g = t_acc + at, t_u = t_acc + tile_cols + at;
                 uint32_t g[32], u[32];
                 float amax_g = 0.0f, amax_u = 0.0f;
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    tmem_ld32(t_acc + c * 32, g);
-                    tmem_ld32(t_acc + kHalf + c * 32, u);
+                for (int c = 0; c < 2; ++c) {
+                    tmem_ld32(t_g + c * 32, g);
+                    tmem_ld32(t_u + c * 32, u);
                     tmem_wait_ld();
-                    if (!SAVE && c == 3) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_leader(&bar_aempty[acc]);
-                    }
+                    if (!SAVE && c == 1) release();
                     if constexpr (SAVE) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
-                            amax_g = fmaxf(amax_g, act_size(__uint_as_float(g[i])));
-                            amax_u = fmaxf(amax_u, act_size(__uint_as_float(u[i])));
+                            amax_g = fmaxf(amax_g, fabsf(__uint_as_float(g[i])));
+                            amax_u = fmaxf(amax_u, fabsf(__uint_as_float(u[i])));
                         }
                     }
                     float h[32];
@@ -295,55 +340,89 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
                     stage32<T>(buf, lane, 4 * c, h);
                 }
                 __syncwarp();
-                flush<T>(buf, 0, 16, dst, p.ldo, rows, cols, lane);
+                flush<T, 8>(buf, 0, static_cast<T*>(p.out[0]) + static_cast<int64_t>(row0) * p.ldo + col0, p.ldo, rows, cols, lane);
                 __syncwarp();
                 if constexpr (SAVE) {
+                    // the block's amax over both halves of the columns, exchanged through the staging buffers
+                    auto both = [&] {
+                        reinterpret_cast<float2*>(buf)[lane] = make_float2(amax_g, amax_u);
+                        pair_of_warps_sync(1 + ew);
+                        const float2 o = reinterpret_cast<const float2*>(staging + ((warp - 4) ^ 4) * kStagingBytes)[lane];
+                        amax_g = fmaxf(amax_g, o.x);
+                        amax_u = fmaxf(amax_u, o.y);
+                        pair_of_warps_sync(1 + ew);
+                    };
+                    both();
+                    const bool infinite = __any_sync(0xffffffffu, fmaxf(amax_g, amax_u) > FLT_MAX);   // the same in both warps
+                    if (infinite) {                              // once more, over the finite values
+                        amax_g = amax_u = 0.0f;
+#pragma unroll 1
+                        for (int c = 0; c < 2; ++c) {
+                            tmem_ld32(t_g + c * 32, g);
+                            tmem_ld32(t_u + c * 32, u);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                amax_g = fmaxf(amax_g, act_size(__uint_as_float(g[i])));
+                                amax_u = fmaxf(amax_u, act_size(__uint_as_float(u[i])));
+                            }
+                        }
+                        both();
+                    }
                     const int64_t nblk = (p.cols + kHalf - 1) / kHalf;
                     const float2 sg = act_scale(amax_g), su = act_scale(amax_u);
-                    if (lane < rows) {
-                        p.scales[0][(row0 + lane) * nblk + tc.n] = sg.x;
-                        p.scales[1][(row0 + lane) * nblk + tc.n] = su.x;
-                    }
+                    if (lane < rows) p.scales[half][(row0 + lane) * nblk + tc.n] = half == 0 ? sg.x : su.x;
 #pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        tmem_ld32(t_acc + c * 32, g);
-                        tmem_ld32(t_acc + kHalf + c * 32, u);
+                    for (int c = 0; c < 2; ++c) {
+                        tmem_ld32(t_g + c * 32, g);
+                        tmem_ld32(t_u + c * 32, u);
                         tmem_wait_ld();
-                        if (c == 3) {
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive_leader(&bar_aempty[acc]);
-                        }
-                        stage_codes32(buf, lane, 2 * c, g, sg.y);
-                        stage_codes32(buf, lane, 8 + 2 * c, u, su.y);
+                        if (c == 1) release();
+                        stage_codes32(buf, lane, 2 * c, g, sg.y, infinite);
+                        stage_codes32(buf, lane, 4 + 2 * c, u, su.y, infinite);
                     }
                     __syncwarp();
-                    const int64_t at = static_cast<int64_t>(row0) * p.cols + col0;
-                    flush<uint8_t>(buf, 0, 8, p.codes[0] + at, p.cols, rows, cols, lane);
-                    flush<uint8_t>(buf, 8, 8, p.codes[1] + at, p.cols, rows, cols, lane);
+                    const int64_t to = static_cast<int64_t>(row0) * p.cols + col0;
+                    flush<uint8_t, 4>(buf, 0, p.codes[0] + to, p.cols, rows, cols, lane);
+                    flush<uint8_t, 4>(buf, 4, p.codes[1] + to, p.cols, rows, cols, lane);
                     __syncwarp();
                 }
             } else {
-#pragma unroll 1
-                for (int half = 0; half < 2; ++half) {
+                const int col0 = tc.n * tile_cols + half * kHalf, cols = p.cols - col0;
+                const uint32_t t_col = t_acc + half * kHalf;
+                if (KIND == FK_DX && p.splits > 1) {             // partial sums in 32 bits, 32 columns at a time
+                    float* dst = p.sums + (static_cast<int64_t>(share) * p.rows + row0) * p.cols + col0;
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
                         uint32_t v[32];
-                        float w[32];
-                        tmem_ld32(t_acc + half * kHalf + c * 32, v);
+                        tmem_ld32(t_col + c * 32, v);
                         tmem_wait_ld();
-                        if (half == 1 && c == 3) {
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive_leader(&bar_aempty[acc]);
-                        }
+                        if (c == 3) release();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) w[i] = __uint_as_float(v[i]);
-                        stage32<T>(buf, lane, 4 * c, w);
+                        for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(staged(buf, lane, q)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                        __syncwarp();
+                        flush<float, 8>(buf, 0, dst + c * 32, p.cols, rows, cols - c * 32, lane);
+                        __syncwarp();
                     }
-                    __syncwarp();
-                    flush<T>(buf, 0, 16, dst + half * kHalf, p.ldo, rows, cols - half * kHalf, lane);
-                    __syncwarp();
+                } else {
+                    T* dst = static_cast<T*>(p.out[sel]) + static_cast<int64_t>(row0) * p.ldo + col0;
+#pragma unroll 1
+                    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                        for (int d = 0; d < 2; ++d) {
+                            uint32_t v[32];
+                            float w[32];
+                            tmem_ld32(t_col + c * 64 + d * 32, v);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) w[i] = __uint_as_float(v[i]);
+                            stage32<T>(buf, lane, 4 * d, w);
+                        }
+                        if (c == 1) release();
+                        __syncwarp();
+                        flush<T, 8>(buf, 0, dst + c * 64, p.ldo, rows, cols - c * 64, lane);
+                        __syncwarp();
+                    }
                 }
             }
         }
@@ -360,13 +439,232 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
     }
 }
 
+// ------------------------------------------------------------------------------------------------
+// Forward block for a decoding batch (m <= 128 rows, no checkpoints): bound by reading the weights, so every SM has to
+// stream an equal share of them.  One CTA per tile of 128 rows x w hidden units (N = 2 w: w rows of Wg, w rows of Wu),
+// with w, a multiple of 8, chosen per call so that the tiles fill one wave (or whole waves) of SMs.  Where f is too
+// small for that, the CTAs of a cluster share the contraction of a tile (SPLIT): each leaves its sums in its shared
+// memory, and each adds up a share of the columns in a fixed order, reading its peers' memory.
+constexpr int kMaxStages = 8;
+struct MidMaps { CUtensorMap x, wg, wu; };
+struct MidArgs {
+    void* h;
+    int m, f, depth;
+    int w, stages, x_rows;                       // hidden units per tile, stages in shared memory, rows of x per copy
+};
+constexpr int kMidRing = 192 * 1024;
+constexpr int kMidSmemBytes = kMidRing + kEpiWarps * kStagingBytes + kBarBytes + 1024;
+
+__device__ __forceinline__ float4 peer_float4(uint32_t addr, uint32_t rank) {
+    uint32_t at;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
+template <typename T, int ACT, int SHARES>
+__global__ void __launch_bounds__(kThreads, 1) k_ffn_mid(const __grid_constant__ MidMaps maps, const __grid_constant__ MidArgs p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* staging = smem + kMidRing;
+    uint64_t* bar_full = reinterpret_cast<uint64_t*>(staging + kEpiWarps * kStagingBytes);
+    uint64_t* bar_empty = bar_full + kMaxStages;
+    uint64_t* bar_afull = bar_empty + kMaxStages;
+    uint64_t* bar_aempty = bar_afull + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_aempty + 2);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const int S = p.stages, w = p.w;
+    const int x_bytes = p.x_rows * 128, stage_bytes = x_bytes + 2 * w * 128;
+    const int KB = (p.depth + kBK - 1) / kBK;
+    constexpr bool SPLIT = SHARES > 1;
+    const int share = SPLIT ? static_cast<int>(cluster_ctarank()) : 0;
+    const int kb0 = KB * share / SHARES, kb1 = KB * (share + 1) / SHARES;
+    const int tiles = (p.f + w - 1) / w;
+    const int t0 = static_cast<int>(blockIdx.x) / SHARES;
+    const int t_step = SPLIT ? tiles : static_cast<int>(gridDim.x);                 // with SPLIT a CTA has one tile
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(&bar_full[s], 1);
+            mbar_init(&bar_empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&bar_afull[b], 1);
+            mbar_init(&bar_aempty[b], kEpiWarps);
+        }
+        mbar_fence_init();
+        tma_prefetch_desc(&maps.x);
+        tma_prefetch_desc(&maps.wg);
+        tma_prefetch_desc(&maps.wu);
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0) {
+        // ---------------- TMA producer ----------------
+        if (lane == 0) {
+            uint32_t s = 0, ph = 1, it = 0;
+            bool ok = true;
+            for (int t = t0; t < tiles && ok; t += t_step) {
+                for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                    if (!mbar_wait(&bar_empty[s], ph, ST_WAIT_SMEM_EMPTY, kb)) { ok = false; break; }
+                    uint8_t* stage = smem + s * stage_bytes;
+                    mbar_expect_tx(&bar_full[s], stage_bytes);
+                    tma_load_2d(stage + x_bytes, &maps.wg, &bar_full[s], kb * kBK, t * w);
+                    tma_load_2d(stage + x_bytes + w * 128, &maps.wu, &bar_full[s], kb * kBK, t * w);
+                    tma_load_2d(stage, &maps.x, &bar_full[s], kb * kBK, 0);
+                    if (++s == static_cast<uint32_t>(S)) { s = 0; ph ^= 1; }
+                }
+            }
+            if (!ok) {
+                // copies in flight land within microseconds; a bounded pause before the CTA may exit
+                const long long c0 = clock64();
+                while (clock64() - c0 < (1ll << 21)) {}
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer ----------------
+        // Rows of x beyond x_rows are whatever follows in shared memory: they reach only rows of the accumulator that
+        // nothing reads.
+        constexpr uint32_t fmt = ActType<T>::kTop > 1e6f ? 1u : 0u;
+        const uint32_t idesc = umma_idesc(fmt, fmt, kHalf, 2 * w);
+        const bool leader = lane == 0;
+        const uint64_t a_desc0 = umma_desc_sw128(smem_u32(smem)), b_desc0 = umma_desc_sw128(smem_u32(smem) + x_bytes);
+        const uint32_t stage_desc = static_cast<uint32_t>(stage_bytes) >> 4;
+        uint32_t s = 0, ph = 0, cnt = 0;
+        bool ready = false;
+        bool ok = true;
+        for (int t = t0; t < tiles && ok; t += t_step, ++cnt) {
+            const uint32_t acc = cnt & 1;
+            if (!mbar_wait(&bar_aempty[acc], ((cnt >> 1) & 1) ^ 1, ST_WAIT_TMEM_EMPTY, t)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t d_tmem = tmem_base + acc * 256;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!ready && !mbar_wait(&bar_full[s], ph, ST_WAIT_SMEM_FULL, kb)) { ok = false; break; }
+                tc_fence_after();
+                const uint64_t a_desc = a_desc0 + s * stage_desc, b_desc = b_desc0 + s * stage_desc;
+                uint64_t* const freed = &bar_empty[s];
+                if (++s == static_cast<uint32_t>(S)) { s = 0; ph ^= 1; }
+                mma_if(leader, d_tmem, a_desc, b_desc, idesc, kb > kb0 ? 1u : 0u);
+                ready = mbar_test_wait(&bar_full[s], ph);
+#pragma unroll
+                for (int k = 1; k < 4; ++k) mma_if(leader, d_tmem, a_desc + 2 * k, b_desc + 2 * k, idesc, 1u);
+                tc_commit_if(leader, freed);
+            }
+            if (ok && leader) tc_commit(&bar_afull[acc]);
+        }
+    } else if (warp >= 4) {
+        // ---------------- epilogue: a warp has 32 rows of one half of the columns ----------------
+        const int ew = (warp - 4) & 3, half = (warp - 4) >> 2;
+        uint8_t* buf = staging + (warp - 4) * kStagingBytes;
+        const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(ew * 32) << 16);
+        uint32_t cnt = 0;
+        bool ok = true;
+        for (int t = t0; t < tiles && ok; t += t_step, ++cnt) {
+            const uint32_t acc = cnt & 1;
+            if (!mbar_wait(&bar_afull[acc], (cnt >> 1) & 1, ST_WAIT_TMEM_FULL, t)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t t_acc = t_lane + acc * 256;
+            const int row0 = ew * 32;
+            if constexpr (SPLIT) {
+                // this CTA's sums, row by row: one half of the warps g, the other u.  A row pitch of 4 more than a multiple of
+                // 16 keeps eight lanes' (rows') 16-byte pieces on different banks.  Every copy into the ring has landed and been
+                // used by the time the accumulator is complete.
+                float* mine = reinterpret_cast<float*>(smem) + (row0 + lane) * (2 * w + 4) + half * w;
+                if (row0 < p.m) {
+#pragma unroll 1
+                    for (int c = 0; c < w; c += 16) {
+                        uint32_t v[16];
+                        tmem_ld16(t_acc + half * w + c, v);
+                        tmem_wait_ld();
+                        if (row0 + lane < p.m) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (c + 4 * i < w) *reinterpret_cast<uint4*>(mine + c + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                        }
+                    }
+                }
+            } else {
+                const int split = (w / 2 + 7) / 8 * 8, at = half * split, n = half == 0 ? split : w - split;
+                const int col0 = t * w + at, cols = min(n, p.f - col0);
+#pragma unroll 1
+                for (int c = 0; c < 2; ++c) {
+                    if (row0 < p.m && c * 32 < n) {
+                        uint32_t g[32], u[32];
+                        tmem_ld32(t_acc + at + c * 32, g);
+                        tmem_ld32(t_acc + w + at + c * 32, u);
+                        tmem_wait_ld();
+                        float h[32];
+                        gated32<ACT>(g, u, h);
+                        stage32<T>(buf, lane, 4 * c, h);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar_aempty[acc]);
+                flush<T, 8>(buf, 0, static_cast<T*>(p.h) + static_cast<int64_t>(row0) * p.f + col0, p.f, p.m - row0, cols, lane);
+                __syncwarp();
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if constexpr (SPLIT) {
+        cluster_sync_all();                                      // every share of the sums is in place
+        const int quads = w / 4, q0 = quads * share / SHARES, qn = quads * (share + 1) / SHARES - q0;
+        const uint32_t base = smem_u32(smem);
+        const bool vec = p.f % 4 == 0 && (reinterpret_cast<uintptr_t>(p.h) & 7) == 0;
+        for (int i = threadIdx.x; i < p.m * qn; i += kThreads) {
+            const int r = i / qn, c = 4 * (q0 + i - r * qn), col = t0 * w + c;
+            const uint32_t at = base + 4 * (r * (2 * w + 4) + c);
+            float4 gs[SHARES], us[SHARES];
+#pragma unroll
+            for (int o = 0; o < SHARES; ++o) {
+                gs[o] = peer_float4(at, o);
+                us[o] = peer_float4(at + 4 * w, o);
+            }
+            float4 g = gs[0], u = us[0];
+#pragma unroll
+            for (int o = 1; o < SHARES; ++o) {
+                g.x += gs[o].x; g.y += gs[o].y; g.z += gs[o].z; g.w += gs[o].w;
+                u.x += us[o].x; u.y += us[o].y; u.z += us[o].z; u.w += us[o].w;
+            }
+            const float v[4] = {gate_value<ACT>(g.x) * u.x, gate_value<ACT>(g.y) * u.y, gate_value<ACT>(g.z) * u.z, gate_value<ACT>(g.w) * u.w};
+            T* h = static_cast<T*>(p.h) + static_cast<int64_t>(r) * p.f + col;
+            if (vec && col < p.f) {
+                *reinterpret_cast<uint2*>(h) = make_uint2(ActType<T>::pack(v[0], v[1]), ActType<T>::pack(v[2], v[3]));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (col + e < p.f) h[e] = ActType<T>::store(v[e]);
+            }
+        }
+        cluster_sync_all();                                      // no CTA leaves while a peer reads its memory
+    }
+    if (warp == 1) {
+        __syncwarp();
+        tmem_dealloc(tmem_base, kTmemCols);
+    }
+}
+
 template <typename T>
 constexpr CUtensorMapDataType tmap_type() { return ActType<T>::kTop > 1e6f ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16; }
 
 // K-major operand: 128 rows x 64 of the contraction.  MN-major operand: 64 rows of the contraction x 64 columns.
 template <typename T>
-int map_k(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t pitch) {
-    return encode_tmap_2d(m, base, tmap_type<T>(), 2, rows, cols, pitch * 2, kHalf, kBK, CU_TENSOR_MAP_SWIZZLE_128B);
+int map_k(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t pitch, int box_rows = kHalf) {
+    return encode_tmap_2d(m, base, tmap_type<T>(), 2, rows, cols, pitch * 2, box_rows, kBK, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 template <typename T>
 int map_mn(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t pitch) {
@@ -393,8 +691,8 @@ int launch_pair(const FfnMaps& maps, const FfnArgs& args, cudaStream_t st) {
         max_pairs = clusters;
         max_pairs_tab.v[dev].store(clusters, std::memory_order_release);
     }
-    const int64_t tile_cols = KIND == FK_FWD ? kHalf : 2 * kHalf;
-    const int64_t tiles = (KIND == FK_DW ? 2 : 1) * ((args.rows + 2 * kHalf - 1) / (2 * kHalf)) * ((args.cols + tile_cols - 1) / tile_cols);
+    const int64_t tile_cols = KIND == FK_FWD ? args.w : 2 * kHalf;
+    const int64_t tiles = (KIND == FK_DW ? 2 : KIND == FK_DX ? args.splits : 1) * ((args.rows + 2 * kHalf - 1) / (2 * kHalf)) * ((args.cols + tile_cols - 1) / tile_cols);
     if (tiles > 0x7fffffffll / kGroupM) return fail(TB200_ERR_UNSUPPORTED, "ffn_gated: too many tiles");
     const int pairs = static_cast<int>(tiles < max_pairs ? tiles : max_pairs);
     kern<<<2 * pairs, kThreads, kSmemBytes, st>>>(maps, args);
@@ -412,16 +710,156 @@ int launch_fwd(const FfnMaps& maps, const FfnArgs& args, int act, cudaStream_t s
     }
 }
 
+// ---- the decoding batch's tiles ----
+struct MidPlan { int w, shares; };
+
+template <int SHARES>
+int clusters_of(int* n) {                        // clusters of SHARES CTAs that the device holds at once
+    static PerDeviceInt tab;
+    int dev = 0;
+    const int rc = current_device(&dev);
+    if (rc != TB200_OK) return rc;
+    *n = tab.v[dev].load(std::memory_order_acquire);
+    if (*n == 0) {
+        auto kern = k_ffn_mid<__nv_bfloat16, TB200_ACT_SILU, SHARES>;
+        TB200_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMidSmemBytes));
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(static_cast<unsigned>(num_sms() / SHARES * SHARES), 1, 1);
+        cfg.blockDim = dim3(kThreads, 1, 1);
+        cfg.dynamicSmemBytes = kMidSmemBytes;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = SHARES;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        TB200_CUDA_TRY(cudaOccupancyMaxActiveClusters(n, kern, &cfg));
+        if (*n < 1) *n = -1;
+        tab.v[dev].store(*n, std::memory_order_release);
+    }
+    return TB200_OK;
+}
+
+// The width and the shares with the least time by a model fitted to measurements (1 to 128 rows, k 512..8192,
+// f 512..28672; it picks within 8 % of the best measured plan).  A stage takes 0.25 us to issue whatever its size, or what it takes to
+// bring its bytes from L2 to the SM (95 GB/s each) or all CTAs' weights from HBM (6.4 TB/s); a wave takes its stages;
+// sharing costs 0.8 us and the peers' sums at 20 GB/s.
+int mid_plan(int64_t m, int64_t f, int64_t k, MidPlan* plan) {
+    int clusters[4] = {num_sms(), 0, 0, 0};
+    int rc = clusters_of<2>(&clusters[1]);
+    if (rc == TB200_OK) rc = clusters_of<4>(&clusters[2]);
+    if (rc == TB200_OK) rc = clusters_of<8>(&clusters[3]);
+    if (rc != TB200_OK) return rc;
+    const int KB = static_cast<int>((k + kBK - 1) / kBK), x_rows = static_cast<int>((m + 7) / 8 * 8);
+    float best = 0.0f;
+    for (int i = 0; i < 4; ++i) {
+        const int shares = 1 << i;
+        if (shares > KB) break;                                  // every share has a stage
+        for (int w = 8; w <= kHalf; w += 8) {
+            const int64_t tiles = (f + w - 1) / w;
+            if (shares > 1 && tiles > clusters[i]) continue;     // shared tiles run in one wave
+            const int64_t waves = (tiles + clusters[i] - 1) / clusters[i], at_once = (tiles < clusters[i] ? tiles : clusters[i]) * shares;
+            const float link = static_cast<float>(x_rows + 2 * w) * (128.0f / 95e3f), hbm = static_cast<float>(at_once) * (2 * w) * (128.0f / 6.4e6f);
+            const float stage = fmaxf(0.25f, fmaxf(link, hbm));
+            const float t = static_cast<float>(waves) * static_cast<float>((KB + shares - 1) / shares) * stage +
+                            (shares > 1 ? 0.8f + static_cast<float>(m) * (8 * w) / 20e3f : 0.012f * w);
+            if (best == 0.0f || t < best) {
+                best = t;
+                *plan = {w, shares};
+            }
+        }
+    }
+    return TB200_OK;
+}
+
+template <typename T, int ACT, int SHARES>
+int launch_mid(const MidMaps& maps, const MidArgs& args, cudaStream_t st) {
+    auto kern = k_ffn_mid<T, ACT, SHARES>;
+    static PerDeviceInt attr_set;
+    const int rc = ensure_max_smem(attr_set, reinterpret_cast<const void*>(kern), kMidSmemBytes);
+    if (rc != TB200_OK) return rc;
+    const int tiles = (args.f + args.w - 1) / args.w;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(SHARES > 1 ? tiles * SHARES : tiles < num_sms() ? tiles : num_sms()), 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = kMidSmemBytes;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = SHARES;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = SHARES > 1 ? 1 : 0;
+    TB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, maps, args));
+    return TB200_OK;
+}
+
+template <typename T, int ACT>
+int launch_mid_shares(const MidMaps& maps, const MidArgs& args, int shares, cudaStream_t st) {
+    switch (shares) {
+        case 1: return launch_mid<T, ACT, 1>(maps, args, st);
+        case 2: return launch_mid<T, ACT, 2>(maps, args, st);
+        case 4: return launch_mid<T, ACT, 4>(maps, args, st);
+        default: return launch_mid<T, ACT, 8>(maps, args, st);
+    }
+}
+
+template <typename T>
+int ffn_mid(const void* x, const void* wg, const void* wu, void* h, int64_t m, int64_t f, int64_t k, int64_t ldx, int act, cudaStream_t st) {
+    MidPlan plan = {kHalf, 1};
+    int rc = mid_plan(m, f, k, &plan);
+    if (rc != TB200_OK) return rc;
+    MidArgs args = {};
+    args.h = h;
+    args.m = static_cast<int>(m);
+    args.f = static_cast<int>(f);
+    args.depth = static_cast<int>(k);
+    args.w = plan.w;
+    args.x_rows = static_cast<int>((m + 7) / 8 * 8);
+    const int stage = (args.x_rows + 2 * plan.w) * 128;
+    args.stages = kMidRing / stage < kMaxStages ? kMidRing / stage : kMaxStages;
+    MidMaps maps;
+    memset(&maps, 0, sizeof(maps));
+    rc = map_k<T>(&maps.x, x, m, k, ldx, args.x_rows);
+    if (rc == TB200_OK) rc = map_k<T>(&maps.wg, wg, f, k, k, plan.w);
+    if (rc == TB200_OK) rc = map_k<T>(&maps.wu, wu, f, k, k, plan.w);
+    if (rc != TB200_OK) return rc;
+    switch (act) {
+        case TB200_ACT_SILU: return launch_mid_shares<T, TB200_ACT_SILU>(maps, args, plan.shares, st);
+        case TB200_ACT_GELU: return launch_mid_shares<T, TB200_ACT_GELU>(maps, args, plan.shares, st);
+        case TB200_ACT_GELU_TANH: return launch_mid_shares<T, TB200_ACT_GELU_TANH>(maps, args, plan.shares, st);
+        default: return launch_mid_shares<T, TB200_ACT_RELU>(maps, args, plan.shares, st);
+    }
+}
+
+// Hidden units per tile of the pair kernel: 128, or the multiple of 8 that leaves the least idle at the end.  A wave
+// costs its tiles' width and some 8 more; below 64 a stage is bound by issuing it.
+int pair_width(int64_t m, int64_t f) {
+    const int64_t pairs = num_sms() / 2, tm = (m + 2 * kHalf - 1) / (2 * kHalf);
+    int best = kHalf;
+    int64_t least = 0;
+    for (int w = kHalf; w >= 64; w -= 8) {
+        const int64_t cost = (tm * ((f + w - 1) / w) + pairs - 1) / pairs * (w + 8);
+        if (least == 0 || cost < least) {
+            least = cost;
+            best = w;
+        }
+    }
+    return best;
+}
+
 template <typename T>
 int ffn_forward(const void* x, const void* wg, const void* wu, void* h, void* gq, float* gs, void* uq, float* us, int64_t m, int64_t f,
                 int64_t k, int64_t ldx, int act, cudaStream_t st) {
+    const int w = gq ? kHalf : pair_width(m, f);
     FfnMaps maps;
     memset(&maps, 0, sizeof(maps));
     int rc = map_k<T>(&maps.a[0], x, m, k, ldx);
-    if (rc == TB200_OK) rc = map_k<T>(&maps.b[0], wg, f, k, k);
-    if (rc == TB200_OK) rc = map_k<T>(&maps.b[1], wu, f, k, k);
+    if (rc == TB200_OK) rc = map_k<T>(&maps.b[0], wg, f, k, k, w);
+    if (rc == TB200_OK) rc = map_k<T>(&maps.b[1], wu, f, k, k, w);
     if (rc != TB200_OK) return rc;
     FfnArgs args = {};
+    args.w = w;
     args.out[0] = h;
     args.rows = static_cast<int>(m);
     args.cols = static_cast<int>(f);
@@ -434,10 +872,44 @@ int ffn_forward(const void* x, const void* wg, const void* wu, void* h, void* gq
     return gq ? launch_fwd<T, true>(maps, args, act, st) : launch_fwd<T, false>(maps, args, act, st);
 }
 
-// dg, du: [m, ldg]; x: [m, k]
+// Shares of dx's contraction, where its tiles are too few for the pairs of SMs: the number with the fewest stages in a
+// row.  A tile costs some 6 stages beside its own; shares are written and added up in 32 bits, at 5 TB/s, by a kernel
+// that costs some 10 more (a stage is 0.27 us).
+int dx_splits(int64_t m, int64_t f, int64_t k) {
+    const int64_t pairs = num_sms() / 2, tiles = ((m + 2 * kHalf - 1) / (2 * kHalf)) * ((k + 2 * kHalf - 1) / (2 * kHalf));
+    const int64_t steps = 2 * ((f + kBK - 1) / kBK);
+    int best = 1;
+    double least = 0.0;
+    for (int s = 1; s <= 8 && steps >= 16 * (s - 1); ++s) {
+        const double cost = static_cast<double>((tiles * s + pairs - 1) / pairs) * ((steps + s - 1) / s + 6) +
+                            (s > 1 ? 10.0 + static_cast<double>(m) * k * 8.0 * s / (5e6 * 0.27) : 0.0);
+        if (s == 1 || cost < least) {
+            least = cost;
+            best = s;
+        }
+    }
+    return best;
+}
+
+// out = the sum of `splits` arrays of n numbers, in order; 8 numbers per thread.
+template <typename T>
+__global__ void __launch_bounds__(256) k_sum_shares(const float4* __restrict__ sums, uint4* __restrict__ out, int64_t n8, int splits) {
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n8; i += static_cast<int64_t>(gridDim.x) * 256) {
+        float4 a = sums[2 * i], b = sums[2 * i + 1];
+#pragma unroll 4
+        for (int s = 1; s < splits; ++s) {
+            const float4 c = sums[2 * (s * n8 + i)], d = sums[2 * (s * n8 + i) + 1];
+            a.x += c.x; a.y += c.y; a.z += c.z; a.w += c.w;
+            b.x += d.x; b.y += d.y; b.z += d.z; b.w += d.w;
+        }
+        out[i] = make_uint4(ActType<T>::pack(a.x, a.y), ActType<T>::pack(a.z, a.w), ActType<T>::pack(b.x, b.y), ActType<T>::pack(b.z, b.w));
+    }
+}
+
+// dg, du: [m, ldg]; x: [m, k]; sums: room for dx_splits() arrays of [m, k] where that is more than 1
 template <typename T>
 int ffn_products_bwd(const void* dg, const void* du, int64_t ldg, const void* x, int64_t ldx, const void* wg, const void* wu, void* dx, void* dwg,
-                     void* dwu, int64_t m, int64_t f, int64_t k, cudaStream_t st) {
+                     void* dwu, float* sums, int64_t m, int64_t f, int64_t k, cudaStream_t st) {
     FfnMaps maps;
     memset(&maps, 0, sizeof(maps));
     int rc = map_k<T>(&maps.a[0], dg, m, f, ldg);
@@ -451,8 +923,16 @@ int ffn_products_bwd(const void* dg, const void* du, int64_t ldg, const void* x,
     args.cols = static_cast<int>(k);
     args.depth = static_cast<int>(f);
     args.ldo = k;
+    args.splits = dx_splits(m, f, k);
+    args.sums = sums;
     rc = launch_pair<FK_DX, T, 0, false>(maps, args, st);
     if (rc != TB200_OK) return rc;
+    if (args.splits > 1) {
+        const int64_t n8 = m * (k / 8), ctas = (n8 + 255) / 256, cap = static_cast<int64_t>(num_sms()) * 8;
+        k_sum_shares<T><<<static_cast<unsigned>(ctas < cap ? ctas : cap), 256, 0, st>>>(reinterpret_cast<const float4*>(sums), static_cast<uint4*>(dx),
+                                                                                      n8, args.splits);
+        TB200_CUDA_TRY(cudaGetLastError());
+    }
 
     memset(&maps, 0, sizeof(maps));
     rc = map_mn<T>(&maps.a[0], dg, m, f, ldg);
@@ -499,13 +979,21 @@ extern "C" int tb200_ffn_gated(const void* x, const void* wg, const void* wu, vo
     if (ldx < k || ldx % 8 != 0) return fail(TB200_ERR_ALIGN, "ffn_gated: row stride of x %lld must be a multiple of 8 and at least k", (long long)ldx);
     if (!aligned16(x) || !aligned16(wg) || !aligned16(wu)) return fail(TB200_ERR_ALIGN, "ffn_gated: x, wg, wu must be 16-byte aligned");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    // Up to 128 rows one CTA's accumulator holds them all and narrow tiles share the weights out evenly (1 row of 4096 ->
+    // 14336: 41 us against the pair kernel's 70); beyond, two CTAs share each weight tile.  Checkpoints need whole
+    // 128-wide blocks, which the pair kernel's tiles are.
+    if (!given && m <= kHalf)
+        return dtype == TB200_DT_F16 ? ffn_mid<__half>(x, wg, wu, h, m, f, k, ldx, act, st)
+                                     : ffn_mid<__nv_bfloat16>(x, wg, wu, h, m, f, k, ldx, act, st);
     return dtype == TB200_DT_F16 ? ffn_forward<__half>(x, wg, wu, h, gq, gs, uq, us, m, f, k, ldx, act, st)
                                  : ffn_forward<__nv_bfloat16>(x, wg, wu, h, gq, gs, uq, us, m, f, k, ldx, act, st);
 }
 
 extern "C" size_t tb200_ffn_gated_bwd_workspace_bytes(int64_t m, int64_t f, int64_t k, int x_codes) {
     if (m <= 0 || f <= 0 || k <= 0) return 0;
-    return static_cast<size_t>(2 * round_up(m * pitch_of(f) * 2, 256) + (x_codes ? round_up(m * k * 2, 256) : 0));
+    const int64_t splits = dx_splits(m, f, k);
+    return static_cast<size_t>(2 * round_up(m * pitch_of(f) * 2, 256) + (x_codes ? round_up(m * k * 2, 256) : 0) +
+                               (splits > 1 ? splits * m * k * 4 : 0));
 }
 
 extern "C" int tb200_ffn_gated_bwd(const void* dh, const void* wg, const void* wu, const void* x, const float* xs, const void* gq,
@@ -537,6 +1025,7 @@ extern "C" int tb200_ffn_gated_bwd(const void* dh, const void* wg, const void* w
     void* dg = ws;
     void* du = ws + round_up(m * ldg * 2, 256);
     void* xr = ws + 2 * round_up(m * ldg * 2, 256);
+    float* sums = reinterpret_cast<float*>(static_cast<uint8_t*>(xr) + (codes ? round_up(m * k * 2, 256) : 0));
     rc = launch_gated_act_bwd(dh, gq, gs, uq, us, dg, du, m, f, ldg, act, dtype, st);
     if (rc != TB200_OK) return rc;
     if (codes) {
@@ -544,6 +1033,6 @@ extern "C" int tb200_ffn_gated_bwd(const void* dh, const void* wg, const void* w
         if (rc != TB200_OK) return rc;
         x = xr;
     }
-    return dtype == TB200_DT_F16 ? ffn_products_bwd<__half>(dg, du, ldg, x, ldx, wg, wu, dx, dwg, dwu, m, f, k, st)
-                                 : ffn_products_bwd<__nv_bfloat16>(dg, du, ldg, x, ldx, wg, wu, dx, dwg, dwu, m, f, k, st);
+    return dtype == TB200_DT_F16 ? ffn_products_bwd<__half>(dg, du, ldg, x, ldx, wg, wu, dx, dwg, dwu, sums, m, f, k, st)
+                                 : ffn_products_bwd<__nv_bfloat16>(dg, du, ldg, x, ldx, wg, wu, dx, dwg, dwu, sums, m, f, k, st);
 }
