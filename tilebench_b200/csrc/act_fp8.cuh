@@ -89,10 +89,27 @@ template <> struct ActType<__nv_bfloat16> {
 // ---- gate functions: f(g), and f'(g) ---------------------------------------------------------------------------
 // All in fp32.  The fast exponential and divide are off by some 2^-21 of the value, far below the 2^-9 (bf16) or
 // 2^-12 (fp16) of the rounding that follows.  The error-function and tanh forms are written so that nothing cancels
-// for large negative g: erfc instead of 1 + erf, and (1 + tanh z) / 2 as the logistic function of 2 z.
+// for large negative g: the normal tail instead of 1 + erf, and (1 + tanh z) / 2 as the logistic function of 2 z.
 __device__ __forceinline__ float gate_logistic(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
 
-constexpr float kSqrtHalf = 0.70710678118654752440f;
+// (Phi(g), exp(-g^2 / 2)) of the normal distribution.  The tail is Phi(-|g|) = exp(-g^2 / 2) t P(t) with
+// t = 1 / (1 + 0.3 |g|); P has degree 7 and was fitted here to exp(g^2 / 2) erfc(|g| / sqrt 2) / (2 t), least largest relative error
+// over |g| <= 14: 1.5e-7.  In 32 bits it comes to 1.3e-6 of the value at |g| = 8, less nearer to zero.  CUDA's erfcf in its
+// place took 6.9 us of a 128 x 256 accumulator's epilogue where the whole of it takes 3.
+__device__ __forceinline__ float2 gate_normal(float g) {
+    const float z = fabsf(g), e = __expf(-0.5f * g * g), t = __fdividef(1.0f, fmaf(0.3f, z, 1.0f));
+    float p = 0.03567477688193321f;
+    p = fmaf(p, t, -0.15720310807228088f);
+    p = fmaf(p, t, 0.20635353028774261f);
+    p = fmaf(p, t, -0.05368367210030556f);
+    p = fmaf(p, t, 0.12856164574623108f);
+    p = fmaf(p, t, 0.09991348534822464f);
+    p = fmaf(p, t, 0.12075395882129669f);
+    p = fmaf(p, t, 0.11962930113077164f);
+    const float tail = p * t * e;
+    return make_float2(g < 0.0f ? tail : 1.0f - tail, e);
+}
+
 constexpr float kInvSqrt2Pi = 0.39894228040143267794f;
 constexpr float kTanhA = 0.79788456080286535588f;               // sqrt(2 / pi)
 constexpr float kTanhB = 0.044715f;
@@ -102,7 +119,7 @@ __device__ __forceinline__ float gate_value(float g) {
     if constexpr (ACT == TB200_ACT_SILU) {
         return g * gate_logistic(g);
     } else if constexpr (ACT == TB200_ACT_GELU) {
-        return 0.5f * g * erfcf(-g * kSqrtHalf);
+        return g * gate_normal(g).x;
     } else if constexpr (ACT == TB200_ACT_GELU_TANH) {
         return g * gate_logistic(2.0f * kTanhA * (g + kTanhB * g * g * g));
     } else {
@@ -116,8 +133,8 @@ __device__ __forceinline__ float2 gate_both(float g) {
         const float s = gate_logistic(g);
         return make_float2(g * s, s * (1.0f + g * (1.0f - s)));
     } else if constexpr (ACT == TB200_ACT_GELU) {
-        const float p = 0.5f * erfcf(-g * kSqrtHalf);
-        return make_float2(g * p, p + g * kInvSqrt2Pi * __expf(-0.5f * g * g));
+        const float2 n = gate_normal(g);
+        return make_float2(g * n.x, n.x + g * kInvSqrt2Pi * n.y);
     } else if constexpr (ACT == TB200_ACT_GELU_TANH) {
         const float s = gate_logistic(2.0f * kTanhA * (g + kTanhB * g * g * g));
         return make_float2(g * s, s + 2.0f * g * s * (1.0f - s) * kTanhA * (1.0f + 3.0f * kTanhB * g * g));

@@ -29,10 +29,11 @@ constexpr int kStages = 6;
 constexpr int kOperandBytes = kHalf * 128;
 constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kAtomBytes = kBK * 128;            // MN-major: one box of 64 contraction rows x 64 columns
-constexpr int kEpiWarps = 8;                     // two per quarter of the tensor memory's lanes
-constexpr int kStagingBytes = 32 * 128;          // per epilogue warp: 32 rows of 128 bytes
+constexpr int kEpiWarps = 16;                    // four per quarter of the tensor memory's lanes (32 rows), each a quarter of the columns
+constexpr int kStagingBytes = 32 * 256;          // per quarter: 32 rows of 256 bytes
+constexpr int kAmaxBytes = 4 * 32 * 8;           // per quarter: 32 rows' amax of g and of u
 constexpr int kBarBytes = 256;
-constexpr int kSmemBytes = kStages * kStageBytes + kEpiWarps * kStagingBytes + kBarBytes + 1024;
+constexpr int kSmemBytes = kStages * kStageBytes + 4 * kStagingBytes + kAmaxBytes + kBarBytes + 1024;
 constexpr int kTmemCols = 512;
 constexpr int kThreads = 128 + 32 * kEpiWarps;   // TMA, MMA, two idle warps, epilogue
 constexpr int kGroupM = 8;                       // tiles are walked in bands of 8 x 256 rows, so that B's tiles stay in L2
@@ -76,63 +77,91 @@ __device__ __forceinline__ void mma_if(uint32_t issue, uint32_t d_tmem, uint64_t
 }
 
 // ---- epilogue helpers --------------------------------------------------------------------------------------------
-// A warp collects 32 rows of 128 bytes in shared memory, 16-byte piece c of row r at place c ^ (r & 7) (free of bank
-// conflicts both ways), and writes them out with neighbouring lanes on neighbouring bytes.
-__device__ __forceinline__ uint8_t* staged(uint8_t* buf, int row, int piece) { return buf + row * 128 + ((piece ^ (row & 7)) << 4); }
+// The four warps of a quarter collect 32 rows of 256 bytes in shared memory, 16-byte piece c of row r at place
+// c ^ (r & 15) (free of bank conflicts both ways); then each writes 8 of the rows out, neighbouring lanes on neighbouring bytes.
+__device__ __forceinline__ uint8_t* staged(uint8_t* buf, int row, int piece) { return buf + row * 256 + ((piece ^ (row & 15)) << 4); }
+__device__ __forceinline__ uint32_t shared_uint(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint32_t shared_byte(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint4 shared_uint4(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ void quarter_sync(int quarter) { asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory"); }
 
-// Pieces [first, first + COUNT) of each row go to row r of dst; rows and columns beyond the valid ones are left out.
-// T: the element.  Rows that begin on 16-byte boundaries take 16-byte stores as they are.  Others (f is odd, say) take
-// 16-byte stores too, of five words shifted into place, between single elements at either end of the row.
-template <typename T, int COUNT>
-__device__ __forceinline__ void flush(uint8_t* buf, int first, T* __restrict__ dst, int64_t pitch, int rows, int cols, int lane) {
-    constexpr int kPer = 32 / COUNT, kSize = sizeof(T);
-    const int bytes = min(cols, COUNT * 16 / kSize) * kSize, sub = lane / COUNT, c = lane % COUNT;
-    rows = min(rows, 32);
-    if (bytes <= 0) return;
+// Columns [0, cols) of rows [r0, min(r0 + 8, rows)), r0 a multiple of 8, which begin at piece `first` (0 or 8), go to row r of
+// dst; at most PIECES pieces of a row.  Rows that begin on 16-byte boundaries take 16-byte stores.  Others (f is odd, say) take a
+// warp each: aligned words, shifted into place, and single bytes at either end.  Row r0 + i lies i * 256 bytes on, its piece c at
+// place (c ^ r0 & 8) ^ i, which leaves one instruction per row to find a piece.
+template <typename T, int PIECES>
+__device__ __forceinline__ void flush(uint8_t* buf, int first, T* __restrict__ dst, int64_t pitch, int r0, int rows, int cols, int lane) {
+    constexpr int kSize = sizeof(T), kPer = 32 / PIECES;
+    const int bytes = min(cols * kSize, PIECES * 16), n = min(8, rows - r0);
+    if (bytes <= 0 || n <= 0) return;
+    const uint32_t base = smem_u32(buf) + r0 * 256;
     if (((reinterpret_cast<uintptr_t>(dst) | static_cast<uintptr_t>(pitch * kSize)) & 15) == 0) {
-#pragma unroll 4
-        for (int r = sub; r < rows; r += kPer) {
-            const uint8_t* src = staged(buf, r, first + c);
-            T* p = dst + r * pitch + c * (16 / kSize);
-            if (16 * c + 16 <= bytes) {
-                *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(src);
-            } else {
-                for (int i = 0; 16 * c + i * kSize < bytes; ++i) p[i] = reinterpret_cast<const T*>(src)[i];
+        const int c = lane % PIECES, sub = lane / PIECES;
+        const uint32_t place = static_cast<uint32_t>((first + c) ^ (r0 & 8) ^ sub) << 4;
+        uint8_t* p = reinterpret_cast<uint8_t*>(dst + (r0 + sub) * pitch) + 16 * c;
+        if (16 * c + 16 <= bytes) {
+#pragma unroll
+            for (int i = 0; i < 8; i += kPer) {
+                if (i + sub < n) *reinterpret_cast<uint4*>(p + i * pitch * kSize) = shared_uint4(base + sub * 256 + i * 256 + (place ^ (i << 4)));
+            }
+        } else if (16 * c < bytes) {
+            for (int i = 0; i + sub < n; i += kPer) {
+                const T* src = reinterpret_cast<const T*>(staged(buf, r0 + i + sub, first + c));
+                for (int e = 0; 16 * c + e * kSize < bytes; ++e) reinterpret_cast<T*>(p + i * pitch * kSize)[e] = src[e];
             }
         }
     } else {
-#pragma unroll 2
-        for (int r = sub; r < rows; r += kPer) {
-            uint8_t* p = reinterpret_cast<uint8_t*>(dst + r * pitch);
-            const int head = min(bytes, static_cast<int>(-reinterpret_cast<uintptr_t>(p) & 15)), tail = (bytes - head) & 15;
-            const int at = head + 16 * c;
-            if (at + 16 <= bytes) {
-                uint32_t w[5];
+        // all words first, so that the rows do not wait for one another
+        constexpr int kWords = PIECES / 8;
+        const uint32_t place = (static_cast<uint32_t>((first + (lane >> 2)) ^ (r0 & 8)) << 4) + (lane & 3) * 4;
+        uint8_t* const p0 = reinterpret_cast<uint8_t*>(dst + r0 * pitch);
+        uint32_t w[8][kWords];
 #pragma unroll
-                for (int i = 0; i < 5; ++i) {
-                    const int word = min(at / 4 + i, 4 * COUNT - 1);        // the fifth is not used where it would lie behind the row
-                    w[i] = *reinterpret_cast<const uint32_t*>(staged(buf, r, first + word / 4) + (word & 3) * 4);
-                }
-                const uint32_t sh = (at & 3) * 8;
-                *reinterpret_cast<uint4*>(p + at) = make_uint4(__funnelshift_r(w[0], w[1], sh), __funnelshift_r(w[1], w[2], sh),
-                                                               __funnelshift_r(w[2], w[3], sh), __funnelshift_r(w[3], w[4], sh));
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < kWords; ++j) w[i][j] = shared_uint(base + i * 256 + (place ^ (j << 7) ^ (i << 4)));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            uint8_t* const p = p0 + i * pitch * kSize;
+            const int mis = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 3), valid = i < n ? bytes : 0;
+            uint32_t before = 0;
+#pragma unroll
+            for (int j = 0; j < kWords; ++j) {                   // lane l has the word that lies 4 (32 j + l) - mis bytes into the row
+                const uint32_t w0 = __shfl_sync(0xffffffffu, lane == 31 ? before : w[i][j], (lane + 31) & 31);
+                const int b = 4 * (32 * j + lane) - mis;
+                if (b >= 0 && b + 4 <= valid) *reinterpret_cast<uint32_t*>(p + b) = __funnelshift_l(w0, w[i][j], 8 * mis);
+                before = w[i][j];
             }
-            for (int e = c; e * kSize < head + tail; e += COUNT) {
-                const int b = e * kSize < head ? e * kSize : bytes - tail + e * kSize - head;
-                *reinterpret_cast<T*>(p + b) = *reinterpret_cast<const T*>(staged(buf, r, first + b / 16) + (b & 15));
-            }
+            const int head = min(-mis & 3, valid), tail = (valid - head) & 3, b = lane < head ? lane : valid - tail + lane - head;
+            if (lane < head + tail) p[b] = static_cast<uint8_t>(shared_byte(base + i * 256 + ((((first + (b >> 4)) ^ (r0 & 8) ^ i) << 4) | (b & 15))));
         }
     }
 }
 
+// 16-bit numbers of 32 columns as 4 pieces, codes of 32 columns as 2
 template <typename T>
-__device__ __forceinline__ void stage32(uint8_t* buf, int row, int piece0, const float (&v)[32]) {      // 32 columns: 4 pieces
+__device__ __forceinline__ void stage32(uint8_t* buf, int row, int piece0, const uint32_t (&v)[32]) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<uint4*>(staged(buf, row, piece0 + q)) = make_uint4(ActType<T>::pack(v[8 * q], v[8 * q + 1]), ActType<T>::pack(v[8 * q + 2], v[8 * q + 3]),
-                                                                             ActType<T>::pack(v[8 * q + 4], v[8 * q + 5]), ActType<T>::pack(v[8 * q + 6], v[8 * q + 7]));
+    for (int q = 0; q < 4; ++q) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = ActType<T>::pack(__uint_as_float(v[8 * q + 2 * e]), __uint_as_float(v[8 * q + 2 * e + 1]));
+        *reinterpret_cast<uint4*>(staged(buf, row, piece0 + q)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
 }
-__device__ __forceinline__ void stage_codes32(uint8_t* buf, int row, int piece0, const uint32_t (&v)[32], float inv, bool checked) {  // 2 pieces
+__device__ __forceinline__ void stage_codes32(uint8_t* buf, int row, int piece0, const uint32_t (&v)[32], float inv, bool checked) {
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
         uint32_t w[4];
@@ -145,12 +174,11 @@ __device__ __forceinline__ void stage_codes32(uint8_t* buf, int row, int piece0,
         *reinterpret_cast<uint4*>(staged(buf, row, piece0 + q)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
-__device__ __forceinline__ void pair_of_warps_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
 template <int ACT>
-__device__ __forceinline__ void gated32(const uint32_t (&g)[32], const uint32_t (&u)[32], float (&h)[32]) {
+__device__ __forceinline__ void gated32(uint32_t (&g)[32], const uint32_t (&u)[32]) {       // h in the place of g
 #pragma unroll
-    for (int i = 0; i < 32; ++i) h[i] = gate_value<ACT>(__uint_as_float(g[i])) * __uint_as_float(u[i]);
+    for (int i = 0; i < 32; ++i) g[i] = __float_as_uint(gate_value<ACT>(__uint_as_float(g[i])) * __uint_as_float(u[i]));
 }
 
 // First step of share i of n.
@@ -174,7 +202,8 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* staging = smem + S * kStageBytes;
-    uint64_t* bar_full = reinterpret_cast<uint64_t*>(staging + kEpiWarps * kStagingBytes);
+    uint32_t* amax = reinterpret_cast<uint32_t*>(staging + 4 * kStagingBytes);      // [quarter][g, u][row], bits of non-negative numbers
+    uint64_t* bar_full = reinterpret_cast<uint64_t*>(staging + 4 * kStagingBytes + kAmaxBytes);
     uint64_t* bar_empty = bar_full + S;
     uint64_t* bar_afull = bar_empty + S;          // [2] accumulator complete
     uint64_t* bar_aempty = bar_afull + 2;         // [2] accumulator read (the epilogue warps of both CTAs)
@@ -193,6 +222,7 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
     const int tiles = tiles_m * tiles_n;
     const int items = KIND == FK_DX ? tiles * p.splits : tiles; // dx: item i is share i / tiles of tile i % tiles
 
+    if (SAVE && threadIdx.x < kAmaxBytes / 4) amax[threadIdx.x] = 0;
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
             mbar_init(&bar_full[s], 1);
@@ -293,10 +323,10 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
             if (ok && leader) tc_commit_pair(&bar_afull[acc], 0x3);
         }
     } else if (warp >= 4) {
-        // ---------------- epilogue (both CTAs; each owns 128 rows of the tile, each warp 32 rows of one half of the columns) ----
-        const int ew = (warp - 4) & 3, half = (warp - 4) >> 2;
-        uint8_t* buf = staging + (warp - 4) * kStagingBytes;
-        const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(ew * 32) << 16);
+        // ---------------- epilogue (both CTAs; each owns 128 rows of the tile, each warp 32 rows of a quarter of the columns) ----
+        const int quarter = (warp - 4) & 3, part = (warp - 4) >> 2, r8 = 8 * part;
+        uint8_t* buf = staging + quarter * kStagingBytes;
+        const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
         uint32_t cnt = 0;
         bool ok = true;
         for (int t = pair; t < items; t += npairs, ++cnt) {
@@ -304,8 +334,9 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
             const Tile tc = tile_at(t - share * tiles, tiles_m, tiles_n);
             const int sel = KIND == FK_DW && tc.m >= tm1 ? 1 : 0;
             const uint32_t acc = cnt & 1;
-            const int row0 = (tc.m - sel * tm1) * 2 * kHalf + rank * kHalf + ew * 32;             // the warp's first row
+            const int row0 = (tc.m - sel * tm1) * 2 * kHalf + rank * kHalf + quarter * 32;        // the quarter's first row
             const int rows = p.rows - row0;                                                       // valid rows (may be <= 0)
+            const int col0 = tc.n * tile_cols, cols = p.cols - col0;
             const uint32_t t_acc = t_lane + acc * 256;
             // a wait that gave up ends the waiting, not the walk: the warps meet at barriers below
             ok = ok && mbar_wait(&bar_afull[acc], (cnt >> 1) & 1, ST_WAIT_TMEM_FULL, t);
@@ -316,113 +347,96 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
                 if (lane == 0) mbar_arrive_leader(&bar_aempty[acc]);
             };
             if constexpr (KIND == FK_FWD) {
-                // columns [at, at + n) of the tile, n <= 64; what is read beyond them belongs to nobody and is not stored
-                const int split = (tile_cols / 2 + 7) / 8 * 8, at = half * split, n = half == 0 ? split : tile_cols - split;
-                const int col0 = tc.n * tile_cols + at, cols = min(n, p.cols - col0);
+                // columns [at, at + 32) of the tile; what lies beyond its w columns belongs to nobody and is not stored
+                const int at = part * ((tile_cols / 4 + 7) / 8 * 8);
                 const uint32_t t_g = t_acc + at, t_u = t_acc + tile_cols + at;
                 uint32_t g[32], u[32];
-                float amax_g = 0.0f, amax_u = 0.0f;
-#pragma unroll 1
-                for (int c = 0; c < 2; ++c) {
-                    tmem_ld32(t_g + c * 32, g);
-                    tmem_ld32(t_u + c * 32, u);
+                tmem_ld32(t_g, g);
+                tmem_ld32(t_u, u);
+                tmem_wait_ld();
+                uint32_t* const row_amax = amax + quarter * 64 + lane;
+                if constexpr (SAVE) {
+                    float a = 0.0f, b = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        a = fmaxf(a, fabsf(__uint_as_float(g[i])));
+                        b = fmaxf(b, fabsf(__uint_as_float(u[i])));
+                    }
+                    atomicMax(row_amax, __float_as_uint(a));
+                    atomicMax(row_amax + 32, __float_as_uint(b));
+                } else {
+                    release();
+                }
+                gated32<ACT>(g, u);
+                stage32<T>(buf, lane, at / 8, g);
+                quarter_sync(quarter);
+                float ag = 0.0f, au = 0.0f;
+                if constexpr (SAVE) {
+                    ag = __uint_as_float(row_amax[0]);
+                    au = __uint_as_float(row_amax[32]);
+                }
+                flush<T, 16>(buf, 0, static_cast<T*>(p.out[0]) + static_cast<int64_t>(row0) * p.ldo + col0, p.ldo, r8, rows, min(cols, tile_cols), lane);
+                quarter_sync(quarter);
+                if constexpr (SAVE) {
+                    tmem_ld32(t_g, g);
+                    tmem_ld32(t_u, u);
                     tmem_wait_ld();
-                    if (!SAVE && c == 1) release();
-                    if constexpr (SAVE) {
+                    release();
+                    const bool infinite = __any_sync(0xffffffffu, fmaxf(ag, au) > FLT_MAX);       // the same in the quarter's warps
+                    if (infinite) {                              // once more, over the finite values
+                        if (part == 0) row_amax[0] = row_amax[32] = 0;
+                        quarter_sync(quarter);
+                        float a = 0.0f, b = 0.0f;
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
-                            amax_g = fmaxf(amax_g, fabsf(__uint_as_float(g[i])));
-                            amax_u = fmaxf(amax_u, fabsf(__uint_as_float(u[i])));
+                            a = fmaxf(a, act_size(__uint_as_float(g[i])));
+                            b = fmaxf(b, act_size(__uint_as_float(u[i])));
                         }
+                        atomicMax(row_amax, __float_as_uint(a));
+                        atomicMax(row_amax + 32, __float_as_uint(b));
+                        quarter_sync(quarter);
+                        ag = __uint_as_float(row_amax[0]);
+                        au = __uint_as_float(row_amax[32]);
                     }
-                    float h[32];
-                    gated32<ACT>(g, u, h);
-                    stage32<T>(buf, lane, 4 * c, h);
-                }
-                __syncwarp();
-                flush<T, 8>(buf, 0, static_cast<T*>(p.out[0]) + static_cast<int64_t>(row0) * p.ldo + col0, p.ldo, rows, cols, lane);
-                __syncwarp();
-                if constexpr (SAVE) {
-                    // the block's amax over both halves of the columns, exchanged through the staging buffers
-                    auto both = [&] {
-                        reinterpret_cast<float2*>(buf)[lane] = make_float2(amax_g, amax_u);
-                        pair_of_warps_sync(1 + ew);
-                        const float2 o = reinterpret_cast<const float2*>(staging + ((warp - 4) ^ 4) * kStagingBytes)[lane];
-                        amax_g = fmaxf(amax_g, o.x);
-                        amax_u = fmaxf(amax_u, o.y);
-                        pair_of_warps_sync(1 + ew);
-                    };
-                    both();
-                    const bool infinite = __any_sync(0xffffffffu, fmaxf(amax_g, amax_u) > FLT_MAX);   // the same in both warps
-                    if (infinite) {                              // once more, over the finite values
-                        amax_g = amax_u = 0.0f;
-#pragma unroll 1
-                        for (int c = 0; c < 2; ++c) {
-                            tmem_ld32(t_g + c * 32, g);
-                            tmem_ld32(t_u + c * 32, u);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                amax_g = fmaxf(amax_g, act_size(__uint_as_float(g[i])));
-                                amax_u = fmaxf(amax_u, act_size(__uint_as_float(u[i])));
-                            }
-                        }
-                        both();
-                    }
+                    const float2 sg = act_scale(ag), su = act_scale(au);
                     const int64_t nblk = (p.cols + kHalf - 1) / kHalf;
-                    const float2 sg = act_scale(amax_g), su = act_scale(amax_u);
-                    if (lane < rows) p.scales[half][(row0 + lane) * nblk + tc.n] = half == 0 ? sg.x : su.x;
-#pragma unroll 1
-                    for (int c = 0; c < 2; ++c) {
-                        tmem_ld32(t_g + c * 32, g);
-                        tmem_ld32(t_u + c * 32, u);
-                        tmem_wait_ld();
-                        if (c == 1) release();
-                        stage_codes32(buf, lane, 2 * c, g, sg.y, infinite);
-                        stage_codes32(buf, lane, 4 + 2 * c, u, su.y, infinite);
-                    }
-                    __syncwarp();
+                    if (part < 2 && lane < rows) p.scales[part][(row0 + lane) * nblk + tc.n] = part == 0 ? sg.x : su.x;
+                    stage_codes32(buf, lane, 2 * part, g, sg.y, infinite);
+                    stage_codes32(buf, lane, 8 + 2 * part, u, su.y, infinite);
+                    quarter_sync(quarter);
+                    if (part == 0) row_amax[0] = row_amax[32] = 0;                                // all have read it, none adds before the next barrier
                     const int64_t to = static_cast<int64_t>(row0) * p.cols + col0;
-                    flush<uint8_t, 4>(buf, 0, p.codes[0] + to, p.cols, rows, cols, lane);
-                    flush<uint8_t, 4>(buf, 4, p.codes[1] + to, p.cols, rows, cols, lane);
-                    __syncwarp();
+                    flush<uint8_t, 8>(buf, 0, p.codes[0] + to, p.cols, r8, rows, cols, lane);
+                    flush<uint8_t, 8>(buf, 8, p.codes[1] + to, p.cols, r8, rows, cols, lane);
+                    quarter_sync(quarter);
+                }
+            } else if (KIND == FK_DX && p.splits > 1) {          // partial sums in 32 bits, 64 columns at a time
+                float* dst = p.sums + (static_cast<int64_t>(share) * p.rows + row0) * p.cols + col0;
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t v[16];
+                    tmem_ld16(t_acc + c * 64 + part * 16, v);
+                    tmem_wait_ld();
+                    if (c == 3) release();
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(staged(buf, lane, 4 * part + q)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                    quarter_sync(quarter);
+                    flush<float, 16>(buf, 0, dst + c * 64, p.cols, r8, rows, cols - c * 64, lane);
+                    quarter_sync(quarter);
                 }
             } else {
-                const int col0 = tc.n * tile_cols + half * kHalf, cols = p.cols - col0;
-                const uint32_t t_col = t_acc + half * kHalf;
-                if (KIND == FK_DX && p.splits > 1) {             // partial sums in 32 bits, 32 columns at a time
-                    float* dst = p.sums + (static_cast<int64_t>(share) * p.rows + row0) * p.cols + col0;
-#pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t v[32];
-                        tmem_ld32(t_col + c * 32, v);
-                        tmem_wait_ld();
-                        if (c == 3) release();
+                T* dst = static_cast<T*>(p.out[sel]) + static_cast<int64_t>(row0) * p.ldo + col0;
+                uint32_t v[2][32];
+                tmem_ld32(t_acc + part * 32, v[0]);
+                tmem_ld32(t_acc + kHalf + part * 32, v[1]);
+                tmem_wait_ld();
+                release();
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(staged(buf, lane, q)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-                        __syncwarp();
-                        flush<float, 8>(buf, 0, dst + c * 32, p.cols, rows, cols - c * 32, lane);
-                        __syncwarp();
-                    }
-                } else {
-                    T* dst = static_cast<T*>(p.out[sel]) + static_cast<int64_t>(row0) * p.ldo + col0;
-#pragma unroll 1
-                    for (int c = 0; c < 2; ++c) {
-#pragma unroll
-                        for (int d = 0; d < 2; ++d) {
-                            uint32_t v[32];
-                            float w[32];
-                            tmem_ld32(t_col + c * 64 + d * 32, v);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) w[i] = __uint_as_float(v[i]);
-                            stage32<T>(buf, lane, 4 * d, w);
-                        }
-                        if (c == 1) release();
-                        __syncwarp();
-                        flush<T, 8>(buf, 0, dst + c * 64, p.ldo, rows, cols - c * 64, lane);
-                        __syncwarp();
-                    }
+                for (int c = 0; c < 2; ++c) {
+                    stage32<T>(buf, lane, 4 * part, v[c]);
+                    quarter_sync(quarter);
+                    flush<T, 16>(buf, 0, dst + c * kHalf, p.ldo, r8, rows, cols - c * kHalf, lane);
+                    quarter_sync(quarter);
                 }
             }
         }
@@ -453,7 +467,7 @@ struct MidArgs {
     int w, stages, x_rows;                       // hidden units per tile, stages in shared memory, rows of x per copy
 };
 constexpr int kMidRing = 192 * 1024;
-constexpr int kMidSmemBytes = kMidRing + kEpiWarps * kStagingBytes + kBarBytes + 1024;
+constexpr int kMidSmemBytes = kMidRing + 4 * kStagingBytes + kBarBytes + 1024;
 
 __device__ __forceinline__ float4 peer_float4(uint32_t addr, uint32_t rank) {
     uint32_t at;
@@ -468,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ffn_mid(const __grid_constant__
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* staging = smem + kMidRing;
-    uint64_t* bar_full = reinterpret_cast<uint64_t*>(staging + kEpiWarps * kStagingBytes);
+    uint64_t* bar_full = reinterpret_cast<uint64_t*>(staging + 4 * kStagingBytes);
     uint64_t* bar_empty = bar_full + kMaxStages;
     uint64_t* bar_afull = bar_empty + kMaxStages;
     uint64_t* bar_aempty = bar_afull + 2;
@@ -563,56 +577,53 @@ __global__ void __launch_bounds__(kThreads, 1) k_ffn_mid(const __grid_constant__
             if (ok && leader) tc_commit(&bar_afull[acc]);
         }
     } else if (warp >= 4) {
-        // ---------------- epilogue: a warp has 32 rows of one half of the columns ----------------
-        const int ew = (warp - 4) & 3, half = (warp - 4) >> 2;
-        uint8_t* buf = staging + (warp - 4) * kStagingBytes;
-        const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(ew * 32) << 16);
+        // ---------------- epilogue: a warp has 32 rows of a quarter of the columns ----------------
+        const int quarter = (warp - 4) & 3, part = (warp - 4) >> 2, row0 = quarter * 32;
+        uint8_t* buf = staging + quarter * kStagingBytes;
+        const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
         uint32_t cnt = 0;
         bool ok = true;
-        for (int t = t0; t < tiles && ok; t += t_step, ++cnt) {
+        for (int t = t0; t < tiles; t += t_step, ++cnt) {
             const uint32_t acc = cnt & 1;
-            if (!mbar_wait(&bar_afull[acc], (cnt >> 1) & 1, ST_WAIT_TMEM_FULL, t)) { ok = false; break; }
+            // a wait that gave up ends the waiting, not the walk: the warps meet at barriers below
+            ok = ok && mbar_wait(&bar_afull[acc], (cnt >> 1) & 1, ST_WAIT_TMEM_FULL, t);
             tc_fence_after();
             const uint32_t t_acc = t_lane + acc * 256;
-            const int row0 = ew * 32;
             if constexpr (SPLIT) {
-                // this CTA's sums, row by row: one half of the warps g, the other u.  A row pitch of 4 more than a multiple of
-                // 16 keeps eight lanes' (rows') 16-byte pieces on different banks.  Every copy into the ring has landed and been
-                // used by the time the accumulator is complete.
-                float* mine = reinterpret_cast<float*>(smem) + (row0 + lane) * (2 * w + 4) + half * w;
+                // this CTA's sums, row by row.  A row pitch of 4 more than a multiple of 16 keeps eight lanes' (rows')
+                // 16-byte pieces on different banks.  Every copy into the ring has landed and been used by the time the
+                // accumulator is complete.
                 if (row0 < p.m) {
+                    const int at = part * ((w / 2 + 7) / 8 * 8), n = min((w / 2 + 7) / 8 * 8, 2 * w - at);
+                    float* mine = reinterpret_cast<float*>(smem) + (row0 + lane) * (2 * w + 4) + at;
 #pragma unroll 1
-                    for (int c = 0; c < w; c += 16) {
+                    for (int c = 0; c < n; c += 16) {
                         uint32_t v[16];
-                        tmem_ld16(t_acc + half * w + c, v);
+                        tmem_ld16(t_acc + at + c, v);
                         tmem_wait_ld();
                         if (row0 + lane < p.m) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
-                                if (c + 4 * i < w) *reinterpret_cast<uint4*>(mine + c + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                                if (c + 4 * i < n) *reinterpret_cast<uint4*>(mine + c + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
                         }
                     }
                 }
             } else {
-                const int split = (w / 2 + 7) / 8 * 8, at = half * split, n = half == 0 ? split : w - split;
-                const int col0 = t * w + at, cols = min(n, p.f - col0);
-#pragma unroll 1
-                for (int c = 0; c < 2; ++c) {
-                    if (row0 < p.m && c * 32 < n) {
-                        uint32_t g[32], u[32];
-                        tmem_ld32(t_acc + at + c * 32, g);
-                        tmem_ld32(t_acc + w + at + c * 32, u);
-                        tmem_wait_ld();
-                        float h[32];
-                        gated32<ACT>(g, u, h);
-                        stage32<T>(buf, lane, 4 * c, h);
-                    }
+                const int at = part * ((w / 4 + 7) / 8 * 8);
+                if (row0 < p.m && at < w) {
+                    uint32_t g[32], u[32];
+                    tmem_ld32(t_acc + at, g);
+                    tmem_ld32(t_acc + w + at, u);
+                    tmem_wait_ld();
+                    gated32<ACT>(g, u);
+                    stage32<T>(buf, lane, at / 8, g);
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar_aempty[acc]);
-                flush<T, 8>(buf, 0, static_cast<T*>(p.h) + static_cast<int64_t>(row0) * p.f + col0, p.f, p.m - row0, cols, lane);
-                __syncwarp();
+                quarter_sync(quarter);
+                flush<T, 16>(buf, 0, static_cast<T*>(p.h) + static_cast<int64_t>(row0) * p.f + t * w, p.f, 8 * part, p.m - row0, min(w, p.f - t * w), lane);
+                quarter_sync(quarter);
             }
         }
     }
