@@ -3,8 +3,6 @@
 // by HBM: saving moves size + 1 bytes per element, restoring 1 + size, the backward step 4 in and 4 out.
 #include "act_fp8.cuh"
 
-#include <limits.h>
-
 namespace tb200 {
 namespace {
 
@@ -184,11 +182,11 @@ __global__ void __launch_bounds__(kThreads) k_restore(const uint8_t* __restrict_
 }
 
 // ---- any width, stride and alignment ---------------------------------------------------------------------------
-// A warp walks a span of one row in parts of 32 pieces of 4 N bytes, piece l in lane l.  Memory is accessed in aligned
-// pieces; where the row begins at another offset, a lane's piece is a window over its own aligned piece and the next
-// lane's (loads; lane 31 takes lane 0's of the part that follows, which is already there), or an aligned piece is a window over
-// the previous lane's codes and its own (stores).  Loads that reach outside the tensor and stores that reach outside
-// the span are made byte by byte.
+// A warp walks a span of one row in parts of 32 lanes with E neighbouring numbers each.  Loads are of aligned 4-byte words, one
+// more than the numbers fill, shifted into place: every lane of a row has the same shift, and the neighbour's word comes from
+// L1.  (16-byte pieces joined by shuffles and selects took a third more time: the kernels are bound by their instructions.)
+// Stores of codes are of aligned words too, of the previous lane's last codes and the lane's own.  Loads that reach outside
+// the tensor and stores that reach outside the span are made byte by byte.
 
 // The piece at byte `off` behind base (base + off is aligned); bytes outside [lo, hi) come as zeros.
 template <int N>
@@ -216,80 +214,46 @@ __device__ __forceinline__ void load_piece(const uint8_t* base, int off, int lo,
         }
     }
 }
-// One row's bytes [at, at + bytes) in parts, kAhead of them on the way.  The tensor is [begin, end).
+// The N + 1 aligned words around N words at p, whatever its alignment.  inside: they all lie inside the tensor [begin, end), in
+// every lane; where not, what does is fetched byte by byte.
 template <int N>
-struct Stream {
-    static constexpr int kAhead = 2, kPart = 32 * 4 * N;
-    const uint8_t* base;
-    int off, lo, hi, stop, mis;
-    uint32_t held[kAhead + 1][N];
-    __device__ __forceinline__ Stream(const uint8_t* at, int64_t bytes, const uint8_t* begin, const uint8_t* end, int lane) {
-        mis = static_cast<int>(reinterpret_cast<uintptr_t>(at) & (4 * N - 1));
-        base = at - mis;
-        off = lane * 4 * N;
-        lo = at - begin >= 4 * N ? 0 : max(0, mis - static_cast<int>(at - begin));
-        stop = mis + static_cast<int>(bytes);
-        hi = end - at >= bytes + 4 * N ? stop + 4 * N : mis + static_cast<int>(end - at);
+__device__ __forceinline__ void load_words(const uint8_t* p, const uint8_t* begin, const uint8_t* end, bool inside, uint32_t (&a)[N + 1]) {
+    const uint8_t* q = p - (reinterpret_cast<uintptr_t>(p) & 3);
+    if (inside) {
 #pragma unroll
-        for (int j = 0; j <= kAhead; ++j) load(j, j);
-    }
-    __device__ __forceinline__ void load(int j, int part) {
-        const int o = off + part * kPart;
-        load_piece<N>(base, o, o < stop ? lo : INT_MAX, hi, held[j]);
-    }
-    // The lane's piece of the current part; fetches the part kAhead + 1 further on and moves on by one.
-    __device__ __forceinline__ void next(int lane, uint32_t (&r)[N]) {
-        if (mis == 0) {
+        for (int i = 0; i <= N; ++i) a[i] = __ldg(reinterpret_cast<const uint32_t*>(q) + i);
+    } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i) r[i] = held[0][i];
-        } else {
-            uint32_t a[2 * N];
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                a[i] = held[0][i];
-                a[N + i] = __shfl_sync(0xffffffffu, lane == 0 ? held[1][i] : held[0][i], (lane + 1) & 31);
-            }
-            // words [mis / 4, mis / 4 + N], then mis % 4 bytes on
-#pragma unroll
-            for (int step = N / 2; step > 0; step >>= 1) {
-                const bool by = (mis & (4 * step)) != 0;
-#pragma unroll
-                for (int i = 0; i < N + step; ++i) a[i] = by ? a[i + step < 2 * N ? i + step : i] : a[i];
-            }
-#pragma unroll
-            for (int i = 0; i < N; ++i) r[i] = __funnelshift_r(a[i], a[i + 1], (mis & 3) * 8);
-        }
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j)
-#pragma unroll
-            for (int i = 0; i < N; ++i) held[j][i] = held[j + 1][i];
-        load(kAhead, kAhead + 1);
-        off += kPart;
-    }
-};
-template <int N>
-__device__ __forceinline__ void store_piece(uint8_t* base, int off, int lo, int hi, const uint32_t (&r)[N]) {
-    if (off >= lo && off + 4 * N <= hi) {
-        if constexpr (N == 2) *reinterpret_cast<uint2*>(base + off) = make_uint2(r[0], r[1]);
-        else *reinterpret_cast<uint32_t*>(base + off) = r[0];
-    } else if (off + 4 * N > lo && off < hi) {
+        for (int i = 0; i <= N; ++i) a[i] = 0;
 #pragma unroll 1
-        for (int i = max(0, lo - off); i < 4 * N && off + i < hi; ++i)
-            base[off + i] = static_cast<uint8_t>((N == 1 || i < 4 ? r[0] : r[N - 1]) >> (8 * (i & 3)));
+        for (int i = 0; i < 4 * N + 4 && q + i < end; ++i) {
+            if (q + i >= begin) {
+                const uint32_t byte = static_cast<uint32_t>(q[i]) << (8 * (i & 3));
+#pragma unroll
+                for (int w = 0; w <= N; ++w) a[w] |= i / 4 == w ? byte : 0;
+            }
+        }
     }
 }
-// The last `mis` bytes of one piece followed by the first of the next; N is 1 or 2, mis in [1, 4 N).
 template <int N>
-__device__ __forceinline__ void join_before(const uint32_t (&before)[N], const uint32_t (&r)[N], int mis, uint32_t (&out)[N]) {
-    static_assert(N == 1 || N == 2, "codes of 4 or 8 numbers");
-    const uint32_t sh = (mis & 3) * 8;
-    if constexpr (N == 1) {
-        out[0] = __funnelshift_l(before[0], r[0], sh);
-    } else {
-        const bool word = mis >= 4;
-        const uint32_t b0 = word ? before[0] : before[1], b1 = word ? before[1] : r[0], b2 = word ? r[0] : r[1];
-        out[0] = __funnelshift_l(b0, b1, sh);
-        out[1] = __funnelshift_l(b1, b2, sh);
+__device__ __forceinline__ void into_place(const uint32_t (&a)[N + 1], const uint8_t* p, uint32_t (&r)[N]) {
+    const uint32_t sh = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 3) * 8;
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = __funnelshift_r(a[i], a[i + 1], sh);
+}
+// Whether all words of a part whose lane 0 begins at p and whose lanes have N words each lie inside the tensor.
+template <int N>
+__device__ __forceinline__ bool part_inside(const uint8_t* p, const uint8_t* begin, const uint8_t* end) {
+    return p - (reinterpret_cast<uintptr_t>(p) & 3) >= begin && p + 32 * 4 * N + 4 <= end;
+}
+// Stores the word at byte b of a row's codes, as far as it lies in [lo, hi).
+__device__ __forceinline__ void store_word(uint8_t* row, int b, int lo, int hi, uint32_t w) {
+    if (b >= lo && b + 4 <= hi) {
+        *reinterpret_cast<uint32_t*>(row + b) = w;
+    } else if (b + 4 > lo && b < hi) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (b + i >= lo && b + i < hi) row[b + i] = static_cast<uint8_t>(w >> (8 * i));
     }
 }
 template <typename T> struct Part {
@@ -309,42 +273,39 @@ __global__ void __launch_bounds__(kThreads) k_save_any(const T* __restrict__ x, 
     for (int64_t s = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); s < spans; s += static_cast<int64_t>(gridDim.x) * (kThreads / 32)) {
         const int64_t row = s / per_row, first = (s - row * per_row) * width;
         const int n = static_cast<int>(min(static_cast<int64_t>(width), cols - first));
-        Stream<4> in(reinterpret_cast<const uint8_t*>(x + row * ldx + first), static_cast<int64_t>(n) * sizeof(T), begin, end, lane);
+        const uint8_t* const from = reinterpret_cast<const uint8_t*>(x + row * ldx + first);
         uint8_t* const to = q + row * cols + first;
         float* const sc = scales + row * nblk + first / kActBlock;
-        const int mis = static_cast<int>(reinterpret_cast<uintptr_t>(to) & (4 * N - 1));
-        uint32_t before[N] = {};                                 // lane 31's codes of the part before
-        int part = 0;
-#pragma unroll 1
-        for (int col = 0; col < n; col += kCols, ++part) {
-            uint32_t r[4], c[N], b[N], out[N];
+        const int mis = static_cast<int>(reinterpret_cast<uintptr_t>(to) & 3);
+        uint32_t before = 0;                                     // lane 31's last word of the part before
+        uint32_t ahead[5];                                       // the next part's words, on the way while one is worked on
+        auto fetch = [&](int col) {
+            const uint8_t* p = from + static_cast<int64_t>(col) * sizeof(T);
+            load_words<4>(p + lane * 16, begin, end, part_inside<4>(p, begin, end), ahead);
+        };
+        fetch(0);
+#pragma unroll 2
+        for (int col = 0; col < n; col += kCols) {
+            uint32_t r[4], c[N];
             float v[E];
-            in.next(lane, r);
-            numbers<T, 4>(r, v);
             const int at = col + lane * E;                       // the lane's first column in the span
+            into_place<4>(ahead, from, r);
+            if (col + kCols < n) fetch(col + kCols);
+            numbers<T, 4>(r, v);
             if (at + E > n) {
 #pragma unroll
                 for (int i = 0; i < E; ++i) v[i] = at + i < n ? v[i] : 0.0f;
             }
             const float scale = encode<E>(v, c);
             if (lane % kLanes == 0 && at < n) sc[at / kActBlock] = scale;
+            // aligned words: the last `mis` bytes of the codes before and the first of the lane's own
+            const uint32_t last = c[N - 1], first_before = __shfl_sync(0xffffffffu, lane == 31 ? before : last, (lane + 31) & 31);
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                b[i] = __shfl_sync(0xffffffffu, lane == 31 ? before[i] : c[i], (lane + 31) & 31);
-                before[i] = c[i];
-            }
-            if (mis != 0) {
-                join_before<N>(b, c, mis, out);
-                store_piece<N>(to - mis, at, mis, mis + n, out);
-            } else {
-                store_piece<N>(to, at, 0, n, c);
-            }
+            for (int i = 0; i < N; ++i) store_word(to, at + 4 * i - mis, 0, n, __funnelshift_l(i == 0 ? first_before : c[0], c[i], 8 * mis));
+            before = last;
         }
-        if (mis != 0 && lane == 31) {                            // the last lane's codes that belong to the piece behind it
-            uint32_t zero[N] = {}, out[N];
-            join_before<N>(before, zero, mis, out);
-            store_piece<N>(to - mis, part * kCols, mis, mis + n, out);
-        }
+        const int end = (n + kCols - 1) / kCols * kCols;         // codes of lane 31 that belong to the word behind the last part's
+        if (lane == 31 && mis != 0) store_word(to, end - mis, 0, n, __funnelshift_l(before, 0, 8 * mis));
     }
 }
 
@@ -486,26 +447,39 @@ __global__ void __launch_bounds__(kThreads) k_gated_bwd_any(const T* __restrict_
                                                             const uint8_t* __restrict__ uq, const float* __restrict__ us, T* __restrict__ dg,
                                                             T* __restrict__ du, int64_t spans, uint32_t per_row, int width, int64_t m, int64_t f,
                                                             int64_t ldg, uint32_t nblk) {
+    static_assert(sizeof(T) == 2, "8 numbers of 16 bits and 8 codes per lane");
     constexpr int E = Part<T>::E, kCols = Part<T>::kCols;
     const int lane = threadIdx.x & 31;
     const int64_t total = m * f;
     for (int64_t s = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); s < spans; s += static_cast<int64_t>(gridDim.x) * (kThreads / 32)) {
         const int64_t row = s / per_row, first = (s - row * per_row) * width, at0 = row * f + first;
         const int n = static_cast<int>(min(static_cast<int64_t>(width), f - first));
-        Stream<4> in(reinterpret_cast<const uint8_t*>(dh + at0), static_cast<int64_t>(n) * sizeof(T), reinterpret_cast<const uint8_t*>(dh),
-                     reinterpret_cast<const uint8_t*>(dh + total), lane);
-        Stream<2> ing(gq + at0, n, gq, gq + total, lane), inu(uq + at0, n, uq, uq + total, lane);
         const int64_t blk = row * nblk + first / kActBlock;
+        const uint8_t *const dh0 = reinterpret_cast<const uint8_t*>(dh), *const d0 = dh0 + 2 * at0, *const g0 = gq + at0, *const u0 = uq + at0;
         T *const to_g = dg + row * ldg + first, *const to_u = du + row * ldg + first;
-#pragma unroll 1
+        // the next part's words and scales, on the way while one is worked on
+        uint32_t ad[5], ag[3], au[3];
+        float asg, asu;
+        auto fetch = [&](int col) {
+            const int at = col + lane * E;
+            const bool inside = part_inside<4>(d0 + 2 * col, dh0, dh0 + 2 * total) && part_inside<2>(g0 + col, gq, gq + total) && part_inside<2>(u0 + col, uq, uq + total);
+            load_words<4>(d0 + 2 * at, dh0, dh0 + 2 * total, inside, ad);
+            load_words<2>(g0 + at, gq, gq + total, inside, ag);
+            load_words<2>(u0 + at, uq, uq + total, inside, au);
+            asg = at < n ? __ldg(gs + blk + at / kActBlock) : 0.0f;
+            asu = at < n ? __ldg(us + blk + at / kActBlock) : 0.0f;
+        };
+        fetch(0);
+#pragma unroll 2
         for (int col = 0; col < n; col += kCols) {
             uint32_t d[4], cg[2], cu[2];
             const int at = col + lane * E;
             const bool here = at < n;
-            const float sg = here ? __ldg(gs + blk + at / kActBlock) : 0.0f, su = here ? __ldg(us + blk + at / kActBlock) : 0.0f;
-            in.next(lane, d);
-            ing.next(lane, cg);
-            inu.next(lane, cu);
+            const float sg = asg, su = asu;
+            into_place<4>(ad, d0, d);
+            into_place<2>(ag, g0, cg);
+            into_place<2>(au, u0, cu);
+            if (col + kCols < n) fetch(col + kCols);
             if (here) {
                 uint4 a, b;
                 gated_bwd8<T, ACT>(d, cg, cu, sg, su, a, b);
@@ -516,15 +490,13 @@ __global__ void __launch_bounds__(kThreads) k_gated_bwd_any(const T* __restrict_
     }
 }
 
-// How k_save_any and k_gated_bwd_any share out their rows: long spans have fewer ragged ends, many spans keep all SMs busy, so the
-// longest spans that still leave every SM 32 warps, and at least two parts each.
+// How k_save_any and k_gated_bwd_any share out their rows: spans of up to 4 parts, fewer where that leaves an SM less than 32
+// warps' worth; neighbouring warps have neighbouring spans.  A whole row per warp has fewer ragged ends, but thousands of places
+// of memory in use at once and a last round that is mostly idle (6525 x 27060: 404 us where this takes 277).
 struct Spans { int64_t count; uint32_t per_row; int width; };
 Spans spans_of(int64_t rows, int64_t cols, int part) {
-    const int64_t parts = (cols + part - 1) / part, enough = static_cast<int64_t>(num_sms()) * 32;
-    int64_t per_row = (enough + rows - 1) / rows;
-    if (per_row > (parts + 1) / 2) per_row = (parts + 1) / 2;
-    const int64_t each = (parts + per_row - 1) / per_row;
-    per_row = (parts + each - 1) / each;
+    const int64_t parts = (cols + part - 1) / part, room = rows * parts / (static_cast<int64_t>(num_sms()) * 32);
+    const int64_t most = room < 1 ? 1 : room > 4 ? 4 : room, per_row = (parts + most - 1) / most, each = (parts + per_row - 1) / per_row;
     return {rows * per_row, static_cast<uint32_t>(per_row), static_cast<int>(each * part)};
 }
 
