@@ -9,13 +9,5 @@ def run(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, act: str = "silu", 
     or bf16; act: silu, gelu, gelu_tanh or relu.  With `checkpoint`: (h, gq, gs, uq, us), where gq, gs and uq, us
     are the 8-bit forms (act_checkpoint_fp8's) of the two projections, which ffn_gated_bwd reads."""
     ext = native.load()
-    code = native.activation(act)
-    m, f = x.shape[0], wg.shape[0]
-    h = torch.empty((m, f), dtype=x.dtype, device=x.device)
-    if not checkpoint:
-        ext.ffn_gated(x, wg, wu, h, code, None, None, None, None)
-        return h
-    gq, uq = (torch.empty((m, f), dtype=torch.float8_e4m3fn, device=x.device) for _ in range(2))
-    gs, us = (torch.empty((m, -(-f // 128)), dtype=torch.float32, device=x.device) for _ in range(2))
-    ext.ffn_gated(x, wg, wu, h, code, gq, gs, uq, us)
-    return h, gq, gs, uq, us
+    run = ext.ffn_gated_checkpoint_new if checkpoint else ext.ffn_gated_new
+    return run(x, wg, wu, native.activation(act))

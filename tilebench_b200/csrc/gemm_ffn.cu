@@ -843,14 +843,15 @@ int ffn_mid(const void* x, const void* wg, const void* wu, void* h, int64_t m, i
     }
 }
 
-// Hidden units per tile of the pair kernel: 128, or the multiple of 8 that leaves the least idle at the end.  A wave
-// costs its tiles' width and some 8 more; below 64 a stage is bound by issuing it.
+// Hidden units per tile of the pair kernel: 128, or the multiple of 8 that leaves the least idle at the end.  A wave's time
+// hardly falls with its tiles' width, since a stage takes 0.27 us to issue whatever its width (measured at k = 2048: 12.1 us
+// a wave of 128-wide tiles, 9.8 of 64-wide ones): it goes as the width + 200.
 int pair_width(int64_t m, int64_t f) {
     const int64_t pairs = num_sms() / 2, tm = (m + 2 * kHalf - 1) / (2 * kHalf);
     int best = kHalf;
     int64_t least = 0;
     for (int w = kHalf; w >= 64; w -= 8) {
-        const int64_t cost = (tm * ((f + w - 1) / w) + pairs - 1) / pairs * (w + 8);
+        const int64_t cost = (tm * ((f + w - 1) / w) + pairs - 1) / pairs * (w + 200);
         if (least == 0 || cost < least) {
             least = cost;
             best = w;

@@ -3,7 +3,9 @@
 // the matching extern "C" entry point of libtb200.so.  A nonzero return code becomes a Python
 // exception carrying tb200_last_error(), which the benchmark engine records as `cuda_err`.
 // Nothing here synchronises or allocates, so every call may run under CUDA-graph capture;
-// outputs and workspaces are allocated by the Python caller with torch.empty.
+// outputs and workspaces are allocated by the Python caller with torch.empty.  The layer operators, which have up to
+// five outputs and run on small inputs too, also have forms (*_new) that make the outputs here, from the same allocator:
+// a torch.empty from Python costs 2.4 us of host time, more than the smallest kernels take.
 #include <torch/extension.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -331,6 +333,57 @@ void ffn_gated_bwd(const torch::Tensor& dh, const torch::Tensor& wg, const torch
              "tb200_ffn_gated_bwd");
 }
 
+// The forms that make their outputs: x may be anything, the functions above check it.
+torch::Tensor empty_on(const torch::Tensor& like, at::IntArrayRef sizes, c10::ScalarType dt) {
+    return at::empty(sizes, at::TensorOptions().dtype(dt).device(like.device()));
+}
+int64_t blocks_of(int64_t cols) { return (cols + 127) / 128; }
+
+std::tuple<torch::Tensor, torch::Tensor> act_checkpoint_fp8_new(const torch::Tensor& x) {
+    check_rows(x, "x");
+    torch::Tensor q = empty_on(x, x.sizes(), torch::kFloat8_e4m3fn), s = empty_on(x, {x.size(0), blocks_of(x.size(1))}, torch::kFloat32);
+    act_checkpoint_fp8(x, q, s);
+    return {q, s};
+}
+
+torch::Tensor act_restore_fp8_new(const torch::Tensor& q, const torch::Tensor& scales, c10::ScalarType dtype) {
+    torch::Tensor out = empty_on(q, q.sizes(), dtype);
+    act_restore_fp8(q, scales, out);
+    return out;
+}
+
+torch::Tensor ffn_gated_new(const torch::Tensor& x, const torch::Tensor& wg, const torch::Tensor& wu, int64_t act) {
+    check_rows(x, "x");
+    TORCH_CHECK(wg.dim() == 2, "wg must be [f, k]");
+    torch::Tensor h = empty_on(x, {x.size(0), wg.size(0)}, x.scalar_type());
+    ffn_gated(x, wg, wu, h, act, c10::nullopt, c10::nullopt, c10::nullopt, c10::nullopt);
+    return h;
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> ffn_gated_checkpoint_new(
+    const torch::Tensor& x, const torch::Tensor& wg, const torch::Tensor& wu, int64_t act) {
+    check_rows(x, "x");
+    TORCH_CHECK(wg.dim() == 2, "wg must be [f, k]");
+    const int64_t m = x.size(0), f = wg.size(0);
+    torch::Tensor h = empty_on(x, {m, f}, x.scalar_type());
+    torch::Tensor gq = empty_on(x, {m, f}, torch::kFloat8_e4m3fn), gs = empty_on(x, {m, blocks_of(f)}, torch::kFloat32);
+    torch::Tensor uq = empty_on(x, {m, f}, torch::kFloat8_e4m3fn), us = empty_on(x, {m, blocks_of(f)}, torch::kFloat32);
+    ffn_gated(x, wg, wu, h, act, gq, gs, uq, us);
+    return {h, gq, gs, uq, us};
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> ffn_gated_bwd_new(
+    const torch::Tensor& dh, const torch::Tensor& wg, const torch::Tensor& wu, const torch::Tensor& x, const c10::optional<torch::Tensor>& xs,
+    const torch::Tensor& gq, const torch::Tensor& gs, const torch::Tensor& uq, const torch::Tensor& us, int64_t act) {
+    TORCH_CHECK(dh.is_cuda() && dh.dim() == 2 && wg.dim() == 2, "dh [m,f], wg [f,k] must be CUDA matrices");
+    const int64_t m = dh.size(0), f = wg.size(0), k = wg.size(1);
+    c10::cuda::CUDAGuard guard(dh.device());                    // the workspace depends on the device's SMs
+    torch::Tensor dx = empty_on(dh, {m, k}, wg.scalar_type()), dwg = empty_on(dh, {f, k}, wg.scalar_type()), dwu = empty_on(dh, {f, k}, wg.scalar_type());
+    torch::Tensor ws = empty_on(dh, {ffn_gated_bwd_workspace_bytes(m, f, k, xs.has_value())}, torch::kUInt8);
+    ffn_gated_bwd(dh, wg, wu, x, xs, gq, gs, uq, us, dx, dwg, dwu, act, ws);
+    return {dx, dwg, dwu};
+}
+
 py::tuple device_status() {
     int code = 0, detail = 0;
     check_rc(tb200_device_status(&code, &detail), "tb200_device_status");
@@ -364,6 +417,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("ffn_gated", &ffn_gated);
     m.def("ffn_gated_bwd_workspace_bytes", &ffn_gated_bwd_workspace_bytes);
     m.def("ffn_gated_bwd", &ffn_gated_bwd);
+    m.def("act_checkpoint_fp8_new", &act_checkpoint_fp8_new);
+    m.def("act_restore_fp8_new", &act_restore_fp8_new);
+    m.def("ffn_gated_new", &ffn_gated_new);
+    m.def("ffn_gated_checkpoint_new", &ffn_gated_checkpoint_new);
+    m.def("ffn_gated_bwd_new", &ffn_gated_bwd_new);
     m.def("device_status", &device_status);
     m.def("clear_device_status", &clear_device_status);
 }
