@@ -90,6 +90,7 @@ __device__ __forceinline__ void decode(const uint32_t (&codes)[E / 4], float s, 
 template <typename T, int U, bool FLAT>
 __global__ void __launch_bounds__(kThreads) k_save(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales,
                                                    uint32_t blocks, uint32_t nblk, int64_t cols, int64_t ldx) {
+    let_next_begin();
     constexpr int E = 32 / sizeof(T), kLanes = kActBlock / E;
     const uint64_t total = static_cast<uint64_t>(blocks) * kLanes, step = static_cast<uint64_t>(gridDim.x) * kThreads;
     for (uint64_t i0 = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x; i0 - (threadIdx.x & 31) < total; i0 += U * step) {
@@ -137,6 +138,7 @@ __global__ void __launch_bounds__(kThreads) k_save(const T* __restrict__ x, uint
 template <typename T, int U, bool FLAT>
 __global__ void __launch_bounds__(kThreads) k_restore(const uint8_t* __restrict__ q, const float* __restrict__ scales, T* __restrict__ out,
                                                       uint32_t blocks, uint32_t nblk, int64_t cols) {
+    let_next_begin();
     constexpr int E = 32 / sizeof(T), kLanes = kActBlock / E;
     const uint64_t total = static_cast<uint64_t>(blocks) * kLanes, step = static_cast<uint64_t>(gridDim.x) * kThreads;
     for (uint64_t i0 = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x; i0 < total; i0 += U * step) {
@@ -267,6 +269,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) k_save_any(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales,
                                                        int64_t spans, uint32_t per_row, int width, uint32_t nblk, int64_t rows, int64_t cols,
                                                        int64_t ldx) {
+    let_next_begin();
     constexpr int E = Part<T>::E, N = E / 4, kLanes = Part<T>::kLanes, kCols = Part<T>::kCols;
     const int lane = threadIdx.x & 31;
     const uint8_t *begin = reinterpret_cast<const uint8_t*>(x), *end = reinterpret_cast<const uint8_t*>(x + (rows - 1) * ldx + cols);
@@ -315,6 +318,7 @@ __global__ void __launch_bounds__(kThreads) k_save_any(const T* __restrict__ x, 
 template <typename T, int U>
 __global__ void __launch_bounds__(kThreads) k_restore_across(const uint8_t* __restrict__ q, const float* __restrict__ scales, T* __restrict__ out,
                                                              int64_t total, uint32_t nblk, int64_t cols) {
+    let_next_begin();
     constexpr int E = 32 / sizeof(T);
     // a warp takes U * 32 neighbouring pieces at a time: their first place is divided once, the lanes' by 32-bit steps
     constexpr int kWarpCols = U * 32 * E;
@@ -378,6 +382,7 @@ __global__ void __launch_bounds__(kThreads) k_restore_across(const uint8_t* __re
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_restore_any(const uint8_t* __restrict__ q, const float* __restrict__ scales, T* __restrict__ out,
                                                           int64_t total, uint32_t nblk, int64_t cols) {
+    let_next_begin();
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * kThreads) {
         const int64_t row = i / cols;
         out[i] = ActType<T>::store(act_held(act_values2(q[i]).x * scales[row * nblk + (i - row * cols) / kActBlock], ActType<T>::kTop));
@@ -410,6 +415,7 @@ template <typename T, int ACT, int U>
 __global__ void __launch_bounds__(kThreads) k_gated_bwd(const uint4* __restrict__ dh, const uint2* __restrict__ gq, const float* __restrict__ gs,
                                                         const uint2* __restrict__ uq, const float* __restrict__ us, uint4* __restrict__ dg,
                                                         uint4* __restrict__ du, uint32_t total, uint32_t per_row, uint32_t nblk) {
+    let_next_begin();
     const uint32_t step = gridDim.x * kThreads;
     for (uint64_t i0 = blockIdx.x * kThreads + threadIdx.x; i0 < total; i0 += U * step) {
         uint4 d[U];
@@ -447,6 +453,7 @@ __global__ void __launch_bounds__(kThreads) k_gated_bwd_any(const T* __restrict_
                                                             const uint8_t* __restrict__ uq, const float* __restrict__ us, T* __restrict__ dg,
                                                             T* __restrict__ du, int64_t spans, uint32_t per_row, int width, int64_t m, int64_t f,
                                                             int64_t ldg, uint32_t nblk) {
+    let_next_begin();
     static_assert(sizeof(T) == 2, "8 numbers of 16 bits and 8 codes per lane");
     constexpr int E = Part<T>::E, kCols = Part<T>::kCols;
     const int lane = threadIdx.x & 31;

@@ -156,6 +156,35 @@ __device__ __forceinline__ float2 gate_both(float g) {
 }
 #endif  // __CUDACC__
 
+// ---- launches that overlap their set-up with the end of the kernel before ----------------------------------------
+// Every kernel of the block lets the next one of its stream begin once all its CTAs have (let_next_begin), and the matrix
+// products are launched so that they may: their launch, barriers, tensor memory and tensor maps overlap with the end of
+// the kernel before, and they wait for it to be complete (wait_for_previous) before they touch global memory.  Only the
+// products are launched that way: what they read comes by TMA, from L2, whereas a load through L1 could meet a line that the
+// kernel before had left there.
+#ifdef __CUDACC__
+__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <typename Args, typename Maps>
+int launch_over_previous(void (*kern)(Maps, Args), int grid, int block, int smem, int cluster, cudaStream_t st, const Maps& maps, const Args& args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+    cfg.blockDim = dim3(static_cast<unsigned>(block), 1, 1);
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    TB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, maps, args));
+    return TB200_OK;
+}
+#endif
+
 // ---- launchers shared between the files of the feed-forward block ----------------------------------------------
 // The products of the backward pass's two intermediates: dg = dh * u * f'(g), du = dh * f(g), row pitch ldg.
 int launch_gated_act_bwd(const void* dh, const void* gq, const float* gs, const void* uq, const float* us, void* dg, void* du,

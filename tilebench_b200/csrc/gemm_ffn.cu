@@ -222,6 +222,7 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
     const int tiles = tiles_m * tiles_n;
     const int items = KIND == FK_DX ? tiles * p.splits : tiles; // dx: item i is share i / tiles of tile i % tiles
 
+    let_next_begin();
     if (SAVE && threadIdx.x < kAmaxBytes / 4) amax[threadIdx.x] = 0;
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
@@ -247,6 +248,7 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
     cluster_sync_all();                                          // the peer's barriers exist before anything signals them
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    wait_for_previous();
 
     if (warp == 0) {
         // ---------------- TMA producer (both CTAs) ----------------
@@ -500,6 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ffn_mid(const __grid_constant__
     const int t0 = static_cast<int>(blockIdx.x) / SHARES;
     const int t_step = SPLIT ? tiles : static_cast<int>(gridDim.x);                 // with SPLIT a CTA has one tile
 
+    let_next_begin();
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
             mbar_init(&bar_full[s], 1);
@@ -522,6 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ffn_mid(const __grid_constant__
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    wait_for_previous();
 
     if (warp == 0) {
         // ---------------- TMA producer ----------------
@@ -706,9 +710,7 @@ int launch_pair(const FfnMaps& maps, const FfnArgs& args, cudaStream_t st) {
     const int64_t tiles = (KIND == FK_DW ? 2 : KIND == FK_DX ? args.splits : 1) * ((args.rows + 2 * kHalf - 1) / (2 * kHalf)) * ((args.cols + tile_cols - 1) / tile_cols);
     if (tiles > 0x7fffffffll / kGroupM) return fail(TB200_ERR_UNSUPPORTED, "ffn_gated: too many tiles");
     const int pairs = static_cast<int>(tiles < max_pairs ? tiles : max_pairs);
-    kern<<<2 * pairs, kThreads, kSmemBytes, st>>>(maps, args);
-    TB200_CUDA_TRY(cudaGetLastError());
-    return TB200_OK;
+    return launch_over_previous(kern, 2 * pairs, kThreads, kSmemBytes, 1, st, maps, args);
 }
 
 template <typename T, bool SAVE>
@@ -790,19 +792,7 @@ int launch_mid(const MidMaps& maps, const MidArgs& args, cudaStream_t st) {
     const int rc = ensure_max_smem(attr_set, reinterpret_cast<const void*>(kern), kMidSmemBytes);
     if (rc != TB200_OK) return rc;
     const int tiles = (args.f + args.w - 1) / args.w;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(SHARES > 1 ? tiles * SHARES : tiles < num_sms() ? tiles : num_sms()), 1, 1);
-    cfg.blockDim = dim3(kThreads, 1, 1);
-    cfg.dynamicSmemBytes = kMidSmemBytes;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = SHARES;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = SHARES > 1 ? 1 : 0;
-    TB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, maps, args));
-    return TB200_OK;
+    return launch_over_previous(kern, SHARES > 1 ? tiles * SHARES : tiles < num_sms() ? tiles : num_sms(), kThreads, kMidSmemBytes, SHARES, st, maps, args);
 }
 
 template <typename T, int ACT>
@@ -906,6 +896,7 @@ int dx_splits(int64_t m, int64_t f, int64_t k) {
 // out = the sum of `splits` arrays of n numbers, in order; 8 numbers per thread.
 template <typename T>
 __global__ void __launch_bounds__(256) k_sum_shares(const float4* __restrict__ sums, uint4* __restrict__ out, int64_t n8, int splits) {
+    let_next_begin();
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n8; i += static_cast<int64_t>(gridDim.x) * 256) {
         float4 a = sums[2 * i], b = sums[2 * i + 1];
 #pragma unroll 4
