@@ -76,6 +76,12 @@ __device__ __forceinline__ void mma_if(uint32_t issue, uint32_t d_tmem, uint64_t
                  "r"(idesc), "r"(accumulate), "r"(issue) : "memory");
 }
 
+// Brings a box towards the SMs, as far as L2.  Nothing is read in the program's sense, so a weight that the kernel before is
+// still writing may be asked for: L2 holds what is written last.
+__device__ __forceinline__ void prefetch_2d(const CUtensorMap* m, int x, int y) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y) : "memory");
+}
+
 // ---- epilogue helpers --------------------------------------------------------------------------------------------
 // The four warps of a quarter collect 32 rows of 256 bytes in shared memory, 16-byte piece c of row r at place
 // c ^ (r & 15) (free of bank conflicts both ways); then each writes 8 of the rows out, neighbouring lanes on neighbouring bytes.
@@ -468,7 +474,9 @@ struct MidArgs {
     int m, f, depth;
     int w, stages, x_rows;                       // hidden units per tile, stages in shared memory, rows of x per copy
 };
-constexpr int kMidRing = 192 * 1024;
+constexpr int kFewRows = 64, kFewCols = 128;     // rows of x, and columns of an accumulator, in the form for few rows
+constexpr int kFewSums = kFewRows * 2 * kHalf * 4;
+constexpr int kMidRing = 192 * 1024;             // in the form for few rows the sums take 32 KB of it beside the staging area
 constexpr int kMidSmemBytes = kMidRing + 4 * kStagingBytes + kBarBytes + 1024;
 
 __device__ __forceinline__ float4 peer_float4(uint32_t addr, uint32_t rank) {
@@ -479,11 +487,49 @@ __device__ __forceinline__ float4 peer_float4(uint32_t addr, uint32_t rank) {
     return v;
 }
 
+// Four neighbouring hidden units c.. of row r from sums that lie row by row, `pitch` apart, g first and u `w` on: in this CTA
+// (SHARES = 1), or in each CTA of the cluster.
 template <typename T, int ACT, int SHARES>
+__device__ __forceinline__ void combine4(uint32_t base, int pitch, int w, int r, int c, int col, T* __restrict__ out, int f, bool vec) {
+    const uint32_t at = base + 4 * (r * pitch + c);
+    float4 gs[SHARES], us[SHARES];
+#pragma unroll
+    for (int o = 0; o < SHARES; ++o) {
+        if constexpr (SHARES > 1) {
+            gs[o] = peer_float4(at, o);
+            us[o] = peer_float4(at + 4 * w, o);
+        } else {
+            const uint4 a = shared_uint4(at), b = shared_uint4(at + 4 * w);
+            gs[o] = make_float4(__uint_as_float(a.x), __uint_as_float(a.y), __uint_as_float(a.z), __uint_as_float(a.w));
+            us[o] = make_float4(__uint_as_float(b.x), __uint_as_float(b.y), __uint_as_float(b.z), __uint_as_float(b.w));
+        }
+    }
+    float4 g = gs[0], u = us[0];
+#pragma unroll
+    for (int o = 1; o < SHARES; ++o) {
+        g.x += gs[o].x; g.y += gs[o].y; g.z += gs[o].z; g.w += gs[o].w;
+        u.x += us[o].x; u.y += us[o].y; u.z += us[o].z; u.w += us[o].w;
+    }
+    const float v[4] = {gate_value<ACT>(g.x) * u.x, gate_value<ACT>(g.y) * u.y, gate_value<ACT>(g.z) * u.z, gate_value<ACT>(g.w) * u.w};
+    T* h = out + static_cast<int64_t>(r) * f + col;
+    if (vec && col < f) {
+        *reinterpret_cast<uint2*>(h) = make_uint2(ActType<T>::pack(v[0], v[1]), ActType<T>::pack(v[2], v[3]));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (col + e < f) h[e] = ActType<T>::store(v[e]);
+    }
+}
+
+// FEW: at most 64 rows.  The weights are the operand of 128 rows then (2 w rows, one or two blocks) and x that of 16 to 64
+// columns, so that the tensor cores multiply by little that is not there: at 1 row of 4096 -> 14336, 128 rows of x cost 43.6 us a
+// pass at the board's power limit, this form 39.6.
+template <typename T, int ACT, int SHARES, bool FEW>
 __global__ void __launch_bounds__(kThreads, 1) k_ffn_mid(const __grid_constant__ MidMaps maps, const __grid_constant__ MidArgs p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* staging = smem + kMidRing;
+    uint8_t* few_sums = staging + 4 * kStagingBytes - kFewSums;
     uint64_t* bar_full = reinterpret_cast<uint64_t*>(staging + 4 * kStagingBytes);
     uint64_t* bar_empty = bar_full + kMaxStages;
     uint64_t* bar_afull = bar_empty + kMaxStages;
@@ -501,6 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ffn_mid(const __grid_constant__
     const int tiles = (p.f + w - 1) / w;
     const int t0 = static_cast<int>(blockIdx.x) / SHARES;
     const int t_step = SPLIT ? tiles : static_cast<int>(gridDim.x);                 // with SPLIT a CTA has one tile
+    const bool vec = p.f % 4 == 0 && (reinterpret_cast<uintptr_t>(p.h) & 7) == 0;   // four of a row's results can be stored at once
 
     let_next_begin();
     if (threadIdx.x == 0) {
@@ -525,6 +572,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_ffn_mid(const __grid_constant__
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    if (warp == 0 && lane == 0 && t0 < tiles) {
+        // the weights of the first stages, while the kernel before ends
+        for (int kb = kb0; kb < min(kb1, kb0 + S); ++kb) {
+            prefetch_2d(&maps.wg, kb * kBK, t0 * w);
+            prefetch_2d(&maps.wu, kb * kBK, t0 * w);
+        }
+    }
     wait_for_previous();
 
     if (warp == 0) {
@@ -554,9 +608,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_ffn_mid(const __grid_constant__
         // Rows of x beyond x_rows are whatever follows in shared memory: they reach only rows of the accumulator that
         // nothing reads.
         constexpr uint32_t fmt = ActType<T>::kTop > 1e6f ? 1u : 0u;
-        const uint32_t idesc = umma_idesc(fmt, fmt, kHalf, 2 * w);
+        const uint32_t idesc = FEW ? umma_idesc(fmt, fmt, kHalf, p.x_rows) : umma_idesc(fmt, fmt, kHalf, 2 * w);
         const bool leader = lane == 0;
-        const uint64_t a_desc0 = umma_desc_sw128(smem_u32(smem)), b_desc0 = umma_desc_sw128(smem_u32(smem) + x_bytes);
+        const uint64_t x_desc0 = umma_desc_sw128(smem_u32(smem)), w_desc0 = umma_desc_sw128(smem_u32(smem) + x_bytes);
+        const uint64_t a_desc0 = FEW ? w_desc0 : x_desc0, b_desc0 = FEW ? x_desc0 : w_desc0;
+        const bool two = FEW && 2 * w > kHalf;
         const uint32_t stage_desc = static_cast<uint32_t>(stage_bytes) >> 4;
         uint32_t s = 0, ph = 0, cnt = 0;
         bool ready = false;
@@ -565,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_ffn_mid(const __grid_constant__
             const uint32_t acc = cnt & 1;
             if (!mbar_wait(&bar_aempty[acc], ((cnt >> 1) & 1) ^ 1, ST_WAIT_TMEM_EMPTY, t)) { ok = false; break; }
             tc_fence_after();
-            const uint32_t d_tmem = tmem_base + acc * 256;
+            const uint32_t d_tmem = tmem_base + acc * (FEW ? kFewCols : 256);
             for (int kb = kb0; kb < kb1; ++kb) {
                 if (!ready && !mbar_wait(&bar_full[s], ph, ST_WAIT_SMEM_FULL, kb)) { ok = false; break; }
                 tc_fence_after();
@@ -576,12 +632,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_ffn_mid(const __grid_constant__
                 ready = mbar_test_wait(&bar_full[s], ph);
 #pragma unroll
                 for (int k = 1; k < 4; ++k) mma_if(leader, d_tmem, a_desc + 2 * k, b_desc + 2 * k, idesc, 1u);
+                if (two) {                                       // rows 128.. of the weights, 16 KB on
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        mma_if(leader, d_tmem + kFewRows, a_desc + (kHalf * 128 >> 4) + 2 * k, b_desc + 2 * k, idesc, kb > kb0 || k > 0 ? 1u : 0u);
+                }
                 tc_commit_if(leader, freed);
             }
             if (ok && leader) tc_commit(&bar_afull[acc]);
         }
     } else if (warp >= 4) {
-        // ---------------- epilogue: a warp has 32 rows of a quarter of the columns ----------------
+        // ---------------- epilogue: a warp has 32 rows (lanes) of a quarter of the columns ----------------
         const int quarter = (warp - 4) & 3, part = (warp - 4) >> 2, row0 = quarter * 32;
         uint8_t* buf = staging + quarter * kStagingBytes;
         const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -592,8 +653,34 @@ __global__ void __launch_bounds__(kThreads, 1) k_ffn_mid(const __grid_constant__
             // a wait that gave up ends the waiting, not the walk: the warps meet at barriers below
             ok = ok && mbar_wait(&bar_afull[acc], (cnt >> 1) & 1, ST_WAIT_TMEM_FULL, t);
             tc_fence_after();
-            const uint32_t t_acc = t_lane + acc * 256;
-            if constexpr (SPLIT) {
+            const uint32_t t_acc = t_lane + acc * (FEW ? kFewCols : 256);
+            if constexpr (FEW) {
+                // A lane has one row of the weights and 16 of the tokens at a time; the sums go token by token to where they are
+                // combined: the ring (SPLIT, as below) or a place of their own.
+                const int block = part >> 1, unit = kHalf * block + 32 * quarter + lane;
+                const int pitch = SPLIT ? 2 * w + 4 : 2 * w;
+                float* sums = reinterpret_cast<float*>(SPLIT ? smem : few_sums);
+                for (int first = (part & 1) * 16; kHalf * block + 32 * quarter < 2 * w && first < p.m; first += 32) {
+                    uint32_t v[16];
+                    tmem_ld16(t_acc + block * kFewRows + first, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (unit < 2 * w && first + i < p.m) sums[(first + i) * pitch + unit] = __uint_as_float(v[i]);
+                }
+                if constexpr (!SPLIT) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bar_aempty[acc]);
+                    asm volatile("bar.sync 5, %0;" ::"n"(32 * kEpiWarps) : "memory");
+                    const int quads = w / 4;
+                    for (int i = threadIdx.x - 128; i < p.m * quads; i += 32 * kEpiWarps) {
+                        const int r = i / quads, c = 4 * (i - r * quads);
+                        combine4<T, ACT, 1>(smem_u32(sums), pitch, w, r, c, t * w + c, static_cast<T*>(p.h), p.f, vec);
+                    }
+                    asm volatile("bar.sync 5, %0;" ::"n"(32 * kEpiWarps) : "memory");
+                }
+            } else if constexpr (SPLIT) {
                 // this CTA's sums, row by row.  A row pitch of 4 more than a multiple of 16 keeps eight lanes' (rows')
                 // 16-byte pieces on different banks.  Every copy into the ring has landed and been used by the time the
                 // accumulator is complete.
@@ -639,31 +726,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_ffn_mid(const __grid_constant__
         cluster_sync_all();                                      // every share of the sums is in place
         const int quads = w / 4, q0 = quads * share / SHARES, qn = quads * (share + 1) / SHARES - q0;
         const uint32_t base = smem_u32(smem);
-        const bool vec = p.f % 4 == 0 && (reinterpret_cast<uintptr_t>(p.h) & 7) == 0;
         for (int i = threadIdx.x; i < p.m * qn; i += kThreads) {
-            const int r = i / qn, c = 4 * (q0 + i - r * qn), col = t0 * w + c;
-            const uint32_t at = base + 4 * (r * (2 * w + 4) + c);
-            float4 gs[SHARES], us[SHARES];
-#pragma unroll
-            for (int o = 0; o < SHARES; ++o) {
-                gs[o] = peer_float4(at, o);
-                us[o] = peer_float4(at + 4 * w, o);
-            }
-            float4 g = gs[0], u = us[0];
-#pragma unroll
-            for (int o = 1; o < SHARES; ++o) {
-                g.x += gs[o].x; g.y += gs[o].y; g.z += gs[o].z; g.w += gs[o].w;
-                u.x += us[o].x; u.y += us[o].y; u.z += us[o].z; u.w += us[o].w;
-            }
-            const float v[4] = {gate_value<ACT>(g.x) * u.x, gate_value<ACT>(g.y) * u.y, gate_value<ACT>(g.z) * u.z, gate_value<ACT>(g.w) * u.w};
-            T* h = static_cast<T*>(p.h) + static_cast<int64_t>(r) * p.f + col;
-            if (vec && col < p.f) {
-                *reinterpret_cast<uint2*>(h) = make_uint2(ActType<T>::pack(v[0], v[1]), ActType<T>::pack(v[2], v[3]));
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (col + e < p.f) h[e] = ActType<T>::store(v[e]);
-            }
+            const int r = i / qn, c = 4 * (q0 + i - r * qn);
+            combine4<T, ACT, SHARES>(base, 2 * w + 4, w, r, c, t0 * w + c, static_cast<T*>(p.h), p.f, vec);
         }
         cluster_sync_all();                                      // no CTA leaves while a peer reads its memory
     }
@@ -734,7 +799,7 @@ int clusters_of(int* n) {                        // clusters of SHARES CTAs that
     if (rc != TB200_OK) return rc;
     *n = tab.v[dev].load(std::memory_order_acquire);
     if (*n == 0) {
-        auto kern = k_ffn_mid<__nv_bfloat16, TB200_ACT_SILU, SHARES>;
+        auto kern = k_ffn_mid<__nv_bfloat16, TB200_ACT_SILU, SHARES, false>;
         TB200_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMidSmemBytes));
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(static_cast<unsigned>(num_sms() / SHARES * SHARES), 1, 1);
@@ -754,7 +819,8 @@ int clusters_of(int* n) {                        // clusters of SHARES CTAs that
 }
 
 // The width and the shares with the least time by a model fitted to measurements (1 to 128 rows, k 512..8192,
-// f 512..28672; it picks within 8 % of the best measured plan).  A stage takes 0.25 us to issue whatever its size, or what it takes to
+// f 512..28672; it picks within 8 % of the best measured plan).  A stage takes 0.25 us to issue whatever its size (0.37 in two
+// blocks of weights), or what it takes to
 // bring its bytes from L2 to the SM (95 GB/s each) or all CTAs' weights from HBM (6.4 TB/s); a wave takes its stages;
 // sharing costs 0.8 us and the peers' sums at 20 GB/s.
 int mid_plan(int64_t m, int64_t f, int64_t k, MidPlan* plan) {
@@ -773,7 +839,7 @@ int mid_plan(int64_t m, int64_t f, int64_t k, MidPlan* plan) {
             if (shares > 1 && tiles > clusters[i]) continue;     // shared tiles run in one wave
             const int64_t waves = (tiles + clusters[i] - 1) / clusters[i], at_once = (tiles < clusters[i] ? tiles : clusters[i]) * shares;
             const float link = static_cast<float>(x_rows + 2 * w) * (128.0f / 95e3f), hbm = static_cast<float>(at_once) * (2 * w) * (128.0f / 6.4e6f);
-            const float stage = fmaxf(0.25f, fmaxf(link, hbm));
+            const float stage = fmaxf(m <= kFewRows && 2 * w > kHalf ? 0.37f : 0.25f, fmaxf(link, hbm));
             const float t = static_cast<float>(waves) * static_cast<float>((KB + shares - 1) / shares) * stage +
                             (shares > 1 ? 0.8f + static_cast<float>(m) * (8 * w) / 20e3f : 0.012f * w);
             if (best == 0.0f || t < best) {
@@ -785,9 +851,9 @@ int mid_plan(int64_t m, int64_t f, int64_t k, MidPlan* plan) {
     return TB200_OK;
 }
 
-template <typename T, int ACT, int SHARES>
+template <typename T, int ACT, int SHARES, bool FEW>
 int launch_mid(const MidMaps& maps, const MidArgs& args, cudaStream_t st) {
-    auto kern = k_ffn_mid<T, ACT, SHARES>;
+    auto kern = k_ffn_mid<T, ACT, SHARES, FEW>;
     static PerDeviceInt attr_set;
     const int rc = ensure_max_smem(attr_set, reinterpret_cast<const void*>(kern), kMidSmemBytes);
     if (rc != TB200_OK) return rc;
@@ -795,13 +861,22 @@ int launch_mid(const MidMaps& maps, const MidArgs& args, cudaStream_t st) {
     return launch_over_previous(kern, SHARES > 1 ? tiles * SHARES : tiles < num_sms() ? tiles : num_sms(), kThreads, kMidSmemBytes, SHARES, st, maps, args);
 }
 
-template <typename T, int ACT>
+template <typename T, int ACT, bool FEW>
 int launch_mid_shares(const MidMaps& maps, const MidArgs& args, int shares, cudaStream_t st) {
     switch (shares) {
-        case 1: return launch_mid<T, ACT, 1>(maps, args, st);
-        case 2: return launch_mid<T, ACT, 2>(maps, args, st);
-        case 4: return launch_mid<T, ACT, 4>(maps, args, st);
-        default: return launch_mid<T, ACT, 8>(maps, args, st);
+        case 1: return launch_mid<T, ACT, 1, FEW>(maps, args, st);
+        case 2: return launch_mid<T, ACT, 2, FEW>(maps, args, st);
+        case 4: return launch_mid<T, ACT, 4, FEW>(maps, args, st);
+        default: return launch_mid<T, ACT, 8, FEW>(maps, args, st);
+    }
+}
+template <typename T, bool FEW>
+int launch_mid_act(const MidMaps& maps, const MidArgs& args, int shares, int act, cudaStream_t st) {
+    switch (act) {
+        case TB200_ACT_SILU: return launch_mid_shares<T, TB200_ACT_SILU, FEW>(maps, args, shares, st);
+        case TB200_ACT_GELU: return launch_mid_shares<T, TB200_ACT_GELU, FEW>(maps, args, shares, st);
+        case TB200_ACT_GELU_TANH: return launch_mid_shares<T, TB200_ACT_GELU_TANH, FEW>(maps, args, shares, st);
+        default: return launch_mid_shares<T, TB200_ACT_RELU, FEW>(maps, args, shares, st);
     }
 }
 
@@ -816,21 +891,18 @@ int ffn_mid(const void* x, const void* wg, const void* wu, void* h, int64_t m, i
     args.f = static_cast<int>(f);
     args.depth = static_cast<int>(k);
     args.w = plan.w;
-    args.x_rows = static_cast<int>((m + 7) / 8 * 8);
+    const bool few = m <= kFewRows;
+    args.x_rows = static_cast<int>(few ? (m + 15) / 16 * 16 : (m + 7) / 8 * 8);
     const int stage = (args.x_rows + 2 * plan.w) * 128;
-    args.stages = kMidRing / stage < kMaxStages ? kMidRing / stage : kMaxStages;
+    const int ring = few ? kMidRing + 4 * kStagingBytes - kFewSums : kMidRing;
+    args.stages = ring / stage < kMaxStages ? ring / stage : kMaxStages;
     MidMaps maps;
     memset(&maps, 0, sizeof(maps));
     rc = map_k<T>(&maps.x, x, m, k, ldx, args.x_rows);
     if (rc == TB200_OK) rc = map_k<T>(&maps.wg, wg, f, k, k, plan.w);
     if (rc == TB200_OK) rc = map_k<T>(&maps.wu, wu, f, k, k, plan.w);
     if (rc != TB200_OK) return rc;
-    switch (act) {
-        case TB200_ACT_SILU: return launch_mid_shares<T, TB200_ACT_SILU>(maps, args, plan.shares, st);
-        case TB200_ACT_GELU: return launch_mid_shares<T, TB200_ACT_GELU>(maps, args, plan.shares, st);
-        case TB200_ACT_GELU_TANH: return launch_mid_shares<T, TB200_ACT_GELU_TANH>(maps, args, plan.shares, st);
-        default: return launch_mid_shares<T, TB200_ACT_RELU>(maps, args, plan.shares, st);
-    }
+    return few ? launch_mid_act<T, true>(maps, args, plan.shares, act, st) : launch_mid_act<T, false>(maps, args, plan.shares, act, st);
 }
 
 // Hidden units per tile of the pair kernel: 128, or the multiple of 8 that leaves the least idle at the end.  A wave's time
