@@ -25,7 +25,9 @@ namespace {
 
 constexpr int kBK = 64;                          // contraction per stage: 128 bytes of 16-bit elements
 constexpr int kHalf = 128;                       // rows of A, and columns of B, that one CTA loads
-constexpr int kStages = 6;
+// Stages in shared memory: dw, whose tiles have the fewest stages, gives one up for a second staging area.  (128 rows at
+// 4096 x 14336: dw 58 -> 45 us; dx would go from 55 to 60.)
+constexpr int stages_of(int kind) { return kind == 2 ? 5 : 6; }
 constexpr int kOperandBytes = kHalf * 128;
 constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kAtomBytes = kBK * 128;            // MN-major: one box of 64 contraction rows x 64 columns
@@ -33,7 +35,7 @@ constexpr int kEpiWarps = 16;                    // four per quarter of the tens
 constexpr int kStagingBytes = 32 * 256;          // per quarter: 32 rows of 256 bytes
 constexpr int kAmaxBytes = 4 * 32 * 8;           // per quarter: 32 rows' amax of g and of u
 constexpr int kBarBytes = 256;
-constexpr int kSmemBytes = kStages * kStageBytes + 4 * kStagingBytes + kAmaxBytes + kBarBytes + 1024;
+constexpr int kSmemBytes = 6 * kStageBytes + 4 * kStagingBytes + kAmaxBytes + kBarBytes + 1024;
 constexpr int kTmemCols = 512;
 constexpr int kThreads = 128 + 32 * kEpiWarps;   // TMA, MMA, two idle warps, epilogue
 constexpr int kGroupM = 8;                       // tiles are walked in bands of 8 x 256 rows, so that B's tiles stay in L2
@@ -43,14 +45,14 @@ enum FfnKind : int { FK_FWD = 0, FK_DX = 1, FK_DW = 2 };
 struct FfnMaps {
     CUtensorMap a[2];                            // forward: x, -      dx: dg, du     dw: dg, du
     CUtensorMap b[2];                            // forward: Wg, Wu    dx: Wg, Wu     dw: x, -
+    CUtensorMap out[2];                          // forward: -         dx: dx, -      dw: dWg, dWu
 };
 struct FfnArgs {
-    void* out[2];                                // forward: h, -      dx: dx, -      dw: dWg, dWu
+    void* out;                                   // forward: h
     float* sums;                                 // dx in shares: [splits, rows, cols] partial sums
     int rows, cols, depth;                       // of one result, and of one product's contraction
     int splits;                                  // dx: shares of the contraction
     int w;                                       // forward: hidden units per tile (128 with checkpoints)
-    int64_t ldo;                                 // row pitch of the result, in elements
     uint8_t* codes[2];                           // forward with checkpoints: codes of g and u, [rows, cols]
     float* scales[2];                            // and their scales, [rows, ceil(cols / 128)]
 };
@@ -201,15 +203,16 @@ __device__ __forceinline__ Tile tile_at(int t, int tiles_m, int tiles_n) {
 template <int KIND, typename T, int ACT, bool SAVE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs p) {
-    constexpr int S = kStages;
+    constexpr int S = stages_of(KIND), kAreas = KIND == FK_DW ? 2 : 1;
+    static_assert(S * kStageBytes + kAreas * 4 * kStagingBytes <= 6 * kStageBytes + 4 * kStagingBytes, "shared memory");
     constexpr bool kAMn = KIND == FK_DW, kBMn = KIND != FK_FWD;
     const int tile_cols = KIND == FK_FWD ? p.w : 2 * kHalf;     // columns of the result that a tile covers
     const int b_bytes = KIND == FK_FWD ? p.w * 128 : kOperandBytes;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* staging = smem + S * kStageBytes;
-    uint32_t* amax = reinterpret_cast<uint32_t*>(staging + 4 * kStagingBytes);      // [quarter][g, u][row], bits of non-negative numbers
-    uint64_t* bar_full = reinterpret_cast<uint64_t*>(staging + 4 * kStagingBytes + kAmaxBytes);
+    uint32_t* amax = reinterpret_cast<uint32_t*>(staging + kAreas * 4 * kStagingBytes);      // [quarter][g, u][row], bits of non-negative numbers
+    uint64_t* bar_full = reinterpret_cast<uint64_t*>(staging + kAreas * 4 * kStagingBytes + kAmaxBytes);
     uint64_t* bar_empty = bar_full + S;
     uint64_t* bar_afull = bar_empty + S;          // [2] accumulator complete
     uint64_t* bar_aempty = bar_afull + 2;         // [2] accumulator read (the epilogue warps of both CTAs)
@@ -244,6 +247,8 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
         tma_prefetch_desc(&maps.b[0]);
         if (KIND != FK_FWD) tma_prefetch_desc(&maps.a[1]);
         if (KIND != FK_DW) tma_prefetch_desc(&maps.b[1]);
+        if (KIND != FK_FWD) tma_prefetch_desc(&maps.out[0]);
+        if (KIND == FK_DW) tma_prefetch_desc(&maps.out[1]);
     }
     if (warp == 1) {
         tmem_alloc_pair(tmem_slot, kTmemCols);
@@ -383,7 +388,7 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
                     ag = __uint_as_float(row_amax[0]);
                     au = __uint_as_float(row_amax[32]);
                 }
-                flush<T, 16>(buf, 0, static_cast<T*>(p.out[0]) + static_cast<int64_t>(row0) * p.ldo + col0, p.ldo, r8, rows, min(cols, tile_cols), lane);
+                flush<T, 16>(buf, 0, static_cast<T*>(p.out) + static_cast<int64_t>(row0) * p.cols + col0, p.cols, r8, rows, min(cols, tile_cols), lane);
                 quarter_sync(quarter);
                 if constexpr (SAVE) {
                     tmem_ld32(t_g, g);
@@ -433,21 +438,41 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
                     quarter_sync(quarter);
                 }
             } else {
-                T* dst = static_cast<T*>(p.out[sel]) + static_cast<int64_t>(row0) * p.ldo + col0;
+                // By TMA, which leaves out what lies beyond the result: 32 rows x 64 columns a copy, in the 128-byte swizzle.  One half of
+                // the columns per staging area; the quarter's first lane, which issues the copies, waits for the area's last ones.
                 uint32_t v[2][32];
                 tmem_ld32(t_acc + part * 32, v[0]);
                 tmem_ld32(t_acc + kHalf + part * 32, v[1]);
                 tmem_wait_ld();
                 release();
+                const bool issuer = part == 0 && lane == 0;
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    stage32<T>(buf, lane, 4 * part, v[c]);
+                    uint8_t* area = staging + (c % kAreas * 4 + quarter) * kStagingBytes;
+                    if (issuer) tma_store_wait_read<kAreas - 1>();        // all but the other area's
                     quarter_sync(quarter);
-                    flush<T, 16>(buf, 0, dst + c * kHalf, p.ldo, r8, rows, cols - c * kHalf, lane);
+                    uint8_t* box = area + (part >> 1) * (32 * 128) + lane * 128;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = ActType<T>::pack(__uint_as_float(v[c][8 * q + 2 * e]), __uint_as_float(v[c][8 * q + 2 * e + 1]));
+                        *reinterpret_cast<uint4*>(box + ((((part & 1) * 4 + q) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                    fence_async_smem();
                     quarter_sync(quarter);
+                    if (issuer) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int x = col0 + c * kHalf + h * 64;
+                            if (rows > 0 && x < p.cols) tma_store_2d(&maps.out[sel], area + h * (32 * 128), x, row0);
+                        }
+                        tma_store_commit();
+                    }
                 }
             }
         }
+        if (KIND != FK_FWD && part == 0 && lane == 0) tma_store_wait<0>();
     }
 
     // neither CTA may leave while the other can still read its shared memory or signal its barriers
@@ -751,6 +776,12 @@ int map_mn(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t
     return encode_tmap_2d(m, base, tmap_type<T>(), 2, rows, cols, pitch * 2, kBK, 64, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// A result that is stored by TMA: 32 rows x 64 columns.
+template <typename T>
+int map_out(CUtensorMap* m, const void* base, int64_t rows, int64_t cols) {
+    return encode_tmap_2d(m, base, tmap_type<T>(), 2, rows, cols, cols * 2, 32, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 template <int KIND, typename T, int ACT, bool SAVE>
 int launch_pair(const FfnMaps& maps, const FfnArgs& args, cudaStream_t st) {
     auto kern = k_ffn_pair<KIND, T, ACT, SAVE>;
@@ -821,8 +852,8 @@ int clusters_of(int* n) {                        // clusters of SHARES CTAs that
 // The width and the shares with the least time by a model fitted to measurements (1 to 128 rows, k 512..8192,
 // f 512..28672; it picks within 8 % of the best measured plan).  A stage takes 0.25 us to issue whatever its size (0.37 in two
 // blocks of weights), or what it takes to
-// bring its bytes from L2 to the SM (95 GB/s each) or all CTAs' weights from HBM (6.4 TB/s); a wave takes its stages;
-// sharing costs 0.8 us and the peers' sums at 20 GB/s.
+// bring its bytes from L2 to the SM (95 GB/s each) or all CTAs' weights from HBM (6.4 TB/s); a wave takes its stages
+// and 0.6 us; sharing costs 0.8 us and the peers' sums at 20 GB/s.
 int mid_plan(int64_t m, int64_t f, int64_t k, MidPlan* plan) {
     int clusters[4] = {num_sms(), 0, 0, 0};
     int rc = clusters_of<2>(&clusters[1]);
@@ -841,7 +872,7 @@ int mid_plan(int64_t m, int64_t f, int64_t k, MidPlan* plan) {
             const float link = static_cast<float>(x_rows + 2 * w) * (128.0f / 95e3f), hbm = static_cast<float>(at_once) * (2 * w) * (128.0f / 6.4e6f);
             const float stage = fmaxf(m <= kFewRows && 2 * w > kHalf ? 0.37f : 0.25f, fmaxf(link, hbm));
             const float t = static_cast<float>(waves) * static_cast<float>((KB + shares - 1) / shares) * stage +
-                            (shares > 1 ? 0.8f + static_cast<float>(m) * (8 * w) / 20e3f : 0.012f * w);
+                            (shares > 1 ? 0.8f + static_cast<float>(m) * (8 * w) / 20e3f : 0.6f * static_cast<float>(waves) + 0.012f * w);
             if (best == 0.0f || t < best) {
                 best = t;
                 *plan = {w, shares};
@@ -934,11 +965,10 @@ int ffn_forward(const void* x, const void* wg, const void* wu, void* h, void* gq
     if (rc != TB200_OK) return rc;
     FfnArgs args = {};
     args.w = w;
-    args.out[0] = h;
+    args.out = h;
     args.rows = static_cast<int>(m);
     args.cols = static_cast<int>(f);
     args.depth = static_cast<int>(k);
-    args.ldo = f;
     args.codes[0] = static_cast<uint8_t*>(gq);
     args.codes[1] = static_cast<uint8_t*>(uq);
     args.scales[0] = gs;
@@ -992,12 +1022,12 @@ int ffn_products_bwd(const void* dg, const void* du, int64_t ldg, const void* x,
     if (rc == TB200_OK) rc = map_mn<T>(&maps.b[0], wg, f, k, k);
     if (rc == TB200_OK) rc = map_mn<T>(&maps.b[1], wu, f, k, k);
     if (rc != TB200_OK) return rc;
+    if (rc == TB200_OK) rc = map_out<T>(&maps.out[0], dx, m, k);
+    if (rc != TB200_OK) return rc;
     FfnArgs args = {};
-    args.out[0] = dx;
     args.rows = static_cast<int>(m);
     args.cols = static_cast<int>(k);
     args.depth = static_cast<int>(f);
-    args.ldo = k;
     args.splits = dx_splits(m, f, k);
     args.sums = sums;
     rc = launch_pair<FK_DX, T, 0, false>(maps, args, st);
@@ -1013,9 +1043,9 @@ int ffn_products_bwd(const void* dg, const void* du, int64_t ldg, const void* x,
     rc = map_mn<T>(&maps.a[0], dg, m, f, ldg);
     if (rc == TB200_OK) rc = map_mn<T>(&maps.a[1], du, m, f, ldg);
     if (rc == TB200_OK) rc = map_mn<T>(&maps.b[0], x, m, k, ldx);
+    if (rc == TB200_OK) rc = map_out<T>(&maps.out[0], dwg, f, k);
+    if (rc == TB200_OK) rc = map_out<T>(&maps.out[1], dwu, f, k);
     if (rc != TB200_OK) return rc;
-    args.out[0] = dwg;
-    args.out[1] = dwu;
     args.rows = static_cast<int>(f);
     args.depth = static_cast<int>(m);
     return launch_pair<FK_DW, T, 0, false>(maps, args, st);
