@@ -48,7 +48,7 @@ struct FfnMaps {
     CUtensorMap out[2];                          // forward: -         dx: dx, -      dw: dWg, dWu
 };
 struct FfnArgs {
-    void* out;                                   // forward: h
+    void* out[2];                                // forward: h, -      dx: dx, -      dw: dWg, dWu
     float* sums;                                 // dx in shares: [splits, rows, cols] partial sums
     int rows, cols, depth;                       // of one result, and of one product's contraction
     int splits;                                  // dx: shares of the contraction
@@ -388,7 +388,7 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
                     ag = __uint_as_float(row_amax[0]);
                     au = __uint_as_float(row_amax[32]);
                 }
-                flush<T, 16>(buf, 0, static_cast<T*>(p.out) + static_cast<int64_t>(row0) * p.cols + col0, p.cols, r8, rows, min(cols, tile_cols), lane);
+                flush<T, 16>(buf, 0, static_cast<T*>(p.out[0]) + static_cast<int64_t>(row0) * p.cols + col0, p.cols, r8, rows, min(cols, tile_cols), lane);
                 quarter_sync(quarter);
                 if constexpr (SAVE) {
                     tmem_ld32(t_g, g);
@@ -440,14 +440,23 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
             } else {
                 // By TMA, which leaves out what lies beyond the result: 32 rows x 64 columns a copy, in the 128-byte swizzle.  One half of
                 // the columns per staging area; the quarter's first lane, which issues the copies, waits for the area's last ones.
+                // Rows that do not begin on 32-byte boundaries are written by the warps, 256 bytes of a row at once: copies of 128
+                // would leave twice as many sectors half written (6 rows of 7192 -> 28637: 221 us where this takes 182).
                 uint32_t v[2][32];
                 tmem_ld32(t_acc + part * 32, v[0]);
                 tmem_ld32(t_acc + kHalf + part * 32, v[1]);
                 tmem_wait_ld();
                 release();
-                const bool issuer = part == 0 && lane == 0;
+                const bool issuer = part == 0 && lane == 0, by_tma = p.cols % 16 == 0;
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
+                    if (!by_tma) {
+                        stage32<T>(buf, lane, 4 * part, v[c]);
+                        quarter_sync(quarter);
+                        flush<T, 16>(buf, 0, static_cast<T*>(p.out[sel]) + static_cast<int64_t>(row0) * p.cols + col0 + c * kHalf, p.cols, r8, rows, cols - c * kHalf, lane);
+                        quarter_sync(quarter);
+                        continue;
+                    }
                     uint8_t* area = staging + (c % kAreas * 4 + quarter) * kStagingBytes;
                     if (issuer) tma_store_wait_read<kAreas - 1>();        // all but the other area's
                     quarter_sync(quarter);
@@ -763,6 +772,169 @@ __global__ void __launch_bounds__(kThreads, 1) k_ffn_mid(const __grid_constant__
     }
 }
 
+// ------------------------------------------------------------------------------------------------
+// dx for few rows (m <= 64): bound by reading the weights, as the forward block of a decoding batch is.  The weights, read as
+// stored, are the operand of 128 rows (128 columns of dx), dg and du the one of 16 to 64; one CTA has 128 columns of dx and
+// a share of the contraction over both products.  Sums go to [shares, m, k] in 32 bits, neighbouring lanes on neighbouring
+// columns.  (4 rows of 4096 x 14336: 48 us, the pair kernel's 256-row tiles 60; at 100 of 2048 x 5632 it was 22 against 19.)
+struct DxFewMaps { CUtensorMap d[2], w[2]; };    // dg, du; Wg, Wu
+struct DxFewArgs {
+    void* dx;                                    // with one share
+    float* sums;                                 // with more
+    int m, k, depth, shares;
+    int rows, stages;                            // of dg per copy: m rounded up to 16; in shared memory
+};
+constexpr int kDxCols = kFewRows;                     // columns of an accumulator
+constexpr int kDxRing = 192 * 1024;
+constexpr int kDxThreads = 256;
+constexpr int kDxSmemBytes = kDxRing + kBarBytes + 1024;
+
+template <typename T>
+__global__ void __launch_bounds__(kDxThreads, 1) k_dx_few(const __grid_constant__ DxFewMaps maps, const __grid_constant__ DxFewArgs p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bar_full = reinterpret_cast<uint64_t*>(smem + kDxRing);
+    uint64_t* bar_empty = bar_full + kMaxStages;
+    uint64_t* bar_afull = bar_empty + kMaxStages;
+    uint64_t* bar_aempty = bar_afull + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_aempty + 2);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const int S = p.stages, d_bytes = p.rows * 128, stage_bytes = kOperandBytes + d_bytes;
+    const int KB = (p.depth + kBK - 1) / kBK, steps = 2 * KB;
+    const int tiles = (p.k + kHalf - 1) / kHalf, items = tiles * p.shares;
+
+    let_next_begin();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(&bar_full[s], 1);
+            mbar_init(&bar_empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&bar_afull[b], 1);
+            mbar_init(&bar_aempty[b], 4);
+        }
+        mbar_fence_init();
+        for (int i = 0; i < 2; ++i) {
+            tma_prefetch_desc(&maps.d[i]);
+            tma_prefetch_desc(&maps.w[i]);
+        }
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, 2 * kDxCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    if (warp == 0 && lane == 0 && static_cast<int>(blockIdx.x) < items) {
+        // the weights of the first stages, while the kernel before ends
+        const int share = blockIdx.x / tiles, col = (blockIdx.x - share * tiles) * kHalf, st0 = share_at(steps, share, p.shares);
+        for (int st = st0; st < min(st0 + S, share_at(steps, share + 1, p.shares)); ++st) {
+            const int prod = st >= KB ? 1 : 0;
+            prefetch_2d(&maps.w[prod], col, (st - prod * KB) * kBK);
+            prefetch_2d(&maps.w[prod], col + 64, (st - prod * KB) * kBK);
+        }
+    }
+    wait_for_previous();
+
+    if (warp == 0) {
+        // ---------------- TMA producer ----------------
+        if (lane == 0) {
+            uint32_t s = 0, ph = 1;
+            bool ok = true;
+            for (int t = blockIdx.x; t < items && ok; t += gridDim.x) {
+                const int share = t / tiles, col = (t - share * tiles) * kHalf;
+                for (int st = share_at(steps, share, p.shares); st < share_at(steps, share + 1, p.shares); ++st) {
+                    if (!mbar_wait(&bar_empty[s], ph, ST_WAIT_SMEM_EMPTY, st)) { ok = false; break; }
+                    uint8_t* stage = smem + s * stage_bytes;
+                    mbar_expect_tx(&bar_full[s], stage_bytes);
+                    const int prod = st >= KB ? 1 : 0, f0 = (st - prod * KB) * kBK;
+                    tma_load_2d(stage, &maps.w[prod], &bar_full[s], col, f0);
+                    tma_load_2d(stage + kAtomBytes, &maps.w[prod], &bar_full[s], col + 64, f0);
+                    tma_load_2d(stage + kOperandBytes, &maps.d[prod], &bar_full[s], f0, 0);
+                    if (++s == static_cast<uint32_t>(S)) { s = 0; ph ^= 1; }
+                }
+            }
+            if (!ok) {
+                // copies in flight land within microseconds; a bounded pause before the CTA may exit
+                const long long c0 = clock64();
+                while (clock64() - c0 < (1ll << 21)) {}
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer ----------------
+        constexpr uint32_t fmt = ActType<T>::kTop > 1e6f ? 1u : 0u;
+        const uint32_t idesc = umma_idesc(fmt, fmt, kHalf, p.rows) | 1u << 15;                   // A is MN-major
+        const bool leader = lane == 0;
+        const uint64_t a_desc0 = desc_mn(smem_u32(smem)), b_desc0 = umma_desc_sw128(smem_u32(smem) + kOperandBytes);
+        const uint32_t stage_desc = static_cast<uint32_t>(stage_bytes) >> 4;
+        uint32_t s = 0, ph = 0, cnt = 0;
+        bool ready = false;
+        bool ok = true;
+        for (int t = blockIdx.x; t < items && ok; t += gridDim.x, ++cnt) {
+            const uint32_t acc = cnt & 1;
+            if (!mbar_wait(&bar_aempty[acc], ((cnt >> 1) & 1) ^ 1, ST_WAIT_TMEM_EMPTY, t)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t d_tmem = tmem_base + acc * kDxCols;
+            const int share = t / tiles, n = share_at(steps, share + 1, p.shares) - share_at(steps, share, p.shares);
+            for (int st = 0; st < n; ++st) {
+                if (!ready && !mbar_wait(&bar_full[s], ph, ST_WAIT_SMEM_FULL, st)) { ok = false; break; }
+                tc_fence_after();
+                const uint64_t a_desc = a_desc0 + s * stage_desc, b_desc = b_desc0 + s * stage_desc;
+                uint64_t* const freed = &bar_empty[s];
+                if (++s == static_cast<uint32_t>(S)) { s = 0; ph ^= 1; }
+                mma_if(leader, d_tmem, a_desc, b_desc, idesc, st > 0 ? 1u : 0u);
+                ready = mbar_test_wait(&bar_full[s], ph);
+#pragma unroll
+                for (int k = 1; k < 4; ++k) mma_if(leader, d_tmem, a_desc + k * (16 * 128 / 16), b_desc + 2 * k, idesc, 1u);
+                tc_commit_if(leader, freed);
+            }
+            if (ok && leader) tc_commit(&bar_afull[acc]);
+        }
+    } else if (warp >= 4) {
+        // ---------------- epilogue: a lane has one column of dx, a register one row ----------------
+        const int quarter = warp - 4;
+        const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+        uint32_t cnt = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; t < items && ok; t += gridDim.x, ++cnt) {
+            const uint32_t acc = cnt & 1;
+            const int share = t / tiles, col = (t - share * tiles) * kHalf + quarter * 32 + lane;
+            if (!mbar_wait(&bar_afull[acc], (cnt >> 1) & 1, ST_WAIT_TMEM_FULL, t)) { ok = false; break; }
+            tc_fence_after();
+#pragma unroll 1
+            for (int r0 = 0; r0 < p.m; r0 += 16) {
+                uint32_t v[16];
+                tmem_ld16(t_lane + acc * kDxCols + r0, v);
+                tmem_wait_ld();
+                if (col < p.k) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        if (r0 + i < p.m) {
+                            if (p.shares > 1) p.sums[(static_cast<int64_t>(share) * p.m + r0 + i) * p.k + col] = __uint_as_float(v[i]);
+                            else static_cast<T*>(p.dx)[static_cast<int64_t>(r0 + i) * p.k + col] = ActType<T>::store(__uint_as_float(v[i]));
+                        }
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar_aempty[acc]);
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) {
+        __syncwarp();
+        tmem_dealloc(tmem_base, 2 * kDxCols);
+    }
+}
+
 template <typename T>
 constexpr CUtensorMapDataType tmap_type() { return ActType<T>::kTop > 1e6f ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16; }
 
@@ -965,7 +1137,7 @@ int ffn_forward(const void* x, const void* wg, const void* wu, void* h, void* gq
     if (rc != TB200_OK) return rc;
     FfnArgs args = {};
     args.w = w;
-    args.out = h;
+    args.out[0] = h;
     args.rows = static_cast<int>(m);
     args.cols = static_cast<int>(f);
     args.depth = static_cast<int>(k);
@@ -976,16 +1148,20 @@ int ffn_forward(const void* x, const void* wg, const void* wu, void* h, void* gq
     return gq ? launch_fwd<T, true>(maps, args, act, st) : launch_fwd<T, false>(maps, args, act, st);
 }
 
-// Shares of dx's contraction, where its tiles are too few for the pairs of SMs: the number with the fewest stages in a
-// row.  A tile costs some 6 stages beside its own; shares are written and added up in 32 bits, at 5 TB/s, by a kernel
-// that costs some 10 more (a stage is 0.27 us).
+// Shares of dx's contraction: the number with the least time by a model in stages of 0.27 us.  A tile costs some 6 beside its
+// own; shares are written and added up in 32 bits, at 5 TB/s, by a kernel that costs some 10 more.  For few rows a
+// stage takes longer where it waits for the weights: 0.38 us at 148 CTAs.
 int dx_splits(int64_t m, int64_t f, int64_t k) {
-    const int64_t pairs = num_sms() / 2, tiles = ((m + 2 * kHalf - 1) / (2 * kHalf)) * ((k + 2 * kHalf - 1) / (2 * kHalf));
+    const bool few = m <= kFewRows;
+    const int64_t places = few ? num_sms() : num_sms() / 2;
+    const int64_t tiles = few ? (k + kHalf - 1) / kHalf : ((m + 2 * kHalf - 1) / (2 * kHalf)) * ((k + 2 * kHalf - 1) / (2 * kHalf));
     const int64_t steps = 2 * ((f + kBK - 1) / kBK);
     int best = 1;
     double least = 0.0;
-    for (int s = 1; s <= 8 && steps >= 16 * (s - 1); ++s) {
-        const double cost = static_cast<double>((tiles * s + pairs - 1) / pairs) * ((steps + s - 1) / s + 6) +
+    for (int s = 1; s <= 16 && steps >= 8 * (s - 1); ++s) {
+        const int64_t at_once = tiles * s < places ? tiles * s : places;
+        const double stage = few ? fmax(1.0, 1.4 * static_cast<double>(at_once) / static_cast<double>(places)) : 1.0;
+        const double cost = static_cast<double>((tiles * s + places - 1) / places) * (static_cast<double>((steps + s - 1) / s) * stage + 6.0) +
                             (s > 1 ? 10.0 + static_cast<double>(m) * k * 8.0 * s / (5e6 * 0.27) : 0.0);
         if (s == 1 || cost < least) {
             least = cost;
@@ -1011,34 +1187,71 @@ __global__ void __launch_bounds__(256) k_sum_shares(const float4* __restrict__ s
     }
 }
 
-// dg, du: [m, ldg]; x: [m, k]; sums: room for dx_splits() arrays of [m, k] where that is more than 1
 template <typename T>
-int ffn_products_bwd(const void* dg, const void* du, int64_t ldg, const void* x, int64_t ldx, const void* wg, const void* wu, void* dx, void* dwg,
-                     void* dwu, float* sums, int64_t m, int64_t f, int64_t k, cudaStream_t st) {
+int dx_pair(const void* dg, const void* du, int64_t ldg, const void* wg, const void* wu, void* dx, float* sums, int splits, int64_t m, int64_t f,
+            int64_t k, cudaStream_t st) {
     FfnMaps maps;
     memset(&maps, 0, sizeof(maps));
     int rc = map_k<T>(&maps.a[0], dg, m, f, ldg);
     if (rc == TB200_OK) rc = map_k<T>(&maps.a[1], du, m, f, ldg);
     if (rc == TB200_OK) rc = map_mn<T>(&maps.b[0], wg, f, k, k);
     if (rc == TB200_OK) rc = map_mn<T>(&maps.b[1], wu, f, k, k);
-    if (rc != TB200_OK) return rc;
     if (rc == TB200_OK) rc = map_out<T>(&maps.out[0], dx, m, k);
     if (rc != TB200_OK) return rc;
     FfnArgs args = {};
     args.rows = static_cast<int>(m);
     args.cols = static_cast<int>(k);
     args.depth = static_cast<int>(f);
-    args.splits = dx_splits(m, f, k);
+    args.splits = splits;
     args.sums = sums;
-    rc = launch_pair<FK_DX, T, 0, false>(maps, args, st);
+    args.out[0] = dx;
+    return launch_pair<FK_DX, T, 0, false>(maps, args, st);
+}
+
+template <typename T>
+int dx_few(const void* dg, const void* du, int64_t ldg, const void* wg, const void* wu, void* dx, float* sums, int splits, int64_t m, int64_t f,
+           int64_t k, cudaStream_t st) {
+    auto kern = k_dx_few<T>;
+    static PerDeviceInt attr_set;
+    int rc = ensure_max_smem(attr_set, reinterpret_cast<const void*>(kern), kDxSmemBytes);
     if (rc != TB200_OK) return rc;
-    if (args.splits > 1) {
+    DxFewArgs args = {};
+    args.dx = dx;
+    args.sums = sums;
+    args.m = static_cast<int>(m);
+    args.k = static_cast<int>(k);
+    args.depth = static_cast<int>(f);
+    args.shares = splits;
+    args.rows = static_cast<int>((m + 15) / 16 * 16);
+    const int stage = kOperandBytes + args.rows * 128;
+    args.stages = kDxRing / stage < kMaxStages ? kDxRing / stage : kMaxStages;
+    DxFewMaps maps;
+    memset(&maps, 0, sizeof(maps));
+    rc = map_k<T>(&maps.d[0], dg, m, f, ldg, args.rows);
+    if (rc == TB200_OK) rc = map_k<T>(&maps.d[1], du, m, f, ldg, args.rows);
+    if (rc == TB200_OK) rc = map_mn<T>(&maps.w[0], wg, f, k, k);
+    if (rc == TB200_OK) rc = map_mn<T>(&maps.w[1], wu, f, k, k);
+    if (rc != TB200_OK) return rc;
+    const int64_t items = (k + kHalf - 1) / kHalf * splits;
+    return launch_over_previous(kern, static_cast<int>(items < num_sms() ? items : num_sms()), kDxThreads, kDxSmemBytes, 1, st, maps, args);
+}
+
+// dg, du: [m, ldg]; x: [m, k]; sums: room for dx_splits() arrays of [m, k] where that is more than 1
+template <typename T>
+int ffn_products_bwd(const void* dg, const void* du, int64_t ldg, const void* x, int64_t ldx, const void* wg, const void* wu, void* dx, void* dwg,
+                     void* dwu, float* sums, int64_t m, int64_t f, int64_t k, cudaStream_t st) {
+    const int splits = dx_splits(m, f, k);
+    int rc = m <= kFewRows ? dx_few<T>(dg, du, ldg, wg, wu, dx, sums, splits, m, f, k, st) : dx_pair<T>(dg, du, ldg, wg, wu, dx, sums, splits, m, f, k, st);
+    if (rc != TB200_OK) return rc;
+    if (splits > 1) {
         const int64_t n8 = m * (k / 8), ctas = (n8 + 255) / 256, cap = static_cast<int64_t>(num_sms()) * 8;
-        k_sum_shares<T><<<static_cast<unsigned>(ctas < cap ? ctas : cap), 256, 0, st>>>(reinterpret_cast<const float4*>(sums), static_cast<uint4*>(dx),
-                                                                                      n8, args.splits);
+        k_sum_shares<T><<<static_cast<unsigned>(ctas < cap ? ctas : cap), 256, 0, st>>>(reinterpret_cast<const float4*>(sums), static_cast<uint4*>(dx), n8,
+                                                                                      splits);
         TB200_CUDA_TRY(cudaGetLastError());
     }
 
+    FfnMaps maps;
+    FfnArgs args = {};
     memset(&maps, 0, sizeof(maps));
     rc = map_mn<T>(&maps.a[0], dg, m, f, ldg);
     if (rc == TB200_OK) rc = map_mn<T>(&maps.a[1], du, m, f, ldg);
@@ -1047,7 +1260,10 @@ int ffn_products_bwd(const void* dg, const void* du, int64_t ldg, const void* x,
     if (rc == TB200_OK) rc = map_out<T>(&maps.out[1], dwu, f, k);
     if (rc != TB200_OK) return rc;
     args.rows = static_cast<int>(f);
+    args.cols = static_cast<int>(k);
     args.depth = static_cast<int>(m);
+    args.out[0] = dwg;
+    args.out[1] = dwu;
     return launch_pair<FK_DW, T, 0, false>(maps, args, st);
 }
 
