@@ -507,6 +507,8 @@ struct MidArgs {
     void* h;
     int m, f, depth;
     int w, stages, x_rows;                       // hidden units per tile, stages in shared memory, rows of x per copy
+    uint8_t* codes[2];                           // with checkpoints: codes of g and u, [m, f]
+    float* scales[2];                            // and their scales, [m, ceil(f / 128)]
 };
 constexpr int kFewRows = 64, kFewCols = 128;     // rows of x, and columns of an accumulator, in the form for few rows
 constexpr int kFewSums = kFewRows * 2 * kHalf * 4;
@@ -521,10 +523,10 @@ __device__ __forceinline__ float4 peer_float4(uint32_t addr, uint32_t rank) {
     return v;
 }
 
-// Four neighbouring hidden units c.. of row r from sums that lie row by row, `pitch` apart, g first and u `w` on: in this CTA
-// (SHARES = 1), or in each CTA of the cluster.
-template <typename T, int ACT, int SHARES>
-__device__ __forceinline__ void combine4(uint32_t base, int pitch, int w, int r, int c, int col, T* __restrict__ out, int f, bool vec) {
+// g and u of four neighbouring hidden units c.. of row r, from sums that lie row by row, `pitch` apart, g first and u `w` on: in
+// this CTA (SHARES = 1), or added up over the CTAs of the cluster.
+template <int SHARES>
+__device__ __forceinline__ void gather4(uint32_t base, int pitch, int w, int r, int c, float (&g)[4], float (&u)[4]) {
     const uint32_t at = base + 4 * (r * pitch + c);
     float4 gs[SHARES], us[SHARES];
 #pragma unroll
@@ -538,13 +540,18 @@ __device__ __forceinline__ void combine4(uint32_t base, int pitch, int w, int r,
             us[o] = make_float4(__uint_as_float(b.x), __uint_as_float(b.y), __uint_as_float(b.z), __uint_as_float(b.w));
         }
     }
-    float4 g = gs[0], u = us[0];
 #pragma unroll
     for (int o = 1; o < SHARES; ++o) {
-        g.x += gs[o].x; g.y += gs[o].y; g.z += gs[o].z; g.w += gs[o].w;
-        u.x += us[o].x; u.y += us[o].y; u.z += us[o].z; u.w += us[o].w;
+        gs[0].x += gs[o].x; gs[0].y += gs[o].y; gs[0].z += gs[o].z; gs[0].w += gs[o].w;
+        us[0].x += us[o].x; us[0].y += us[o].y; us[0].z += us[o].z; us[0].w += us[o].w;
     }
-    const float v[4] = {gate_value<ACT>(g.x) * u.x, gate_value<ACT>(g.y) * u.y, gate_value<ACT>(g.z) * u.z, gate_value<ACT>(g.w) * u.w};
+    g[0] = gs[0].x; g[1] = gs[0].y; g[2] = gs[0].z; g[3] = gs[0].w;
+    u[0] = us[0].x; u[1] = us[0].y; u[2] = us[0].z; u[3] = us[0].w;
+}
+// h of them, for row r and the result's columns col..; vec: four can be stored at once.
+template <typename T, int ACT>
+__device__ __forceinline__ void store4(const float (&g)[4], const float (&u)[4], T* __restrict__ out, int r, int col, int f, bool vec) {
+    const float v[4] = {gate_value<ACT>(g[0]) * u[0], gate_value<ACT>(g[1]) * u[1], gate_value<ACT>(g[2]) * u[2], gate_value<ACT>(g[3]) * u[3]};
     T* h = out + static_cast<int64_t>(r) * f + col;
     if (vec && col < f) {
         *reinterpret_cast<uint2*>(h) = make_uint2(ActType<T>::pack(v[0], v[1]), ActType<T>::pack(v[2], v[3]));
@@ -554,11 +561,34 @@ __device__ __forceinline__ void combine4(uint32_t base, int pitch, int w, int r,
             if (col + e < f) h[e] = ActType<T>::store(v[e]);
     }
 }
+// Scale and codes of a row's 1 x 128 block, four numbers per lane of a warp.
+__device__ __forceinline__ void save4(const float (&v)[4], uint8_t* __restrict__ codes, float* __restrict__ scale, int col, int f, bool vec, int lane) {
+    float amax = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const bool infinite = amax > FLT_MAX;                        // the same in all lanes
+    if (infinite) {
+        amax = fmaxf(fmaxf(act_size(v[0]), act_size(v[1])), fmaxf(act_size(v[2]), act_size(v[3])));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    }
+    const float2 s = act_scale(amax);
+    const uint32_t c = infinite ? act_codes4_checked(v[0], v[1], v[2], v[3], s.y) : act_codes4(v[0], v[1], v[2], v[3], s.y);
+    if (vec && col < f) {
+        *reinterpret_cast<uint32_t*>(codes + col) = c;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (col + e < f) codes[col + e] = static_cast<uint8_t>(c >> (8 * e));
+    }
+    if (lane == 0) *scale = s.x;
+}
 
 // FEW: at most 64 rows.  The weights are the operand of 128 rows then (2 w rows, one or two blocks) and x that of 16 to 64
 // columns, so that the tensor cores multiply by little that is not there: at 1 row of 4096 -> 14336, 128 rows of x cost 43.6 us a
 // pass at the board's power limit, this form 39.6.
-template <typename T, int ACT, int SHARES, bool FEW>
+// SAVE (with FEW, tiles of 128 hidden units): a warp takes a row of the tile, which is one block of g and of u.
+template <typename T, int ACT, int SHARES, bool FEW, bool SAVE>
 __global__ void __launch_bounds__(kThreads, 1) k_ffn_mid(const __grid_constant__ MidMaps maps, const __grid_constant__ MidArgs p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -581,7 +611,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_ffn_mid(const __grid_constant__
     const int tiles = (p.f + w - 1) / w;
     const int t0 = static_cast<int>(blockIdx.x) / SHARES;
     const int t_step = SPLIT ? tiles : static_cast<int>(gridDim.x);                 // with SPLIT a CTA has one tile
-    const bool vec = p.f % 4 == 0 && (reinterpret_cast<uintptr_t>(p.h) & 7) == 0;   // four of a row's results can be stored at once
+    const bool vec = p.f % 4 == 0 && (reinterpret_cast<uintptr_t>(p.h) & 7) == 0 &&  // four of a row's results can be stored at once
+                     ((reinterpret_cast<uintptr_t>(p.codes[0]) | reinterpret_cast<uintptr_t>(p.codes[1])) & 3) == 0;
+    auto save_row = [&](uint32_t base, int pitch, int r, int t) {
+        float g[4], u[4];
+        gather4<SHARES>(base, pitch, kHalf, r, 4 * lane, g, u);
+        const int col = t * kHalf + 4 * lane;
+        const int64_t row = static_cast<int64_t>(r) * p.f, blk = static_cast<int64_t>(r) * ((p.f + kHalf - 1) / kHalf) + t;
+        store4<T, ACT>(g, u, static_cast<T*>(p.h), r, col, p.f, vec);
+        save4(g, p.codes[0] + row, p.scales[0] + blk, col, p.f, vec, lane);
+        save4(u, p.codes[1] + row, p.scales[1] + blk, col, p.f, vec, lane);
+    };
 
     let_next_begin();
     if (threadIdx.x == 0) {
@@ -707,10 +747,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_ffn_mid(const __grid_constant__
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bar_aempty[acc]);
                     asm volatile("bar.sync 5, %0;" ::"n"(32 * kEpiWarps) : "memory");
-                    const int quads = w / 4;
-                    for (int i = threadIdx.x - 128; i < p.m * quads; i += 32 * kEpiWarps) {
-                        const int r = i / quads, c = 4 * (i - r * quads);
-                        combine4<T, ACT, 1>(smem_u32(sums), pitch, w, r, c, t * w + c, static_cast<T*>(p.h), p.f, vec);
+                    if constexpr (SAVE) {
+                        for (int r = warp - 4; r < p.m; r += kEpiWarps) save_row(smem_u32(sums), pitch, r, t);
+                    } else {
+                        const int quads = w / 4;
+                        for (int i = threadIdx.x - 128; i < p.m * quads; i += 32 * kEpiWarps) {
+                            const int r = i / quads, c = 4 * (i - r * quads);
+                            float g[4], u[4];
+                            gather4<1>(smem_u32(sums), pitch, w, r, c, g, u);
+                            store4<T, ACT>(g, u, static_cast<T*>(p.h), r, t * w + c, p.f, vec);
+                        }
                     }
                     asm volatile("bar.sync 5, %0;" ::"n"(32 * kEpiWarps) : "memory");
                 }
@@ -760,9 +806,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_ffn_mid(const __grid_constant__
         cluster_sync_all();                                      // every share of the sums is in place
         const int quads = w / 4, q0 = quads * share / SHARES, qn = quads * (share + 1) / SHARES - q0;
         const uint32_t base = smem_u32(smem);
-        for (int i = threadIdx.x; i < p.m * qn; i += kThreads) {
-            const int r = i / qn, c = 4 * (q0 + i - r * qn);
-            combine4<T, ACT, SHARES>(base, 2 * w + 4, w, r, c, t0 * w + c, static_cast<T*>(p.h), p.f, vec);
+        if constexpr (SAVE) {
+            for (int r = share + SHARES * warp; r < p.m; r += SHARES * (kThreads / 32)) save_row(base, 2 * w + 4, r, t0);
+        } else {
+            for (int i = threadIdx.x; i < p.m * qn; i += kThreads) {
+                const int r = i / qn, c = 4 * (q0 + i - r * qn);
+                float g[4], u[4];
+                gather4<SHARES>(base, 2 * w + 4, w, r, c, g, u);
+                store4<T, ACT>(g, u, static_cast<T*>(p.h), r, t0 * w + c, p.f, vec);
+            }
         }
         cluster_sync_all();                                      // no CTA leaves while a peer reads its memory
     }
@@ -1002,7 +1054,7 @@ int clusters_of(int* n) {                        // clusters of SHARES CTAs that
     if (rc != TB200_OK) return rc;
     *n = tab.v[dev].load(std::memory_order_acquire);
     if (*n == 0) {
-        auto kern = k_ffn_mid<__nv_bfloat16, TB200_ACT_SILU, SHARES, false>;
+        auto kern = k_ffn_mid<__nv_bfloat16, TB200_ACT_SILU, SHARES, false, false>;
         TB200_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMidSmemBytes));
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(static_cast<unsigned>(num_sms() / SHARES * SHARES), 1, 1);
@@ -1026,7 +1078,7 @@ int clusters_of(int* n) {                        // clusters of SHARES CTAs that
 // blocks of weights), or what it takes to
 // bring its bytes from L2 to the SM (95 GB/s each) or all CTAs' weights from HBM (6.4 TB/s); a wave takes its stages
 // and 0.6 us; sharing costs 0.8 us and the peers' sums at 20 GB/s.
-int mid_plan(int64_t m, int64_t f, int64_t k, MidPlan* plan) {
+int mid_plan(int64_t m, int64_t f, int64_t k, int least_width, MidPlan* plan) {
     int clusters[4] = {num_sms(), 0, 0, 0};
     int rc = clusters_of<2>(&clusters[1]);
     if (rc == TB200_OK) rc = clusters_of<4>(&clusters[2]);
@@ -1037,7 +1089,7 @@ int mid_plan(int64_t m, int64_t f, int64_t k, MidPlan* plan) {
     for (int i = 0; i < 4; ++i) {
         const int shares = 1 << i;
         if (shares > KB) break;                                  // every share has a stage
-        for (int w = 8; w <= kHalf; w += 8) {
+        for (int w = least_width; w <= kHalf; w += 8) {
             const int64_t tiles = (f + w - 1) / w;
             if (shares > 1 && tiles > clusters[i]) continue;     // shared tiles run in one wave
             const int64_t waves = (tiles + clusters[i] - 1) / clusters[i], at_once = (tiles < clusters[i] ? tiles : clusters[i]) * shares;
@@ -1054,9 +1106,9 @@ int mid_plan(int64_t m, int64_t f, int64_t k, MidPlan* plan) {
     return TB200_OK;
 }
 
-template <typename T, int ACT, int SHARES, bool FEW>
+template <typename T, int ACT, int SHARES, bool FEW, bool SAVE>
 int launch_mid(const MidMaps& maps, const MidArgs& args, cudaStream_t st) {
-    auto kern = k_ffn_mid<T, ACT, SHARES, FEW>;
+    auto kern = k_ffn_mid<T, ACT, SHARES, FEW, SAVE>;
     static PerDeviceInt attr_set;
     const int rc = ensure_max_smem(attr_set, reinterpret_cast<const void*>(kern), kMidSmemBytes);
     if (rc != TB200_OK) return rc;
@@ -1064,32 +1116,37 @@ int launch_mid(const MidMaps& maps, const MidArgs& args, cudaStream_t st) {
     return launch_over_previous(kern, SHARES > 1 ? tiles * SHARES : tiles < num_sms() ? tiles : num_sms(), kThreads, kMidSmemBytes, SHARES, st, maps, args);
 }
 
-template <typename T, int ACT, bool FEW>
+template <typename T, int ACT, bool FEW, bool SAVE>
 int launch_mid_shares(const MidMaps& maps, const MidArgs& args, int shares, cudaStream_t st) {
     switch (shares) {
-        case 1: return launch_mid<T, ACT, 1, FEW>(maps, args, st);
-        case 2: return launch_mid<T, ACT, 2, FEW>(maps, args, st);
-        case 4: return launch_mid<T, ACT, 4, FEW>(maps, args, st);
-        default: return launch_mid<T, ACT, 8, FEW>(maps, args, st);
+        case 1: return launch_mid<T, ACT, 1, FEW, SAVE>(maps, args, st);
+        case 2: return launch_mid<T, ACT, 2, FEW, SAVE>(maps, args, st);
+        case 4: return launch_mid<T, ACT, 4, FEW, SAVE>(maps, args, st);
+        default: return launch_mid<T, ACT, 8, FEW, SAVE>(maps, args, st);
     }
 }
-template <typename T, bool FEW>
+template <typename T, bool FEW, bool SAVE>
 int launch_mid_act(const MidMaps& maps, const MidArgs& args, int shares, int act, cudaStream_t st) {
     switch (act) {
-        case TB200_ACT_SILU: return launch_mid_shares<T, TB200_ACT_SILU, FEW>(maps, args, shares, st);
-        case TB200_ACT_GELU: return launch_mid_shares<T, TB200_ACT_GELU, FEW>(maps, args, shares, st);
-        case TB200_ACT_GELU_TANH: return launch_mid_shares<T, TB200_ACT_GELU_TANH, FEW>(maps, args, shares, st);
-        default: return launch_mid_shares<T, TB200_ACT_RELU, FEW>(maps, args, shares, st);
+        case TB200_ACT_SILU: return launch_mid_shares<T, TB200_ACT_SILU, FEW, SAVE>(maps, args, shares, st);
+        case TB200_ACT_GELU: return launch_mid_shares<T, TB200_ACT_GELU, FEW, SAVE>(maps, args, shares, st);
+        case TB200_ACT_GELU_TANH: return launch_mid_shares<T, TB200_ACT_GELU_TANH, FEW, SAVE>(maps, args, shares, st);
+        default: return launch_mid_shares<T, TB200_ACT_RELU, FEW, SAVE>(maps, args, shares, st);
     }
 }
 
 template <typename T>
-int ffn_mid(const void* x, const void* wg, const void* wu, void* h, int64_t m, int64_t f, int64_t k, int64_t ldx, int act, cudaStream_t st) {
+int ffn_mid(const void* x, const void* wg, const void* wu, void* h, void* gq, float* gs, void* uq, float* us, int64_t m, int64_t f, int64_t k,
+            int64_t ldx, int act, cudaStream_t st) {
     MidPlan plan = {kHalf, 1};
-    int rc = mid_plan(m, f, k, &plan);
+    int rc = mid_plan(m, f, k, gq ? kHalf : 8, &plan);
     if (rc != TB200_OK) return rc;
     MidArgs args = {};
     args.h = h;
+    args.codes[0] = static_cast<uint8_t*>(gq);
+    args.codes[1] = static_cast<uint8_t*>(uq);
+    args.scales[0] = gs;
+    args.scales[1] = us;
     args.m = static_cast<int>(m);
     args.f = static_cast<int>(f);
     args.depth = static_cast<int>(k);
@@ -1105,7 +1162,8 @@ int ffn_mid(const void* x, const void* wg, const void* wu, void* h, int64_t m, i
     if (rc == TB200_OK) rc = map_k<T>(&maps.wg, wg, f, k, k, plan.w);
     if (rc == TB200_OK) rc = map_k<T>(&maps.wu, wu, f, k, k, plan.w);
     if (rc != TB200_OK) return rc;
-    return few ? launch_mid_act<T, true>(maps, args, plan.shares, act, st) : launch_mid_act<T, false>(maps, args, plan.shares, act, st);
+    if (gq) return launch_mid_act<T, true, true>(maps, args, plan.shares, act, st);
+    return few ? launch_mid_act<T, true, false>(maps, args, plan.shares, act, st) : launch_mid_act<T, false, false>(maps, args, plan.shares, act, st);
 }
 
 // Hidden units per tile of the pair kernel: 128, or the multiple of 8 that leaves the least idle at the end.  A wave's time
@@ -1301,11 +1359,11 @@ extern "C" int tb200_ffn_gated(const void* x, const void* wg, const void* wu, vo
     if (!aligned16(x) || !aligned16(wg) || !aligned16(wu)) return fail(TB200_ERR_ALIGN, "ffn_gated: x, wg, wu must be 16-byte aligned");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // Up to 128 rows one CTA's accumulator holds them all and narrow tiles share the weights out evenly (1 row of 4096 ->
-    // 14336: 41 us against the pair kernel's 70); beyond, two CTAs share each weight tile.  Checkpoints need whole
-    // 128-wide blocks, which the pair kernel's tiles are.
-    if (!given && m <= kHalf)
-        return dtype == TB200_DT_F16 ? ffn_mid<__half>(x, wg, wu, h, m, f, k, ldx, act, st)
-                                     : ffn_mid<__nv_bfloat16>(x, wg, wu, h, m, f, k, ldx, act, st);
+    // 14336: 40 us against the pair kernel's 70); beyond, two CTAs share each weight tile.  Checkpoints need whole
+    // 128-wide blocks: tiles of that width for up to 64 rows, the pair kernel's beyond.
+    if (m <= (given ? kFewRows : kHalf))
+        return dtype == TB200_DT_F16 ? ffn_mid<__half>(x, wg, wu, h, gq, gs, uq, us, m, f, k, ldx, act, st)
+                                     : ffn_mid<__nv_bfloat16>(x, wg, wu, h, gq, gs, uq, us, m, f, k, ldx, act, st);
     return dtype == TB200_DT_F16 ? ffn_forward<__half>(x, wg, wu, h, gq, gs, uq, us, m, f, k, ldx, act, st)
                                  : ffn_forward<__nv_bfloat16>(x, wg, wu, h, gq, gs, uq, us, m, f, k, ldx, act, st);
 }
