@@ -283,6 +283,28 @@ def test_backward_gates(cuda_device, act):
         check_gradients(bwd.run(*args, act), args, act, torch.float16)
 
 
+@pytest.mark.parametrize("m,k,f", [(3000, 136, 140), (9000, 264, 24), (520, 72, 9000), (70, 2056, 5000)])
+def test_backward_in_shares(cuda_device, m, k, f):
+    """Sizes whose tiles are too few, for the gradient of x or for those of the weights: the contraction is shared out."""
+    for x_codes in (True, False):
+        args = backward_inputs(m, k, f, torch.bfloat16, x_codes)
+        check_gradients(bwd.run(*args, "silu"), args, "silu", torch.bfloat16)
+
+
+@pytest.mark.parametrize("offset", [1, 2, 4])
+def test_backward_takes_codes_at_odd_addresses(cuda_device, offset):
+    args = list(backward_inputs(33, 72, 136, torch.float16))
+    want = bwd.run(*args, "relu")
+
+    def moved(t):
+        flat = torch.zeros(t.numel() + 16, dtype=torch.uint8, device="cuda")
+        flat[offset:offset + t.numel()] = t.view(torch.uint8).flatten()
+        return flat[offset:offset + t.numel()].view(t.shape).view(t.dtype)
+    for i in (3, 5, 7):
+        args[i] = moved(args[i])
+    assert all(torch.equal(a, b) for a, b in zip(bwd.run(*args, "relu"), want))
+
+
 def test_backward_takes_a_strided_input(cuda_device):
     args = list(backward_inputs(70, 136, 200, torch.bfloat16, x_codes=False))
     wide = torch.zeros(70, 160, dtype=torch.bfloat16, device="cuda")

@@ -389,6 +389,46 @@ __global__ void __launch_bounds__(kThreads) k_restore_any(const uint8_t* __restr
     }
 }
 
+// The backward pass's input, where it is small, restored by the last CTAs of the kernel that makes dg and du (a launch of its own
+// takes 3 us whatever the work): 8 codes per thread, columns a multiple of 8, so that no piece has two scales.
+struct RestoreJob {
+    const uint2* q;
+    const float* scales;
+    uint4* out;
+    uint32_t total, per_row, nblk;                               // pieces of 8, in all and per row; blocks per row
+    int ctas;                                                    // 0: nothing to restore
+};
+template <typename T>
+__device__ __forceinline__ void restore_job(const RestoreJob& job, uint32_t cta) {
+    constexpr int U = 2;
+    const uint64_t step = static_cast<uint64_t>(job.ctas) * kThreads;
+    for (uint64_t i0 = static_cast<uint64_t>(cta) * kThreads + threadIdx.x; i0 < job.total; i0 += U * step) {
+        uint2 c[U];
+        float s[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const uint64_t i = i0 + j * step;
+            if (i < job.total) {
+                const uint32_t row = static_cast<uint32_t>(i) / job.per_row;
+                c[j] = __ldcs(job.q + i);
+                s[j] = __ldg(job.scales + static_cast<int64_t>(row) * job.nblk + (static_cast<uint32_t>(i) - row * job.per_row) / 16);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const uint64_t i = i0 + j * step;
+            if (i < job.total) {
+                const uint32_t codes[2] = {c[j].x, c[j].y};
+                float v[8];
+                uint32_t w[4];
+                decode<8>(codes, s[j], ActType<T>::kTop, v);
+                words<T, 4>(v, w);
+                job.out[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+    }
+}
+
 // dg = dh * u * f'(g), du = dh * f(g) for 8 numbers of a lane.
 template <typename T, int ACT>
 __device__ __forceinline__ void gated_bwd8(const uint32_t (&d)[4], const uint32_t (&cg)[2], const uint32_t (&cu)[2], float sg, float su,
@@ -414,9 +454,11 @@ __device__ __forceinline__ void gated_bwd8(const uint32_t (&d)[4], const uint32_
 template <typename T, int ACT, int U>
 __global__ void __launch_bounds__(kThreads) k_gated_bwd(const uint4* __restrict__ dh, const uint2* __restrict__ gq, const float* __restrict__ gs,
                                                         const uint2* __restrict__ uq, const float* __restrict__ us, uint4* __restrict__ dg,
-                                                        uint4* __restrict__ du, uint32_t total, uint32_t per_row, uint32_t nblk) {
+                                                        uint4* __restrict__ du, uint32_t total, uint32_t per_row, uint32_t nblk,
+                                                        const RestoreJob job) {
     let_next_begin();
-    const uint32_t step = gridDim.x * kThreads;
+    const uint32_t ctas = gridDim.x - job.ctas, step = ctas * kThreads;
+    if (blockIdx.x >= ctas) return restore_job<T>(job, blockIdx.x - ctas);
     for (uint64_t i0 = blockIdx.x * kThreads + threadIdx.x; i0 < total; i0 += U * step) {
         uint4 d[U];
         uint2 cg[U], cu[U];
@@ -452,13 +494,15 @@ template <typename T, int ACT>
 __global__ void __launch_bounds__(kThreads) k_gated_bwd_any(const T* __restrict__ dh, const uint8_t* __restrict__ gq, const float* __restrict__ gs,
                                                             const uint8_t* __restrict__ uq, const float* __restrict__ us, T* __restrict__ dg,
                                                             T* __restrict__ du, int64_t spans, uint32_t per_row, int width, int64_t m, int64_t f,
-                                                            int64_t ldg, uint32_t nblk) {
+                                                            int64_t ldg, uint32_t nblk, const RestoreJob job) {
     let_next_begin();
+    const uint32_t ctas = gridDim.x - job.ctas;
+    if (blockIdx.x >= ctas) return restore_job<T>(job, blockIdx.x - ctas);
     static_assert(sizeof(T) == 2, "8 numbers of 16 bits and 8 codes per lane");
     constexpr int E = Part<T>::E, kCols = Part<T>::kCols;
     const int lane = threadIdx.x & 31;
     const int64_t total = m * f;
-    for (int64_t s = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); s < spans; s += static_cast<int64_t>(gridDim.x) * (kThreads / 32)) {
+    for (int64_t s = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); s < spans; s += static_cast<int64_t>(ctas) * (kThreads / 32)) {
         const int64_t row = s / per_row, first = (s - row * per_row) * width, at0 = row * f + first;
         const int n = static_cast<int>(min(static_cast<int64_t>(width), f - first));
         const int64_t blk = row * nblk + first / kActBlock;
@@ -557,19 +601,19 @@ int launch_restore(const uint8_t* q, const float* scales, T* out, int64_t rows, 
 
 template <typename T, int ACT>
 int launch_gated(const void* dh, const void* gq, const float* gs, const void* uq, const float* us, void* dg, void* du, int64_t m, int64_t f,
-                 int64_t ldg, cudaStream_t st) {
+                 int64_t ldg, const RestoreJob& job, cudaStream_t st) {
     const uint32_t nblk = static_cast<uint32_t>((f + kActBlock - 1) / kActBlock);
     if (f % 8 == 0 && aligned_to(16, dh, 0) && aligned_to(8, gq, 0) && aligned_to(8, uq, 0) && m * (f / 8) <= 0xFFFFFFFFll) {
         const int64_t total = m * (f / 8);
         constexpr int U = 2;
-        k_gated_bwd<T, ACT, U><<<capped((total + kThreads * U - 1) / (kThreads * U), 8), kThreads, 0, st>>>(
+        k_gated_bwd<T, ACT, U><<<capped((total + kThreads * U - 1) / (kThreads * U), 8) + job.ctas, kThreads, 0, st>>>(
             static_cast<const uint4*>(dh), static_cast<const uint2*>(gq), gs, static_cast<const uint2*>(uq), us, static_cast<uint4*>(dg),
-            static_cast<uint4*>(du), static_cast<uint32_t>(total), static_cast<uint32_t>(f / 8), nblk);
+            static_cast<uint4*>(du), static_cast<uint32_t>(total), static_cast<uint32_t>(f / 8), nblk, job);
     } else {
         const Spans sp = spans_of(m, f, Part<T>::kCols);
-        k_gated_bwd_any<T, ACT><<<capped((sp.count + 7) / 8, 8), kThreads, 0, st>>>(
+        k_gated_bwd_any<T, ACT><<<capped((sp.count + 7) / 8, 8) + job.ctas, kThreads, 0, st>>>(
             static_cast<const T*>(dh), static_cast<const uint8_t*>(gq), gs, static_cast<const uint8_t*>(uq), us, static_cast<T*>(dg),
-            static_cast<T*>(du), sp.count, sp.per_row, sp.width, m, f, ldg, nblk);
+            static_cast<T*>(du), sp.count, sp.per_row, sp.width, m, f, ldg, nblk, job);
     }
     TB200_CUDA_TRY(cudaGetLastError());
     return TB200_OK;
@@ -577,12 +621,12 @@ int launch_gated(const void* dh, const void* gq, const float* gs, const void* uq
 
 template <typename T>
 int launch_gated_act(const void* dh, const void* gq, const float* gs, const void* uq, const float* us, void* dg, void* du, int64_t m, int64_t f,
-                     int64_t ldg, int act, cudaStream_t st) {
+                     int64_t ldg, const RestoreJob& job, int act, cudaStream_t st) {
     switch (act) {
-        case TB200_ACT_SILU: return launch_gated<T, TB200_ACT_SILU>(dh, gq, gs, uq, us, dg, du, m, f, ldg, st);
-        case TB200_ACT_GELU: return launch_gated<T, TB200_ACT_GELU>(dh, gq, gs, uq, us, dg, du, m, f, ldg, st);
-        case TB200_ACT_GELU_TANH: return launch_gated<T, TB200_ACT_GELU_TANH>(dh, gq, gs, uq, us, dg, du, m, f, ldg, st);
-        default: return launch_gated<T, TB200_ACT_RELU>(dh, gq, gs, uq, us, dg, du, m, f, ldg, st);
+        case TB200_ACT_SILU: return launch_gated<T, TB200_ACT_SILU>(dh, gq, gs, uq, us, dg, du, m, f, ldg, job, st);
+        case TB200_ACT_GELU: return launch_gated<T, TB200_ACT_GELU>(dh, gq, gs, uq, us, dg, du, m, f, ldg, job, st);
+        case TB200_ACT_GELU_TANH: return launch_gated<T, TB200_ACT_GELU_TANH>(dh, gq, gs, uq, us, dg, du, m, f, ldg, job, st);
+        default: return launch_gated<T, TB200_ACT_RELU>(dh, gq, gs, uq, us, dg, du, m, f, ldg, job, st);
     }
 }
 
@@ -597,9 +641,22 @@ int check_sizes(const char* what, int64_t rows, int64_t cols) {
 }  // namespace
 
 int launch_gated_act_bwd(const void* dh, const void* gq, const float* gs, const void* uq, const float* us, void* dg, void* du,
-                         int64_t m, int64_t f, int64_t ldg, int act, int dtype, cudaStream_t st) {
-    return dtype == TB200_DT_F16 ? launch_gated_act<__half>(dh, gq, gs, uq, us, dg, du, m, f, ldg, act, st)
-                                 : launch_gated_act<__nv_bfloat16>(dh, gq, gs, uq, us, dg, du, m, f, ldg, act, st);
+                         int64_t m, int64_t f, int64_t ldg, const void* xq, const float* xs, void* x, int64_t k, int act, int dtype,
+                         cudaStream_t st) {
+    RestoreJob job = {};
+    if (xq) {
+        const int64_t total = m * (k / 8);
+        // up to 4 M numbers (5 us by themselves); 12867 x 3616 took 52 us together with dg and du, 40 in two launches
+        if ((reinterpret_cast<uintptr_t>(xq) & 7) == 0 && m * k <= (4ll << 20)) {
+            job = {static_cast<const uint2*>(xq), xs, static_cast<uint4*>(x), static_cast<uint32_t>(total), static_cast<uint32_t>(k / 8),
+                   static_cast<uint32_t>((k + kActBlock - 1) / kActBlock), capped((total + 2 * kThreads - 1) / (2 * kThreads), 8)};
+        } else {
+            const int rc = launch_act_restore(xq, xs, x, dtype, m, k, st);
+            if (rc != TB200_OK) return rc;
+        }
+    }
+    return dtype == TB200_DT_F16 ? launch_gated_act<__half>(dh, gq, gs, uq, us, dg, du, m, f, ldg, job, act, st)
+                                 : launch_gated_act<__nv_bfloat16>(dh, gq, gs, uq, us, dg, du, m, f, ldg, job, act, st);
 }
 
 int launch_act_restore(const void* q, const float* scales, void* out, int dtype, int64_t rows, int64_t cols, cudaStream_t st) {

@@ -186,9 +186,11 @@ int launch_over_previous(void (*kern)(Maps, Args), int grid, int block, int smem
 #endif
 
 // ---- launchers shared between the files of the feed-forward block ----------------------------------------------
-// The products of the backward pass's two intermediates: dg = dh * u * f'(g), du = dh * f(g), row pitch ldg.
+// The backward pass's two intermediates, dg = dh * u * f'(g) and du = dh * f(g) with row pitch ldg; and, where xq is given, the
+// block's input [m, k] restored from its 8-bit form (k a multiple of 8).
 int launch_gated_act_bwd(const void* dh, const void* gq, const float* gs, const void* uq, const float* us, void* dg, void* du,
-                         int64_t m, int64_t f, int64_t ldg, int act, int dtype, cudaStream_t st);
+                         int64_t m, int64_t f, int64_t ldg, const void* xq, const float* xs, void* x, int64_t k, int act, int dtype,
+                         cudaStream_t st);
 int launch_act_restore(const void* q, const float* scales, void* out, int dtype, int64_t rows, int64_t cols, cudaStream_t st);
 
 }  // namespace tb200

@@ -49,9 +49,9 @@ struct FfnMaps {
 };
 struct FfnArgs {
     void* out[2];                                // forward: h, -      dx: dx, -      dw: dWg, dWu
-    float* sums;                                 // dx in shares: [splits, rows, cols] partial sums
+    float* sums;                                 // in shares: partial sums, dx [splits, rows, cols], dw [splits, 2, rows, cols]
     int rows, cols, depth;                       // of one result, and of one product's contraction
-    int splits;                                  // dx: shares of the contraction
+    int splits;                                  // dx, dw: shares of the contraction
     int w;                                       // forward: hidden units per tile (128 with checkpoints)
     uint8_t* codes[2];                           // forward with checkpoints: codes of g and u, [rows, cols]
     float* scales[2];                            // and their scales, [rows, ceil(cols / 128)]
@@ -229,7 +229,7 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
     const int tiles_m = KIND == FK_DW ? 2 * tm1 : tm1;          // dw: the tiles of dWg, then those of dWu
     const int tiles_n = (p.cols + tile_cols - 1) / tile_cols;
     const int tiles = tiles_m * tiles_n;
-    const int items = KIND == FK_DX ? tiles * p.splits : tiles; // dx: item i is share i / tiles of tile i % tiles
+    const int items = KIND != FK_FWD ? tiles * p.splits : tiles; // dx, dw: item i is share i / tiles of tile i % tiles
 
     let_next_begin();
     if (SAVE && threadIdx.x < kAmaxBytes / 4) amax[threadIdx.x] = 0;
@@ -267,12 +267,12 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
             uint32_t s = 0, ph = 1;
             bool ok = true;
             for (int t = pair; t < items && ok; t += npairs) {
-                const int share = KIND == FK_DX ? t / tiles : 0;
+                const int share = KIND != FK_FWD ? t / tiles : 0;
                 const Tile tc = tile_at(t - share * tiles, tiles_m, tiles_n);
                 const int sel = KIND == FK_DW && tc.m >= tm1 ? 1 : 0;
                 const int a_row = (tc.m - sel * tm1) * 2 * kHalf + rank * kHalf;
                 const int b_col = KIND == FK_FWD ? tc.n * tile_cols : tc.n * 2 * kHalf + rank * kHalf;
-                const int st0 = KIND == FK_DX ? share_at(steps, share, p.splits) : 0, st1 = KIND == FK_DX ? share_at(steps, share + 1, p.splits) : steps;
+                const int st0 = KIND != FK_FWD ? share_at(steps, share, p.splits) : 0, st1 = KIND != FK_FWD ? share_at(steps, share + 1, p.splits) : steps;
                 for (int st = st0; st < st1; ++st) {
                     if (!mbar_wait(&bar_empty[s], ph, ST_WAIT_SMEM_EMPTY, st)) { ok = false; break; }
                     uint8_t* stage = smem + s * kStageBytes;
@@ -318,8 +318,8 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
             if (!mbar_wait(&bar_aempty[acc], ((cnt >> 1) & 1) ^ 1, ST_WAIT_TMEM_EMPTY, t)) { ok = false; break; }
             tc_fence_after();
             const uint32_t d_tmem = tmem_base + acc * 256;
-            const int share = KIND == FK_DX ? t / tiles : 0;
-            const int n = KIND == FK_DX ? share_at(steps, share + 1, p.splits) - share_at(steps, share, p.splits) : steps;
+            const int share = KIND != FK_FWD ? t / tiles : 0;
+            const int n = KIND != FK_FWD ? share_at(steps, share + 1, p.splits) - share_at(steps, share, p.splits) : steps;
             for (int st = 0; st < n; ++st) {
                 if (!ready && !mbar_wait(&bar_full[s], ph, ST_WAIT_SMEM_FULL, st)) { ok = false; break; }
                 tc_fence_after();
@@ -343,7 +343,7 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
         uint32_t cnt = 0;
         bool ok = true;
         for (int t = pair; t < items; t += npairs, ++cnt) {
-            const int share = KIND == FK_DX ? t / tiles : 0;
+            const int share = KIND != FK_FWD ? t / tiles : 0;
             const Tile tc = tile_at(t - share * tiles, tiles_m, tiles_n);
             const int sel = KIND == FK_DW && tc.m >= tm1 ? 1 : 0;
             const uint32_t acc = cnt & 1;
@@ -423,8 +423,8 @@ k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs
                     flush<uint8_t, 8>(buf, 8, p.codes[1] + to, p.cols, r8, rows, cols, lane);
                     quarter_sync(quarter);
                 }
-            } else if (KIND == FK_DX && p.splits > 1) {          // partial sums in 32 bits, 64 columns at a time
-                float* dst = p.sums + (static_cast<int64_t>(share) * p.rows + row0) * p.cols + col0;
+            } else if (p.splits > 1) {                           // partial sums in 32 bits, 64 columns at a time
+                float* dst = p.sums + (static_cast<int64_t>(KIND == FK_DW ? 2 * share + sel : share) * p.rows + row0) * p.cols + col0;
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     uint32_t v[16];
@@ -1027,7 +1027,7 @@ int launch_pair(const FfnMaps& maps, const FfnArgs& args, cudaStream_t st) {
         max_pairs_tab.v[dev].store(clusters, std::memory_order_release);
     }
     const int64_t tile_cols = KIND == FK_FWD ? args.w : 2 * kHalf;
-    const int64_t tiles = (KIND == FK_DW ? 2 : KIND == FK_DX ? args.splits : 1) * ((args.rows + 2 * kHalf - 1) / (2 * kHalf)) * ((args.cols + tile_cols - 1) / tile_cols);
+    const int64_t tiles = (KIND == FK_DW ? 2 : 1) * (KIND == FK_FWD ? 1 : args.splits) * ((args.rows + 2 * kHalf - 1) / (2 * kHalf)) * ((args.cols + tile_cols - 1) / tile_cols);
     if (tiles > 0x7fffffffll / kGroupM) return fail(TB200_ERR_UNSUPPORTED, "ffn_gated: too many tiles");
     const int pairs = static_cast<int>(tiles < max_pairs ? tiles : max_pairs);
     return launch_over_previous(kern, 2 * pairs, kThreads, kSmemBytes, 1, st, maps, args);
@@ -1229,15 +1229,32 @@ int dx_splits(int64_t m, int64_t f, int64_t k) {
     return best;
 }
 
-// out = the sum of `splits` arrays of n numbers, in order; 8 numbers per thread.
+// The same for dw, whose tiles are too few where the model is small and the tokens are many.
+int dw_splits(int64_t m, int64_t f, int64_t k) {
+    const int64_t pairs = num_sms() / 2, tiles = 2 * ((f + 2 * kHalf - 1) / (2 * kHalf)) * ((k + 2 * kHalf - 1) / (2 * kHalf));
+    const int64_t steps = (m + kBK - 1) / kBK;
+    int best = 1;
+    double least = 0.0;
+    for (int s = 1; s <= 16 && steps >= 8 * (s - 1); ++s) {
+        const double cost = static_cast<double>((tiles * s + pairs - 1) / pairs) * static_cast<double>((steps + s - 1) / s + 2) +
+                            (s > 1 ? 20.0 + static_cast<double>(f) * k * 16.0 * s / (5e6 * 0.27) : 0.0);
+        if (s == 1 || cost < least) {
+            least = cost;
+            best = s;
+        }
+    }
+    return best;
+}
+
+// out = the sum of `splits` arrays of n numbers that lie `stride8` pieces of 8 apart, in order; 8 numbers per thread.
 template <typename T>
-__global__ void __launch_bounds__(256) k_sum_shares(const float4* __restrict__ sums, uint4* __restrict__ out, int64_t n8, int splits) {
+__global__ void __launch_bounds__(256) k_sum_shares(const float4* __restrict__ sums, uint4* __restrict__ out, int64_t n8, int64_t stride8, int splits) {
     let_next_begin();
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n8; i += static_cast<int64_t>(gridDim.x) * 256) {
         float4 a = sums[2 * i], b = sums[2 * i + 1];
 #pragma unroll 4
         for (int s = 1; s < splits; ++s) {
-            const float4 c = sums[2 * (s * n8 + i)], d = sums[2 * (s * n8 + i) + 1];
+            const float4 c = sums[2 * (s * stride8 + i)], d = sums[2 * (s * stride8 + i) + 1];
             a.x += c.x; a.y += c.y; a.z += c.z; a.w += c.w;
             b.x += d.x; b.y += d.y; b.z += d.z; b.w += d.w;
         }
@@ -1294,22 +1311,26 @@ int dx_few(const void* dg, const void* du, int64_t ldg, const void* wg, const vo
     return launch_over_previous(kern, static_cast<int>(items < num_sms() ? items : num_sms()), kDxThreads, kDxSmemBytes, 1, st, maps, args);
 }
 
-// dg, du: [m, ldg]; x: [m, k]; sums: room for dx_splits() arrays of [m, k] where that is more than 1
+template <typename T>
+int launch_sum(const float* sums, void* out, int64_t n, int64_t stride, int splits, cudaStream_t st) {
+    const int64_t ctas = (n / 8 + 255) / 256, cap = static_cast<int64_t>(num_sms()) * 8;
+    k_sum_shares<T><<<static_cast<unsigned>(ctas < cap ? ctas : cap), 256, 0, st>>>(reinterpret_cast<const float4*>(sums), static_cast<uint4*>(out), n / 8,
+                                                                                  stride / 8, splits);
+    TB200_CUDA_TRY(cudaGetLastError());
+    return TB200_OK;
+}
+
+// dg, du: [m, ldg]; x: [m, k]; sums: room for dx_splits() arrays of [m, k] and, later, for dw_splits() of [2, f, k], where those are
+// more than 1
 template <typename T>
 int ffn_products_bwd(const void* dg, const void* du, int64_t ldg, const void* x, int64_t ldx, const void* wg, const void* wu, void* dx, void* dwg,
                      void* dwu, float* sums, int64_t m, int64_t f, int64_t k, cudaStream_t st) {
-    const int splits = dx_splits(m, f, k);
+    int splits = dx_splits(m, f, k);
     int rc = m <= kFewRows ? dx_few<T>(dg, du, ldg, wg, wu, dx, sums, splits, m, f, k, st) : dx_pair<T>(dg, du, ldg, wg, wu, dx, sums, splits, m, f, k, st);
+    if (rc == TB200_OK && splits > 1) rc = launch_sum<T>(sums, dx, m * k, m * k, splits, st);
     if (rc != TB200_OK) return rc;
-    if (splits > 1) {
-        const int64_t n8 = m * (k / 8), ctas = (n8 + 255) / 256, cap = static_cast<int64_t>(num_sms()) * 8;
-        k_sum_shares<T><<<static_cast<unsigned>(ctas < cap ? ctas : cap), 256, 0, st>>>(reinterpret_cast<const float4*>(sums), static_cast<uint4*>(dx), n8,
-                                                                                      splits);
-        TB200_CUDA_TRY(cudaGetLastError());
-    }
 
     FfnMaps maps;
-    FfnArgs args = {};
     memset(&maps, 0, sizeof(maps));
     rc = map_mn<T>(&maps.a[0], dg, m, f, ldg);
     if (rc == TB200_OK) rc = map_mn<T>(&maps.a[1], du, m, f, ldg);
@@ -1317,12 +1338,19 @@ int ffn_products_bwd(const void* dg, const void* du, int64_t ldg, const void* x,
     if (rc == TB200_OK) rc = map_out<T>(&maps.out[0], dwg, f, k);
     if (rc == TB200_OK) rc = map_out<T>(&maps.out[1], dwu, f, k);
     if (rc != TB200_OK) return rc;
+    splits = dw_splits(m, f, k);
+    FfnArgs args = {};
+    args.out[0] = dwg;
+    args.out[1] = dwu;
+    args.sums = sums;
     args.rows = static_cast<int>(f);
     args.cols = static_cast<int>(k);
     args.depth = static_cast<int>(m);
-    args.out[0] = dwg;
-    args.out[1] = dwu;
-    return launch_pair<FK_DW, T, 0, false>(maps, args, st);
+    args.splits = splits;
+    rc = launch_pair<FK_DW, T, 0, false>(maps, args, st);
+    if (rc == TB200_OK && splits > 1) rc = launch_sum<T>(sums, dwg, f * k, 2 * f * k, splits, st);
+    if (rc == TB200_OK && splits > 1) rc = launch_sum<T>(sums + f * k, dwu, f * k, 2 * f * k, splits, st);
+    return rc;
 }
 
 constexpr int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
@@ -1370,9 +1398,10 @@ extern "C" int tb200_ffn_gated(const void* x, const void* wg, const void* wu, vo
 
 extern "C" size_t tb200_ffn_gated_bwd_workspace_bytes(int64_t m, int64_t f, int64_t k, int x_codes) {
     if (m <= 0 || f <= 0 || k <= 0) return 0;
-    const int64_t splits = dx_splits(m, f, k);
+    const int64_t dx = dx_splits(m, f, k), dw = dw_splits(m, f, k);
+    const int64_t dx_sums = dx > 1 ? dx * m * k * 4 : 0, dw_sums = dw > 1 ? dw * 2 * f * k * 4 : 0;
     return static_cast<size_t>(2 * round_up(m * pitch_of(f) * 2, 256) + (x_codes ? round_up(m * k * 2, 256) : 0) +
-                               (splits > 1 ? splits * m * k * 4 : 0));
+                               (dx_sums > dw_sums ? dx_sums : dw_sums));
 }
 
 extern "C" int tb200_ffn_gated_bwd(const void* dh, const void* wg, const void* wu, const void* x, const float* xs, const void* gq,
@@ -1405,13 +1434,9 @@ extern "C" int tb200_ffn_gated_bwd(const void* dh, const void* wg, const void* w
     void* du = ws + round_up(m * ldg * 2, 256);
     void* xr = ws + 2 * round_up(m * ldg * 2, 256);
     float* sums = reinterpret_cast<float*>(static_cast<uint8_t*>(xr) + (codes ? round_up(m * k * 2, 256) : 0));
-    rc = launch_gated_act_bwd(dh, gq, gs, uq, us, dg, du, m, f, ldg, act, dtype, st);
+    rc = launch_gated_act_bwd(dh, gq, gs, uq, us, dg, du, m, f, ldg, codes ? x : nullptr, xs, xr, k, act, dtype, st);
     if (rc != TB200_OK) return rc;
-    if (codes) {
-        rc = launch_act_restore(x, xs, xr, dtype, m, k, st);
-        if (rc != TB200_OK) return rc;
-        x = xr;
-    }
+    if (codes) x = xr;
     return dtype == TB200_DT_F16 ? ffn_products_bwd<__half>(dg, du, ldg, x, ldx, wg, wu, dx, dwg, dwu, sums, m, f, k, st)
                                  : ffn_products_bwd<__nv_bfloat16>(dg, du, ldg, x, ldx, wg, wu, dx, dwg, dwu, sums, m, f, k, st);
 }
