@@ -88,7 +88,7 @@ __device__ __forceinline__ void decode(const uint32_t (&codes)[E / 4], float s, 
 // ends inside a block where cols is not a multiple of 128 (lanes past it hold zeros).  FLAT: rows are whole blocks and
 // adjacent, so the piece's number is its place.
 template <typename T, int U, bool FLAT>
-__global__ void __launch_bounds__(kThreads) k_save(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales,
+__global__ void __launch_bounds__(kThreads) tb200_k_act_save(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales,
                                                    uint32_t blocks, uint32_t nblk, int64_t cols, int64_t ldx) {
     let_next_begin();
     constexpr int E = 32 / sizeof(T), kLanes = kActBlock / E;
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(kThreads) k_save(const T* __restrict__ x, uint
 
 // Restoring: E codes per lane make one 32-byte piece.
 template <typename T, int U, bool FLAT>
-__global__ void __launch_bounds__(kThreads) k_restore(const uint8_t* __restrict__ q, const float* __restrict__ scales, T* __restrict__ out,
+__global__ void __launch_bounds__(kThreads) tb200_k_act_restore(const uint8_t* __restrict__ q, const float* __restrict__ scales, T* __restrict__ out,
                                                       uint32_t blocks, uint32_t nblk, int64_t cols) {
     let_next_begin();
     constexpr int E = 32 / sizeof(T), kLanes = kActBlock / E;
@@ -266,7 +266,7 @@ template <typename T> struct Part {
 
 // spans: warps' shares of the rows, per_row of them in a row, `width` columns each (a multiple of the part).
 template <typename T>
-__global__ void __launch_bounds__(kThreads) k_save_any(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales,
+__global__ void __launch_bounds__(kThreads) tb200_k_act_save_any(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales,
                                                        int64_t spans, uint32_t per_row, int width, uint32_t nblk, int64_t rows, int64_t cols,
                                                        int64_t ldx) {
     let_next_begin();
@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(kThreads) k_save_any(const T* __restrict__ x, 
 // between rows, so pieces of 16 (8 for fp32) are taken across the ends of rows and blocks.  At most two ends lie inside a piece (those
 // of a whole block and of a last one that is shorter than a piece); each code takes the scale of its side.
 template <typename T, int U>
-__global__ void __launch_bounds__(kThreads) k_restore_across(const uint8_t* __restrict__ q, const float* __restrict__ scales, T* __restrict__ out,
+__global__ void __launch_bounds__(kThreads) tb200_k_act_restore_across(const uint8_t* __restrict__ q, const float* __restrict__ scales, T* __restrict__ out,
                                                              int64_t total, uint32_t nblk, int64_t cols) {
     let_next_begin();
     constexpr int E = 32 / sizeof(T);
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(kThreads) k_restore_across(const uint8_t* __re
 
 // Restoring at any alignment and width, one number per thread.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) k_restore_any(const uint8_t* __restrict__ q, const float* __restrict__ scales, T* __restrict__ out,
+__global__ void __launch_bounds__(kThreads) tb200_k_act_restore_any(const uint8_t* __restrict__ q, const float* __restrict__ scales, T* __restrict__ out,
                                                           int64_t total, uint32_t nblk, int64_t cols) {
     let_next_begin();
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * kThreads) {
@@ -452,7 +452,7 @@ __device__ __forceinline__ void gated_bwd8(const uint32_t (&d)[4], const uint32_
 
 // Widths that are multiples of 8, 16-byte boundaries: 8 numbers per thread.
 template <typename T, int ACT, int U>
-__global__ void __launch_bounds__(kThreads) k_gated_bwd(const uint4* __restrict__ dh, const uint2* __restrict__ gq, const float* __restrict__ gs,
+__global__ void __launch_bounds__(kThreads) tb200_k_ffn_gated_bwd(const uint4* __restrict__ dh, const uint2* __restrict__ gq, const float* __restrict__ gs,
                                                         const uint2* __restrict__ uq, const float* __restrict__ us, uint4* __restrict__ dg,
                                                         uint4* __restrict__ du, uint32_t total, uint32_t per_row, uint32_t nblk,
                                                         const RestoreJob job) {
@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(kThreads) k_gated_bwd(const uint4* __restrict_
 
 // The same for any width and alignment of dh and the codes; dg and du have rows on 16-byte boundaries, ldg >= f a multiple of 8.
 template <typename T, int ACT>
-__global__ void __launch_bounds__(kThreads) k_gated_bwd_any(const T* __restrict__ dh, const uint8_t* __restrict__ gq, const float* __restrict__ gs,
+__global__ void __launch_bounds__(kThreads) tb200_k_ffn_gated_bwd_any(const T* __restrict__ dh, const uint8_t* __restrict__ gq, const float* __restrict__ gs,
                                                             const uint8_t* __restrict__ uq, const float* __restrict__ us, T* __restrict__ dg,
                                                             T* __restrict__ du, int64_t spans, uint32_t per_row, int width, int64_t m, int64_t f,
                                                             int64_t ldg, uint32_t nblk, const RestoreJob job) {
@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(kThreads) k_gated_bwd_any(const T* __restrict_
     }
 }
 
-// How k_save_any and k_gated_bwd_any share out their rows: spans of up to 4 parts, fewer where that leaves an SM less than 32
+// How tb200_k_act_save_any and tb200_k_ffn_gated_bwd_any share out their rows: spans of up to 4 parts, fewer where that leaves an SM less than 32
 // warps' worth; neighbouring warps have neighbouring spans.  A whole row per warp has fewer ragged ends, but thousands of places
 // of memory in use at once and a last round that is mostly idle (6525 x 27060: 404 us where this takes 277).
 struct Spans { int64_t count; uint32_t per_row; int width; };
@@ -568,12 +568,12 @@ int launch_save(const T* x, uint8_t* q, float* scales, int64_t rows, int64_t col
         const uint32_t blocks = static_cast<uint32_t>(rows * nblk);
         const int grid = capped((static_cast<int64_t>(blocks) * (kActBlock / E) + kThreads * U - 1) / (kThreads * U), 8);
         if (cols % kActBlock == 0 && (ldx == cols || rows == 1))
-            k_save<T, U, true><<<grid, kThreads, 0, st>>>(x, q, scales, blocks, nblk, cols, ldx);
+            tb200_k_act_save<T, U, true><<<grid, kThreads, 0, st>>>(x, q, scales, blocks, nblk, cols, ldx);
         else
-            k_save<T, U, false><<<grid, kThreads, 0, st>>>(x, q, scales, blocks, nblk, cols, ldx);
+            tb200_k_act_save<T, U, false><<<grid, kThreads, 0, st>>>(x, q, scales, blocks, nblk, cols, ldx);
     } else {
         const Spans sp = spans_of(rows, cols, Part<T>::kCols);
-        k_save_any<T><<<capped((sp.count + 7) / 8, 8), kThreads, 0, st>>>(x, q, scales, sp.count, sp.per_row, sp.width, nblk, rows, cols, ldx);
+        tb200_k_act_save_any<T><<<capped((sp.count + 7) / 8, 8), kThreads, 0, st>>>(x, q, scales, sp.count, sp.per_row, sp.width, nblk, rows, cols, ldx);
     }
     TB200_CUDA_TRY(cudaGetLastError());
     return TB200_OK;
@@ -586,14 +586,14 @@ int launch_restore(const uint8_t* q, const float* scales, T* out, int64_t rows, 
     if (cols % E == 0 && aligned_to(E, q, 0) && aligned_to(32, out, 0)) {
         const uint32_t blocks = static_cast<uint32_t>(rows * nblk);
         const int grid = capped((static_cast<int64_t>(blocks) * (kActBlock / E) + kThreads * U - 1) / (kThreads * U), 8);
-        if (cols % kActBlock == 0) k_restore<T, U, true><<<grid, kThreads, 0, st>>>(q, scales, out, blocks, nblk, cols);
-        else k_restore<T, U, false><<<grid, kThreads, 0, st>>>(q, scales, out, blocks, nblk, cols);
+        if (cols % kActBlock == 0) tb200_k_act_restore<T, U, true><<<grid, kThreads, 0, st>>>(q, scales, out, blocks, nblk, cols);
+        else tb200_k_act_restore<T, U, false><<<grid, kThreads, 0, st>>>(q, scales, out, blocks, nblk, cols);
     } else if (cols >= 16 && aligned_to(16, q, 0) && aligned_to(32, out, 0)) {
         const int64_t total = rows * cols;
-        k_restore_across<T, U><<<capped((total + kThreads * E * U - 1) / (kThreads * E * U), 8), kThreads, 0, st>>>(q, scales, out, total, nblk, cols);
+        tb200_k_act_restore_across<T, U><<<capped((total + kThreads * E * U - 1) / (kThreads * E * U), 8), kThreads, 0, st>>>(q, scales, out, total, nblk, cols);
     } else {
         const int64_t total = rows * cols;
-        k_restore_any<T><<<capped((total + kThreads - 1) / kThreads, 8), kThreads, 0, st>>>(q, scales, out, total, nblk, cols);
+        tb200_k_act_restore_any<T><<<capped((total + kThreads - 1) / kThreads, 8), kThreads, 0, st>>>(q, scales, out, total, nblk, cols);
     }
     TB200_CUDA_TRY(cudaGetLastError());
     return TB200_OK;
@@ -606,12 +606,12 @@ int launch_gated(const void* dh, const void* gq, const float* gs, const void* uq
     if (f % 8 == 0 && aligned_to(16, dh, 0) && aligned_to(8, gq, 0) && aligned_to(8, uq, 0) && m * (f / 8) <= 0xFFFFFFFFll) {
         const int64_t total = m * (f / 8);
         constexpr int U = 2;
-        k_gated_bwd<T, ACT, U><<<capped((total + kThreads * U - 1) / (kThreads * U), 8) + job.ctas, kThreads, 0, st>>>(
+        tb200_k_ffn_gated_bwd<T, ACT, U><<<capped((total + kThreads * U - 1) / (kThreads * U), 8) + job.ctas, kThreads, 0, st>>>(
             static_cast<const uint4*>(dh), static_cast<const uint2*>(gq), gs, static_cast<const uint2*>(uq), us, static_cast<uint4*>(dg),
             static_cast<uint4*>(du), static_cast<uint32_t>(total), static_cast<uint32_t>(f / 8), nblk, job);
     } else {
         const Spans sp = spans_of(m, f, Part<T>::kCols);
-        k_gated_bwd_any<T, ACT><<<capped((sp.count + 7) / 8, 8) + job.ctas, kThreads, 0, st>>>(
+        tb200_k_ffn_gated_bwd_any<T, ACT><<<capped((sp.count + 7) / 8, 8) + job.ctas, kThreads, 0, st>>>(
             static_cast<const T*>(dh), static_cast<const uint8_t*>(gq), gs, static_cast<const uint8_t*>(uq), us, static_cast<T*>(dg),
             static_cast<T*>(du), sp.count, sp.per_row, sp.width, m, f, ldg, nblk, job);
     }

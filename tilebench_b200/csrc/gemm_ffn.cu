@@ -202,7 +202,7 @@ __device__ __forceinline__ Tile tile_at(int t, int tiles_m, int tiles_n) {
 // KIND as above; T fp16 or bf16; ACT the gate (forward only); SAVE writes the codes of g and u (forward only).
 template <int KIND, typename T, int ACT, bool SAVE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs p) {
+tb200_k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs p) {
     constexpr int S = stages_of(KIND), kAreas = KIND == FK_DW ? 2 : 1;
     static_assert(S * kStageBytes + kAreas * 4 * kStagingBytes <= 6 * kStageBytes + 4 * kStagingBytes, "shared memory");
     constexpr bool kAMn = KIND == FK_DW, kBMn = KIND != FK_FWD;
@@ -589,7 +589,7 @@ __device__ __forceinline__ void save4(const float (&v)[4], uint8_t* __restrict__
 // pass at the board's power limit, this form 39.6.
 // SAVE (with FEW, tiles of 128 hidden units): a warp takes a row of the tile, which is one block of g and of u.
 template <typename T, int ACT, int SHARES, bool FEW, bool SAVE>
-__global__ void __launch_bounds__(kThreads, 1) k_ffn_mid(const __grid_constant__ MidMaps maps, const __grid_constant__ MidArgs p) {
+__global__ void __launch_bounds__(kThreads, 1) tb200_k_ffn_mid(const __grid_constant__ MidMaps maps, const __grid_constant__ MidArgs p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* staging = smem + kMidRing;
@@ -842,7 +842,7 @@ constexpr int kDxThreads = 256;
 constexpr int kDxSmemBytes = kDxRing + kBarBytes + 1024;
 
 template <typename T>
-__global__ void __launch_bounds__(kDxThreads, 1) k_dx_few(const __grid_constant__ DxFewMaps maps, const __grid_constant__ DxFewArgs p) {
+__global__ void __launch_bounds__(kDxThreads, 1) tb200_k_ffn_dx_few(const __grid_constant__ DxFewMaps maps, const __grid_constant__ DxFewArgs p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bar_full = reinterpret_cast<uint64_t*>(smem + kDxRing);
@@ -1008,7 +1008,7 @@ int map_out(CUtensorMap* m, const void* base, int64_t rows, int64_t cols) {
 
 template <int KIND, typename T, int ACT, bool SAVE>
 int launch_pair(const FfnMaps& maps, const FfnArgs& args, cudaStream_t st) {
-    auto kern = k_ffn_pair<KIND, T, ACT, SAVE>;
+    auto kern = tb200_k_ffn_pair<KIND, T, ACT, SAVE>;
     static PerDeviceInt max_pairs_tab;
     int dev = 0;
     const int rc = current_device(&dev);
@@ -1054,7 +1054,7 @@ int clusters_of(int* n) {                        // clusters of SHARES CTAs that
     if (rc != TB200_OK) return rc;
     *n = tab.v[dev].load(std::memory_order_acquire);
     if (*n == 0) {
-        auto kern = k_ffn_mid<__nv_bfloat16, TB200_ACT_SILU, SHARES, false, false>;
+        auto kern = tb200_k_ffn_mid<__nv_bfloat16, TB200_ACT_SILU, SHARES, false, false>;
         TB200_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMidSmemBytes));
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(static_cast<unsigned>(num_sms() / SHARES * SHARES), 1, 1);
@@ -1108,7 +1108,7 @@ int mid_plan(int64_t m, int64_t f, int64_t k, int least_width, MidPlan* plan) {
 
 template <typename T, int ACT, int SHARES, bool FEW, bool SAVE>
 int launch_mid(const MidMaps& maps, const MidArgs& args, cudaStream_t st) {
-    auto kern = k_ffn_mid<T, ACT, SHARES, FEW, SAVE>;
+    auto kern = tb200_k_ffn_mid<T, ACT, SHARES, FEW, SAVE>;
     static PerDeviceInt attr_set;
     const int rc = ensure_max_smem(attr_set, reinterpret_cast<const void*>(kern), kMidSmemBytes);
     if (rc != TB200_OK) return rc;
@@ -1248,7 +1248,7 @@ int dw_splits(int64_t m, int64_t f, int64_t k) {
 
 // out = the sum of `splits` arrays of n numbers that lie `stride8` pieces of 8 apart, in order; 8 numbers per thread.
 template <typename T>
-__global__ void __launch_bounds__(256) k_sum_shares(const float4* __restrict__ sums, uint4* __restrict__ out, int64_t n8, int64_t stride8, int splits) {
+__global__ void __launch_bounds__(256) tb200_k_ffn_sum_shares(const float4* __restrict__ sums, uint4* __restrict__ out, int64_t n8, int64_t stride8, int splits) {
     let_next_begin();
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n8; i += static_cast<int64_t>(gridDim.x) * 256) {
         float4 a = sums[2 * i], b = sums[2 * i + 1];
@@ -1286,7 +1286,7 @@ int dx_pair(const void* dg, const void* du, int64_t ldg, const void* wg, const v
 template <typename T>
 int dx_few(const void* dg, const void* du, int64_t ldg, const void* wg, const void* wu, void* dx, float* sums, int splits, int64_t m, int64_t f,
            int64_t k, cudaStream_t st) {
-    auto kern = k_dx_few<T>;
+    auto kern = tb200_k_ffn_dx_few<T>;
     static PerDeviceInt attr_set;
     int rc = ensure_max_smem(attr_set, reinterpret_cast<const void*>(kern), kDxSmemBytes);
     if (rc != TB200_OK) return rc;
@@ -1314,7 +1314,7 @@ int dx_few(const void* dg, const void* du, int64_t ldg, const void* wg, const vo
 template <typename T>
 int launch_sum(const float* sums, void* out, int64_t n, int64_t stride, int splits, cudaStream_t st) {
     const int64_t ctas = (n / 8 + 255) / 256, cap = static_cast<int64_t>(num_sms()) * 8;
-    k_sum_shares<T><<<static_cast<unsigned>(ctas < cap ? ctas : cap), 256, 0, st>>>(reinterpret_cast<const float4*>(sums), static_cast<uint4*>(out), n / 8,
+    tb200_k_ffn_sum_shares<T><<<static_cast<unsigned>(ctas < cap ? ctas : cap), 256, 0, st>>>(reinterpret_cast<const float4*>(sums), static_cast<uint4*>(out), n / 8,
                                                                                   stride / 8, splits);
     TB200_CUDA_TRY(cudaGetLastError());
     return TB200_OK;

@@ -20,7 +20,7 @@ import yaml
 from tilebench_b200.core.dtypes import resolve_dtype
 from tilebench_b200.core.timer import flush_l2_cache
 from tilebench_b200.data.tensors import get_generator
-from tilebench_b200.paths import operator_config
+from tilebench_b200.paths import operator_config, operator_package
 
 
 def main() -> None:
@@ -37,7 +37,7 @@ def main() -> None:
         case.setdefault(k, v[0] if isinstance(v, list) else None)
     case.update(json.loads(args.case))
     dtype = resolve_dtype(case.pop("dtype", "fp32"))
-    impl = importlib.import_module(f"tilebench_b200.benchmarks.operators.{args.operator}.impl_cuda")
+    impl = importlib.import_module(f"{operator_package(args.operator)}.impl_cuda")
     inputs = get_generator(args.operator)(**case, dtype=dtype, device="cpu", seed=args.seed)
     inputs = tuple(x.cuda() if isinstance(x, torch.Tensor) else x for x in inputs)
     for _ in range(args.warmup):

@@ -38,6 +38,10 @@ KERNEL_REGEX = {
     "gemm_fp8_blockscaled": "tb200_k_gemm_fp8",
     "matmul_int8": "tb200_k_gemm_i8",
     "matmul_fp32_fp16_fp8": "tb200_k_gemm_(f16|bf16|tf32|f8)_",
+    "act_checkpoint_fp8": "tb200_k_act_save",
+    "act_restore_fp8": "tb200_k_act_restore",
+    "ffn_gated": "tb200_k_ffn_(mid|pair)",
+    "ffn_gated_bwd": "tb200_k_(ffn|act_restore)",
 }
 
 
