@@ -3,6 +3,9 @@
 Tolerances.  A rounding is off by half a step at most: E = finfo.eps / 2 of the value (and half the spacing of the
 subnormal numbers, TINY).  A product of depth n summed in 32 bits, in steps of 16, is off by at most (n / 16 + 16) * 2^-23 of
 the sum of magnitudes (each step may truncate).  Gate functions are evaluated to 2^-19 of the value in 32 bits."""
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -13,6 +16,7 @@ from tilebench_b200.benchmarks.layers.ffn_gated import impl_cuda as ffn
 from tilebench_b200.benchmarks.layers.ffn_gated_bwd import impl_cuda as bwd
 from tilebench_b200.core.engine import run_benchmark_suite
 from tilebench_b200.data import tensors
+from tilebench_b200.paths import REPO_ROOT
 
 pytestmark = pytest.mark.gpu
 
@@ -118,6 +122,20 @@ def test_every_code_is_restored(cuda_device):
     for dtype in (torch.float32, torch.float16, torch.bfloat16):
         assert same_codes(restore.run(q, s, dtype), tensors.restore_fp8(q, s, dtype))
         assert same_codes(restore.run(q[:, :250].contiguous(), s, dtype), tensors.restore_fp8(q[:, :250], s, dtype))
+
+
+@pytest.mark.parametrize("cols", [256, 250, 131, 15])
+def test_scales_of_either_sign_and_any_size(cuda_device, cols):
+    """Scales need not be act_checkpoint_fp8's own: products beyond the type's range are held to it on either side."""
+    g = gen(cols)
+    codes = torch.arange(256, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    q = codes[torch.randint(0, 256, (64, cols), generator=g, device="cuda")]
+    blocks = (cols + 127) // 128
+    s = torch.exp2(torch.randint(-140, 128, (64, blocks), generator=g, device="cuda").float()) * (1 + torch.rand(64, blocks, generator=g, device="cuda"))
+    s[::2] *= -1
+    s[5, 0], s[6, 0], s[7, -1] = float("inf"), -float("inf"), float("nan")
+    for dtype in (torch.float32, torch.float16, torch.bfloat16):
+        assert same_codes(restore.run(q, s, dtype), tensors.restore_fp8(q, s, dtype))
 
 
 # ---- forward -----------------------------------------------------------------------------------------
@@ -283,6 +301,14 @@ def test_backward_gates(cuda_device, act):
         check_gradients(bwd.run(*args, act), args, act, torch.float16)
 
 
+@pytest.mark.parametrize("act", ACTS)
+def test_backward_of_very_large_projections(cuda_device, act):
+    """|g| up to 2^104: f'(g) is 0 or 1 there, and the squares and cubes that the formulas name leave fp32's range."""
+    args = list(backward_inputs(40, 64, 40, torch.bfloat16))
+    args[6] = torch.exp2(torch.arange(40, device="cuda") * 2.0 + 18)[:, None].contiguous()       # times codes of up to 448
+    check_gradients(bwd.run(*args, act), args, act, torch.bfloat16)
+
+
 @pytest.mark.parametrize("m,k,f", [(3000, 136, 140), (9000, 264, 24), (520, 72, 9000), (70, 2056, 5000)])
 def test_backward_in_shares(cuda_device, m, k, f):
     """Sizes whose tiles are too few, for the gradient of x or for those of the weights: the contraction is shared out."""
@@ -396,6 +422,77 @@ def test_captured_steps_replay_on_new_inputs(cuda_device, m):
         for x, wg, wu, dh, act, out in state:
             want = (*train_step(x, wg, wu, dh, act), ffn.run(x, wg, wu, act))
             assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_captured_behind_copies_fills_and_another_stream(cuda_device, m):
+    """What a call waits for may be a copy, a fill or another stream's work instead of a kernel."""
+    x, wg, wu = block_inputs(m, 136, 200, torch.bfloat16)
+    dh = normal(gen(m), m, 200, dtype=torch.bfloat16)
+    source, weight = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in (x, wg)]
+    into, w, zeros = torch.empty_like(source), torch.empty_like(weight), torch.ones_like(source)
+    side = torch.cuda.Stream()
+
+    def step():
+        into.copy_(source)
+        plain = ffn.run(into, wg, wu)
+        zeros.zero_()
+        none = ffn.run(zeros, wg, wu)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            w.copy_(weight)
+            w.mul_(2.0)
+        out = train_step(into, wg, wu, dh, "silu")
+        torch.cuda.current_stream().wait_stream(side)
+        return (plain, none, *out, ffn.run(into, w, wu), *train_step(into, w, wu, dh, "gelu"))
+
+    def expected():
+        a, b = source.clone(), weight * 2.0
+        torch.cuda.synchronize()
+        return (ffn.run(a, wg, wu), torch.zeros(m, 200, dtype=torch.bfloat16, device="cuda"), *train_step(a, wg, wu, dh, "silu"), ffn.run(a, b, wu),
+                *train_step(a, b, wu, dh, "gelu"))
+    source.copy_(x), weight.copy_(wg)
+    warm = torch.cuda.Stream()
+    warm.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(warm):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for turn in range(4):
+        source.copy_(normal(gen(turn), m, 136))
+        weight.copy_(normal(gen(50 + turn), 200, 136, scale=0.1))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, expected()))
+        assert all(torch.equal(a, b) for a, b in zip(step(), expected()))
+        torch.cuda.synchronize()
+
+
+def test_first_call_of_a_process_inside_a_capture(cuda_device):
+    """Nothing that a first call sets up is refused under capture."""
+    code = """
+import torch
+from tilebench_b200 import native
+from tilebench_b200.benchmarks.layers.ffn_gated import impl_cuda as ffn
+from tilebench_b200.benchmarks.layers.ffn_gated_bwd import impl_cuda as bwd
+native.load()
+x, wg, wu, dh = (torch.randn(s, device="cuda").half() for s in ((200, 64), (136, 64), (136, 64), (200, 136)))
+def step():
+    h, *held = ffn.run(x, wg, wu, "gelu_tanh", checkpoint=True)
+    return (h, *bwd.run(dh, wg, wu, x, None, *held, "gelu_tanh"), ffn.run(x[:3], wg, wu, "gelu_tanh"))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = step()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, step()))
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=REPO_ROOT, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 def test_calls_on_two_streams_at_once(cuda_device):

@@ -173,6 +173,8 @@ def test_refusals_of_the_forward_block(lib):
     assert call(ldx=56) == ALIGN and call(ldx=68) == ALIGN
     assert call(x=ctypes.c_void_p(8)) == ALIGN and call(wu=ctypes.c_void_p(24)) == ALIGN
     assert call(m=1 << 31) == UNSUPPORTED
+    odd = ctypes.c_void_p((1 << 20) + 1)
+    assert call(h=odd) == ALIGN and call(ckpt=(P, odd, P, P)) == ALIGN and call(ckpt=(P, P, P, odd)) == ALIGN
 
 
 def test_refusals_of_the_backward_block(lib):
@@ -190,6 +192,8 @@ def test_refusals_of_the_backward_block(lib):
     assert call(xs=None, ldx=60) == ALIGN and call(xs=None, x=ctypes.c_void_p(8)) == ALIGN and call(dx=ctypes.c_void_p(8)) == ALIGN
     assert call(ws=None) == WORKSPACE and call(nbytes=need - 1) == WORKSPACE and call(ws=ctypes.c_void_p(128)) == WORKSPACE
     assert str(need) in native.last_error()
+    odd = ctypes.c_void_p((1 << 20) + 2)
+    assert all(call(**{name: odd}) == ALIGN for name in ("gs", "us", "xs")) and call(dh=ctypes.c_void_p(1)) == ALIGN
 
 
 def test_operators_refuse_host_tensors(lib):

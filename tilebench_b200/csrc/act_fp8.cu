@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(kThreads) tb200_k_act_restore_across(const uin
 #pragma unroll
                 for (int e = 0; e < E; ++e) v[e] *= e < cut[j] ? s0[j] : e < cut2[j] ? s1[j] : s2[j];
             }
-            if (act_may_exceed(fmaxf(s0[j], fmaxf(s1[j], s2[j])), ActType<T>::kTop)) {
+            if (act_may_exceed(fmaxf(fabsf(s0[j]), fmaxf(fabsf(s1[j]), fabsf(s2[j]))), ActType<T>::kTop)) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) v[e] = act_held(v[e], ActType<T>::kTop);
             }
@@ -429,7 +429,8 @@ __device__ __forceinline__ void restore_job(const RestoreJob& job, uint32_t cta)
     }
 }
 
-// dg = dh * u * f'(g), du = dh * f(g) for 8 numbers of a lane.
+// dg = dh * u * f'(g), du = dh * f(g) for 8 numbers of a lane, in fp32 and rounded once to T: they are operands of 16 bits in the
+// products that follow (half a step, 2^-9 of the value in bf16, which the products' sums average out).
 template <typename T, int ACT>
 __device__ __forceinline__ void gated_bwd8(const uint32_t (&d)[4], const uint32_t (&cg)[2], const uint32_t (&cu)[2], float sg, float su,
                                            uint4& dg, uint4& du) {

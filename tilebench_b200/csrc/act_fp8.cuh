@@ -52,7 +52,7 @@ __device__ __forceinline__ float2 act_values2(uint32_t codes) { // two codes in 
 }
 // code * scale, held within +-top: a block whose amax is close to the type's largest value may round up beyond it,
 // which takes a scale above top / 448.
-__device__ __forceinline__ bool act_may_exceed(float s, float top) { return s > top * (1.0f / 448.0f) * 0.999f; }
+__device__ __forceinline__ bool act_may_exceed(float s, float top) { return fabsf(s) > top * (1.0f / 448.0f) * 0.999f; }
 __device__ __forceinline__ float act_held(float v, float top) {
     return fabsf(v) > top ? copysignf(top, v) : v;              // NaN stays NaN
 }
@@ -149,7 +149,8 @@ __device__ __forceinline__ float2 gate_both(float g) {
         return make_float2(g * n.x, n.x + g * kInvSqrt2Pi * n.y);
     } else if constexpr (ACT == TB200_ACT_GELU_TANH) {
         const float s = gate_logistic(2.0f * kTanhA * (g + kTanhB * g * g * g));
-        return make_float2(g * s, s + 2.0f * g * s * (1.0f - s) * kTanhA * (1.0f + 3.0f * kTanhB * g * g));
+        // s (1 - s) is 0 long before g^2 leaves fp32's range, and has to stay 0 there
+        return make_float2(g * s, s + 2.0f * kTanhA * (s * (1.0f - s)) * g * (1.0f + 3.0f * kTanhB * fminf(g * g, 1e30f)));
     } else {
         return make_float2(g <= 0.0f ? 0.0f : g, g > 0.0f ? 1.0f : 0.0f);
     }

@@ -1166,14 +1166,15 @@ int ffn_mid(const void* x, const void* wg, const void* wu, void* h, void* gq, fl
     return few ? launch_mid_act<T, true, false>(maps, args, plan.shares, act, st) : launch_mid_act<T, false, false>(maps, args, plan.shares, act, st);
 }
 
-// Hidden units per tile of the pair kernel: 128, or the multiple of 8 that leaves the least idle at the end.  A wave's time
+// Hidden units per tile of the pair kernel: 128, or the multiple of 16 (a pair's MMA is 32 columns or a multiple wide) that leaves
+// the least idle at the end.  A wave's time
 // hardly falls with its tiles' width, since a stage takes 0.27 us to issue whatever its width (measured at k = 2048: 12.1 us
 // a wave of 128-wide tiles, 9.8 of 64-wide ones): it goes as the width + 200.
 int pair_width(int64_t m, int64_t f) {
     const int64_t pairs = num_sms() / 2, tm = (m + 2 * kHalf - 1) / (2 * kHalf);
     int best = kHalf;
     int64_t least = 0;
-    for (int w = kHalf; w >= 64; w -= 8) {
+    for (int w = kHalf; w >= 64; w -= 16) {
         const int64_t cost = (tm * ((f + w - 1) / w) + pairs - 1) / pairs * (w + 200);
         if (least == 0 || cost < least) {
             least = cost;
@@ -1353,6 +1354,7 @@ int ffn_products_bwd(const void* dg, const void* du, int64_t ldg, const void* x,
     return rc;
 }
 
+bool to_elements(const void* p, uintptr_t size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
 constexpr int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 int64_t pitch_of(int64_t f) { return round_up(f, 8); }          // rows of dg and du begin on 16-byte boundaries
 
@@ -1385,6 +1387,7 @@ extern "C" int tb200_ffn_gated(const void* x, const void* wg, const void* wu, vo
     if (m == 1) ldx = k;
     if (ldx < k || ldx % 8 != 0) return fail(TB200_ERR_ALIGN, "ffn_gated: row stride of x %lld must be a multiple of 8 and at least k", (long long)ldx);
     if (!aligned16(x) || !aligned16(wg) || !aligned16(wu)) return fail(TB200_ERR_ALIGN, "ffn_gated: x, wg, wu must be 16-byte aligned");
+    if (!to_elements(h, 2) || !to_elements(gs, 4) || !to_elements(us, 4)) return fail(TB200_ERR_ALIGN, "ffn_gated: h, gs, us must be aligned to their elements");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // Up to 128 rows one CTA's accumulator holds them all and narrow tiles share the weights out evenly (1 row of 4096 ->
     // 14336: 40 us against the pair kernel's 70); beyond, two CTAs share each weight tile.  Checkpoints need whole
@@ -1423,7 +1426,8 @@ extern "C" int tb200_ffn_gated_bwd(const void* dh, const void* wg, const void* w
     if (ldx < k || ldx % 8 != 0) return fail(TB200_ERR_ALIGN, "ffn_gated_bwd: row stride of x %lld must be a multiple of 8 and at least k", (long long)ldx);
     if (!aligned16(wg) || !aligned16(wu) || !aligned16(dx) || !aligned16(dwg) || !aligned16(dwu) || (!codes && !aligned16(x)))
         return fail(TB200_ERR_ALIGN, "ffn_gated_bwd: x, wg, wu, dx, dwg, dwu must be 16-byte aligned");
-    if (reinterpret_cast<uintptr_t>(dh) & 1) return fail(TB200_ERR_ALIGN, "ffn_gated_bwd: dh must be aligned to its elements");
+    if (!to_elements(dh, 2) || !to_elements(gs, 4) || !to_elements(us, 4) || !to_elements(xs, 4))
+        return fail(TB200_ERR_ALIGN, "ffn_gated_bwd: dh, gs, us, xs must be aligned to their elements");
     if (m > (1ll << 40) / f) return fail(TB200_ERR_UNSUPPORTED, "ffn_gated_bwd: m=%lld f=%lld is too large", (long long)m, (long long)f);
     const size_t need = tb200_ffn_gated_bwd_workspace_bytes(m, f, k, codes ? 1 : 0);
     if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
