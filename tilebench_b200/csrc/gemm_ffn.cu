@@ -1,10 +1,10 @@
 // Matrix products of the gated feed-forward block, forward and backward, on tcgen05 (kind::f16, fp32 accumulation).
 //
 //   forward   g = x Wg^T, u = x Wu^T, h = f(g) * u         one kernel; the codes of g and u in 8 bits on request
-//   dx        dx = dg Wg + du Wu                            one kernel, one accumulator over both products
-//   dw        dWg = dg^T x, dWu = du^T x                    one launch over the tiles of both results
+//   backward  dx = dg Wg + du Wu                            one accumulator over both products
+//             dWg = dg^T x, dWu = du^T x                    one kernel over the tiles of all three results
 //
-// All three are one CTA-pair kernel (cta_group::2): 256 x 256 accumulators in tensor memory, two of them, so that the
+// Both are one CTA-pair kernel (cta_group::2): 256 x 256 accumulators in tensor memory, two of them, so that the
 // epilogue of a tile runs under the main loop of the next.  Each CTA of a pair loads 128 rows of A and one 128-wide
 // half of B per 64-deep stage.  What differs is where the operands lie:
 //   forward   A = x and B = W with the contraction contiguous (K-major).  The leader's half of B is 128 rows of Wg,
@@ -19,15 +19,17 @@
 
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 namespace tb200 {
 namespace {
 
 constexpr int kBK = 64;                          // contraction per stage: 128 bytes of 16-bit elements
 constexpr int kHalf = 128;                       // rows of A, and columns of B, that one CTA loads
-// Stages in shared memory: dw, whose tiles have the fewest stages, gives one up for a second staging area.  (128 rows at
-// 4096 x 14336: dw 58 -> 45 us; dx would go from 55 to 60.)
-constexpr int stages_of(int kind) { return kind == 2 ? 5 : 6; }
+// Stages in shared memory, and copies of the result under way per quarter: two places of 4 KB leave room for 6 stages.  Where dx has a
+// kernel of its own, dw's tiles have a single stage: 4 are enough there, and four places keep more copies under way.
+constexpr int stages_of(int kind) { return kind == 2 ? 4 : 6; }
+constexpr int places_of(int kind) { return kind == 2 ? 4 : 2; }
 constexpr int kOperandBytes = kHalf * 128;
 constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kAtomBytes = kBK * 128;            // MN-major: one box of 64 contraction rows x 64 columns
@@ -40,21 +42,26 @@ constexpr int kTmemCols = 512;
 constexpr int kThreads = 128 + 32 * kEpiWarps;   // TMA, MMA, two idle warps, epilogue
 constexpr int kGroupM = 8;                       // tiles are walked in bands of 8 x 256 rows, so that B's tiles stay in L2
 
-enum FfnKind : int { FK_FWD = 0, FK_DX = 1, FK_DW = 2 };
+enum FfnKind : int { FK_FWD = 0, FK_BWD = 1, FK_DW = 2 };       // FK_DW: the backward pass without dx
 
-struct FfnMaps {
-    CUtensorMap a[2];                            // forward: x, -      dx: dg, du     dw: dg, du
-    CUtensorMap b[2];                            // forward: Wg, Wu    dx: Wg, Wu     dw: x, -
-    CUtensorMap out[2];                          // forward: -         dx: dx, -      dw: dWg, dWu
+template <int KIND> struct FfnMaps;
+template <> struct FfnMaps<FK_FWD> { CUtensorMap a[1], b[2]; };                  // x; Wg, Wu
+struct FfnBwdMaps {
+    CUtensorMap a[2], b[2];                      // of dx: dg, du; Wg, Wu
+    CUtensorMap at[2], x;                        // of dw: dg, du; x
+    CUtensorMap out[3];                          // dx, dWg, dWu
 };
+template <> struct FfnMaps<FK_BWD> : FfnBwdMaps {};
+template <> struct FfnMaps<FK_DW> : FfnBwdMaps {};
 struct FfnArgs {
-    void* out[2];                                // forward: h, -      dx: dx, -      dw: dWg, dWu
-    float* sums;                                 // in shares: partial sums, dx [splits, rows, cols], dw [splits, 2, rows, cols]
-    int rows, cols, depth;                       // of one result, and of one product's contraction
-    int splits;                                  // dx, dw: shares of the contraction
+    void* out[3];                                // forward: h; backward: dx, dWg, dWu
+    int m, f, k;
     int w;                                       // forward: hidden units per tile (128 with checkpoints)
-    uint8_t* codes[2];                           // forward with checkpoints: codes of g and u, [rows, cols]
-    float* scales[2];                            // and their scales, [rows, ceil(cols / 128)]
+    uint8_t* codes[2];                           // forward with checkpoints: codes of g and u, [m, f]
+    float* scales[2];                            // and their scales, [m, ceil(f / 128)]
+    float* sums[2];                              // backward, in shares: partial sums of dx [shares, m, k], of dw [shares, 2, f, k]
+    int shares[2];                               // of the contraction of dx, and of dw; 0: not in this launch
+    int early;                                   // backward, see item_at
 };
 
 __device__ __forceinline__ uint64_t desc_mn(uint32_t smem_addr) {       // MN-major, 128-byte swizzle
@@ -189,8 +196,8 @@ __device__ __forceinline__ void gated32(uint32_t (&g)[32], const uint32_t (&u)[3
     for (int i = 0; i < 32; ++i) g[i] = __float_as_uint(gate_value<ACT>(__uint_as_float(g[i])) * __uint_as_float(u[i]));
 }
 
-// First step of share i of n.
-__device__ __forceinline__ int share_at(int steps, int i, int n) { return static_cast<int>(static_cast<int64_t>(steps) * i / n); }
+// First step of share i of n.  (At most 2^25 steps and 16 shares.)
+__device__ __forceinline__ int share_at(int steps, int i, int n) { return n == 1 ? i * steps : static_cast<int>(static_cast<uint32_t>(steps) * i / n); }
 
 struct Tile { int m, n; };
 __device__ __forceinline__ Tile tile_at(int t, int tiles_m, int tiles_n) {
@@ -199,20 +206,71 @@ __device__ __forceinline__ Tile tile_at(int t, int tiles_m, int tiles_n) {
     return {first + r % size, r / size};
 }
 
+// A pair's i-th piece of work: a share of a tile.  Backward: the items of dx, which are long, go round the pairs first.  Those
+// of dw follow: where the last round of dx leaves pairs without an item, they take `early` ones of dw in its place; then all take
+// turns, in an order that begins with them.  (dx and dw in launches of their own, each with a last round that is partly idle: 500
+// rows of 4096 x 14336 211 us, 4096 rows 1368; in one: 198 and 1329.)
+struct Item {
+    bool any, dw;
+    int sel, share;                              // dw: 0 dWg, 1 dWu
+    Tile tile;                                   // of the result
+    int st0, steps;                              // stages of the contraction; dx: dg Wg, then du Wu
+};
+__host__ __device__ __forceinline__ constexpr int ceil_to(int v, int n) { return (v + n - 1) / n; }
+template <int KIND>
+__device__ __forceinline__ Item item_at(const FfnArgs& p, int pair, int npairs, int i) {
+    Item it = {};
+    if constexpr (KIND == FK_FWD) {
+        const int tiles_m = ceil_to(p.m, 2 * kHalf), tiles_n = ceil_to(p.f, p.w), t = pair + i * npairs;
+        it.any = t < tiles_m * tiles_n;
+        it.tile = tile_at(t, tiles_m, tiles_n);
+        it.steps = ceil_to(p.k, kBK);
+    } else {
+        const int tiles_n = ceil_to(p.k, 2 * kHalf), tiles_x = ceil_to(p.m, 2 * kHalf) * tiles_n, tm = ceil_to(p.f, 2 * kHalf), tiles_w = 2 * tm * tiles_n;
+        const int items_x = KIND == FK_BWD ? tiles_x * p.shares[0] : 0, rounds = items_x / npairs, last = items_x - rounds * npairs;   // pairs 0..last-1 have one more
+        const bool more = pair < last;
+        const int mine = rounds + more;
+        if (KIND == FK_BWD && i < mine) {
+            const int t = pair + i * npairs, n = p.shares[0], steps = 2 * ceil_to(p.f, kBK);
+            it.any = true;
+            it.share = n == 1 ? 0 : t / tiles_x;
+            it.tile = tile_at(t - it.share * tiles_x, ceil_to(p.m, 2 * kHalf), tiles_n);
+            it.st0 = share_at(steps, it.share, n);
+            it.steps = share_at(steps, it.share + 1, n) - it.st0;
+        } else {
+            const int j = i - mine, n = p.shares[1], steps = ceil_to(p.m, kBK);
+            int t;
+            if (KIND == FK_DW) t = pair + i * npairs;
+            else if (more) t = p.early * (npairs - last) + j * npairs + npairs - last + pair;
+            else if (j < p.early) t = j * (npairs - last) + pair - last;
+            else t = p.early * (npairs - last) + (j - p.early) * npairs + pair - last;
+            it.any = t < tiles_w * n;
+            if (!it.any) return it;
+            it.dw = true;
+            it.share = n == 1 ? 0 : t / tiles_w;
+            it.tile = tile_at(t - it.share * tiles_w, 2 * tm, tiles_n);          // the tiles of dWg, then those of dWu
+            it.sel = it.tile.m >= tm;
+            it.tile.m -= it.sel * tm;
+            it.st0 = share_at(steps, it.share, n);
+            it.steps = share_at(steps, it.share + 1, n) - it.st0;
+        }
+    }
+    return it;
+}
+
 // KIND as above; T fp16 or bf16; ACT the gate (forward only); SAVE writes the codes of g and u (forward only).
 template <int KIND, typename T, int ACT, bool SAVE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-tb200_k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnArgs p) {
-    constexpr int S = stages_of(KIND), kAreas = KIND == FK_DW ? 2 : 1;
-    static_assert(S * kStageBytes + kAreas * 4 * kStagingBytes <= 6 * kStageBytes + 4 * kStagingBytes, "shared memory");
-    constexpr bool kAMn = KIND == FK_DW, kBMn = KIND != FK_FWD;
+tb200_k_ffn_pair(const __grid_constant__ FfnMaps<KIND> maps, const __grid_constant__ FfnArgs p) {
+    constexpr int S = stages_of(KIND), kPlaces = places_of(KIND), kStaging = kPlaces * (kStagingBytes / 2);
+    static_assert(S * kStageBytes + 4 * kStaging <= 6 * kStageBytes + 4 * kStagingBytes, "shared memory");
     const int tile_cols = KIND == FK_FWD ? p.w : 2 * kHalf;     // columns of the result that a tile covers
     const int b_bytes = KIND == FK_FWD ? p.w * 128 : kOperandBytes;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* staging = smem + S * kStageBytes;
-    uint32_t* amax = reinterpret_cast<uint32_t*>(staging + kAreas * 4 * kStagingBytes);      // [quarter][g, u][row], bits of non-negative numbers
-    uint64_t* bar_full = reinterpret_cast<uint64_t*>(staging + kAreas * 4 * kStagingBytes + kAmaxBytes);
+    uint32_t* amax = reinterpret_cast<uint32_t*>(staging + 4 * kStaging);      // [quarter][g, u][row], bits of non-negative numbers
+    uint64_t* bar_full = reinterpret_cast<uint64_t*>(staging + 4 * kStaging + kAmaxBytes);
     uint64_t* bar_empty = bar_full + S;
     uint64_t* bar_afull = bar_empty + S;          // [2] accumulator complete
     uint64_t* bar_aempty = bar_afull + 2;         // [2] accumulator read (the epilogue warps of both CTAs)
@@ -223,13 +281,6 @@ tb200_k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ F
     const int rank = static_cast<int>(cluster_ctarank());       // 0 = leader
     const int pair = blockIdx.x >> 1;
     const int npairs = gridDim.x >> 1;
-    const int KB = (p.depth + kBK - 1) / kBK;                   // stages of one product
-    const int steps = KIND == FK_DX ? 2 * KB : KB;              // of a tile; dx: dg Wg, then du Wu
-    const int tm1 = (p.rows + 2 * kHalf - 1) / (2 * kHalf);
-    const int tiles_m = KIND == FK_DW ? 2 * tm1 : tm1;          // dw: the tiles of dWg, then those of dWu
-    const int tiles_n = (p.cols + tile_cols - 1) / tile_cols;
-    const int tiles = tiles_m * tiles_n;
-    const int items = KIND != FK_FWD ? tiles * p.splits : tiles; // dx, dw: item i is share i / tiles of tile i % tiles
 
     let_next_begin();
     if (SAVE && threadIdx.x < kAmaxBytes / 4) amax[threadIdx.x] = 0;
@@ -243,12 +294,8 @@ tb200_k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ F
             mbar_init(&bar_aempty[b], 2 * kEpiWarps);
         }
         mbar_fence_init();
-        tma_prefetch_desc(&maps.a[0]);
-        tma_prefetch_desc(&maps.b[0]);
-        if (KIND != FK_FWD) tma_prefetch_desc(&maps.a[1]);
-        if (KIND != FK_DW) tma_prefetch_desc(&maps.b[1]);
-        if (KIND != FK_FWD) tma_prefetch_desc(&maps.out[0]);
-        if (KIND == FK_DW) tma_prefetch_desc(&maps.out[1]);
+        const CUtensorMap* all = reinterpret_cast<const CUtensorMap*>(&maps);
+        for (int i = 0; i < static_cast<int>(sizeof(maps) / sizeof(CUtensorMap)); ++i) tma_prefetch_desc(all + i);
     }
     if (warp == 1) {
         tmem_alloc_pair(tmem_slot, kTmemCols);
@@ -266,33 +313,37 @@ tb200_k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ F
         if (lane == 0) {
             uint32_t s = 0, ph = 1;
             bool ok = true;
-            for (int t = pair; t < items && ok; t += npairs) {
-                const int share = KIND != FK_FWD ? t / tiles : 0;
-                const Tile tc = tile_at(t - share * tiles, tiles_m, tiles_n);
-                const int sel = KIND == FK_DW && tc.m >= tm1 ? 1 : 0;
-                const int a_row = (tc.m - sel * tm1) * 2 * kHalf + rank * kHalf;
-                const int b_col = KIND == FK_FWD ? tc.n * tile_cols : tc.n * 2 * kHalf + rank * kHalf;
-                const int st0 = KIND != FK_FWD ? share_at(steps, share, p.splits) : 0, st1 = KIND != FK_FWD ? share_at(steps, share + 1, p.splits) : steps;
-                for (int st = st0; st < st1; ++st) {
-                    if (!mbar_wait(&bar_empty[s], ph, ST_WAIT_SMEM_EMPTY, st)) { ok = false; break; }
-                    uint8_t* stage = smem + s * kStageBytes;
-                    if (rank == 0) mbar_expect_tx(&bar_full[s], 2 * (kOperandBytes + b_bytes));  // both CTAs' bytes
-                    const int prod = KIND == FK_DX && st >= KB ? 1 : 0;
-                    const int k0 = (st - prod * KB) * kBK;
-                    if constexpr (kAMn) {
-                        tma_load_2d_pair(stage, &maps.a[sel], &bar_full[s], a_row, k0);
-                        tma_load_2d_pair(stage + kAtomBytes, &maps.a[sel], &bar_full[s], a_row + 64, k0);
-                    } else {
-                        tma_load_2d_pair(stage, &maps.a[prod], &bar_full[s], k0, a_row);
+            const int KB = ceil_to(p.f, kBK);                    // stages of one of dx's products
+            for (int i = 0; ok; ++i) {
+                const Item it = item_at<KIND>(p, pair, npairs, i);
+                if (!it.any) break;
+                const int a_row = it.tile.m * 2 * kHalf + rank * kHalf;
+                const int b_col = KIND == FK_FWD ? it.tile.n * tile_cols : it.tile.n * 2 * kHalf + rank * kHalf;
+                // one loop per kind of item: the loops are what paces the pair, and carry no choice
+                auto load = [&](auto dw) {
+                    for (int st = it.st0; st < it.st0 + it.steps; ++st) {
+                        if (!mbar_wait(&bar_empty[s], ph, ST_WAIT_SMEM_EMPTY, st)) { ok = false; break; }
+                        uint8_t* stage = smem + s * kStageBytes;
+                        if (rank == 0) mbar_expect_tx(&bar_full[s], 2 * (kOperandBytes + b_bytes));  // both CTAs' bytes
+                        if constexpr (KIND == FK_FWD) {
+                            tma_load_2d_pair(stage, &maps.a[0], &bar_full[s], st * kBK, a_row);
+                            tma_load_2d_pair(stage + kOperandBytes, &maps.b[rank], &bar_full[s], st * kBK, b_col);
+                        } else if constexpr (dw) {
+                            tma_load_2d_pair(stage, &maps.at[it.sel], &bar_full[s], a_row, st * kBK);
+                            tma_load_2d_pair(stage + kAtomBytes, &maps.at[it.sel], &bar_full[s], a_row + 64, st * kBK);
+                            tma_load_2d_pair(stage + kOperandBytes, &maps.x, &bar_full[s], b_col, st * kBK);
+                            tma_load_2d_pair(stage + kOperandBytes + kAtomBytes, &maps.x, &bar_full[s], b_col + 64, st * kBK);
+                        } else {
+                            const int prod = st >= KB ? 1 : 0, k0 = (st - prod * KB) * kBK;
+                            tma_load_2d_pair(stage, &maps.a[prod], &bar_full[s], k0, a_row);
+                            tma_load_2d_pair(stage + kOperandBytes, &maps.b[prod], &bar_full[s], b_col, k0);
+                            tma_load_2d_pair(stage + kOperandBytes + kAtomBytes, &maps.b[prod], &bar_full[s], b_col + 64, k0);
+                        }
+                        if (++s == S) { s = 0; ph ^= 1; }
                     }
-                    if constexpr (kBMn) {
-                        tma_load_2d_pair(stage + kOperandBytes, &maps.b[prod], &bar_full[s], b_col, k0);
-                        tma_load_2d_pair(stage + kOperandBytes + kAtomBytes, &maps.b[prod], &bar_full[s], b_col + 64, k0);
-                    } else {
-                        tma_load_2d_pair(stage + kOperandBytes, &maps.b[rank], &bar_full[s], k0, b_col);
-                    }
-                    if (++s == S) { s = 0; ph ^= 1; }
-                }
+                };
+                if (KIND == FK_DW || (KIND == FK_BWD && it.dw)) load(std::true_type());
+                else if (KIND != FK_DW) load(std::false_type());
             }
             if (!ok) {
                 // copies in flight land within microseconds; a bounded pause before the CTA may exit
@@ -303,56 +354,62 @@ tb200_k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ F
     } else if (warp == 1 && rank == 0) {
         // ---------------- MMA issuer (leader only; the whole warp walks the loop, lane 0 issues by predication) ------
         constexpr uint32_t fmt = sizeof(T) == 2 && ActType<T>::kTop > 1e6f ? 1u : 0u;            // 1 = bf16, 0 = fp16
-        const uint32_t idesc = umma_idesc(fmt, fmt, 2 * kHalf, KIND == FK_FWD ? 2 * tile_cols : 2 * kHalf) | (kAMn ? 1u << 15 : 0u) | (kBMn ? 1u << 16 : 0u);
+        const uint32_t idesc0 = umma_idesc(fmt, fmt, 2 * kHalf, KIND == FK_FWD ? 2 * tile_cols : 2 * kHalf) | (KIND != FK_FWD ? 1u << 16 : 0u);
         constexpr uint32_t kStageDesc = kStageBytes >> 4;
         // 16 of the 64 contraction elements per MMA: 32 bytes along a K-major row, 16 rows of an MN-major box
-        constexpr uint64_t a_step = kAMn ? 16 * 128 / 16 : 2, b_step = kBMn ? 16 * 128 / 16 : 2;
+        constexpr uint64_t kAlongRow = 2, kDownBox = 16 * 128 / 16, b_step = KIND != FK_FWD ? kDownBox : kAlongRow;
         const bool leader = lane == 0;
-        const uint64_t a_desc0 = kAMn ? desc_mn(smem_u32(smem)) : umma_desc_sw128(smem_u32(smem));
-        const uint64_t b_desc0 = kBMn ? desc_mn(smem_u32(smem) + kOperandBytes) : umma_desc_sw128(smem_u32(smem) + kOperandBytes);
+        const uint64_t b_desc0 = KIND != FK_FWD ? desc_mn(smem_u32(smem) + kOperandBytes) : umma_desc_sw128(smem_u32(smem) + kOperandBytes);
         uint32_t s = 0, ph = 0, cnt = 0;
         bool ready = false;
         bool ok = true;
-        for (int t = pair; t < items && ok; t += npairs, ++cnt) {
+        for (; ok; ++cnt) {
+            const Item it = item_at<KIND>(p, pair, npairs, cnt);
+            if (!it.any) break;
             const uint32_t acc = cnt & 1;
-            if (!mbar_wait(&bar_aempty[acc], ((cnt >> 1) & 1) ^ 1, ST_WAIT_TMEM_EMPTY, t)) { ok = false; break; }
+            if (!mbar_wait(&bar_aempty[acc], ((cnt >> 1) & 1) ^ 1, ST_WAIT_TMEM_EMPTY, cnt)) { ok = false; break; }
             tc_fence_after();
             const uint32_t d_tmem = tmem_base + acc * 256;
-            const int share = KIND != FK_FWD ? t / tiles : 0;
-            const int n = KIND != FK_FWD ? share_at(steps, share + 1, p.splits) - share_at(steps, share, p.splits) : steps;
-            for (int st = 0; st < n; ++st) {
-                if (!ready && !mbar_wait(&bar_full[s], ph, ST_WAIT_SMEM_FULL, st)) { ok = false; break; }
-                tc_fence_after();
-                const uint64_t a_desc = a_desc0 + s * kStageDesc;
-                const uint64_t b_desc = b_desc0 + s * kStageDesc;
-                uint64_t* const freed = &bar_empty[s];
-                if (++s == static_cast<uint32_t>(S)) { s = 0; ph ^= 1; }
-                mma_pair_if(leader, d_tmem, a_desc, b_desc, idesc, st > 0 ? 1u : 0u);
-                ready = mbar_test_wait(&bar_full[s], ph);
+            auto multiply = [&](auto dw) {
+                const uint32_t idesc = idesc0 | (dw ? 1u << 15 : 0u);
+                const uint64_t a_desc0 = dw ? desc_mn(smem_u32(smem)) : umma_desc_sw128(smem_u32(smem));
+                constexpr uint64_t a_step = dw ? kDownBox : kAlongRow;
+                for (int st = 0; st < it.steps; ++st) {
+                    if (!ready && !mbar_wait(&bar_full[s], ph, ST_WAIT_SMEM_FULL, st)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint64_t a_desc = a_desc0 + s * kStageDesc;
+                    const uint64_t b_desc = b_desc0 + s * kStageDesc;
+                    uint64_t* const freed = &bar_empty[s];
+                    if (++s == static_cast<uint32_t>(S)) { s = 0; ph ^= 1; }
+                    mma_pair_if(leader, d_tmem, a_desc, b_desc, idesc, st > 0 ? 1u : 0u);
+                    ready = mbar_test_wait(&bar_full[s], ph);
 #pragma unroll
-                for (int k = 1; k < 4; ++k) mma_pair_if(leader, d_tmem, a_desc + k * a_step, b_desc + k * b_step, idesc, 1u);
-                if (leader) tc_commit_pair(freed, 0x3);
-            }
+                    for (int k = 1; k < 4; ++k) mma_pair_if(leader, d_tmem, a_desc + k * a_step, b_desc + k * b_step, idesc, 1u);
+                    if (leader) tc_commit_pair(freed, 0x3);
+                }
+            };
+            if (KIND == FK_DW || (KIND == FK_BWD && it.dw)) multiply(std::true_type());
+            else if (KIND != FK_DW) multiply(std::false_type());
             if (ok && leader) tc_commit_pair(&bar_afull[acc], 0x3);
         }
     } else if (warp >= 4) {
         // ---------------- epilogue (both CTAs; each owns 128 rows of the tile, each warp 32 rows of a quarter of the columns) ----
         const int quarter = (warp - 4) & 3, part = (warp - 4) >> 2, r8 = 8 * part;
-        uint8_t* buf = staging + quarter * kStagingBytes;
+        uint8_t* buf = staging + quarter * kStaging;
         const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
         uint32_t cnt = 0;
         bool ok = true;
-        for (int t = pair; t < items; t += npairs, ++cnt) {
-            const int share = KIND != FK_FWD ? t / tiles : 0;
-            const Tile tc = tile_at(t - share * tiles, tiles_m, tiles_n);
-            const int sel = KIND == FK_DW && tc.m >= tm1 ? 1 : 0;
+        for (;; ++cnt) {
+            const Item it = item_at<KIND>(p, pair, npairs, cnt);
+            if (!it.any) break;
             const uint32_t acc = cnt & 1;
-            const int row0 = (tc.m - sel * tm1) * 2 * kHalf + rank * kHalf + quarter * 32;        // the quarter's first row
-            const int rows = p.rows - row0;                                                       // valid rows (may be <= 0)
-            const int col0 = tc.n * tile_cols, cols = p.cols - col0;
+            const int all_rows = KIND != FK_FWD && it.dw ? p.f : p.m, all_cols = KIND == FK_FWD ? p.f : p.k;
+            const int row0 = it.tile.m * 2 * kHalf + rank * kHalf + quarter * 32;                 // the quarter's first row
+            const int rows = all_rows - row0;                                                     // valid rows (may be <= 0)
+            const int col0 = it.tile.n * tile_cols, cols = all_cols - col0;
             const uint32_t t_acc = t_lane + acc * 256;
             // a wait that gave up ends the waiting, not the walk: the warps meet at barriers below
-            ok = ok && mbar_wait(&bar_afull[acc], (cnt >> 1) & 1, ST_WAIT_TMEM_FULL, t);
+            ok = ok && mbar_wait(&bar_afull[acc], (cnt >> 1) & 1, ST_WAIT_TMEM_FULL, cnt);
             tc_fence_after();
             auto release = [&] {                                                                  // the warp has read its part of the accumulator
                 tc_fence_before();
@@ -388,7 +445,7 @@ tb200_k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ F
                     ag = __uint_as_float(row_amax[0]);
                     au = __uint_as_float(row_amax[32]);
                 }
-                flush<T, 16>(buf, 0, static_cast<T*>(p.out[0]) + static_cast<int64_t>(row0) * p.cols + col0, p.cols, r8, rows, min(cols, tile_cols), lane);
+                flush<T, 16>(buf, 0, static_cast<T*>(p.out[0]) + static_cast<int64_t>(row0) * p.f + col0, p.f, r8, rows, min(cols, tile_cols), lane);
                 quarter_sync(quarter);
                 if constexpr (SAVE) {
                     tmem_ld32(t_g, g);
@@ -412,19 +469,21 @@ tb200_k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ F
                         au = __uint_as_float(row_amax[32]);
                     }
                     const float2 sg = act_scale(ag), su = act_scale(au);
-                    const int64_t nblk = (p.cols + kHalf - 1) / kHalf;
-                    if (part < 2 && lane < rows) p.scales[part][(row0 + lane) * nblk + tc.n] = part == 0 ? sg.x : su.x;
+                    const int64_t nblk = ceil_to(p.f, kHalf);
+                    if (part < 2 && lane < rows) p.scales[part][(row0 + lane) * nblk + it.tile.n] = part == 0 ? sg.x : su.x;
                     stage_codes32(buf, lane, 2 * part, g, sg.y, infinite);
                     stage_codes32(buf, lane, 8 + 2 * part, u, su.y, infinite);
                     quarter_sync(quarter);
                     if (part == 0) row_amax[0] = row_amax[32] = 0;                                // all have read it, none adds before the next barrier
-                    const int64_t to = static_cast<int64_t>(row0) * p.cols + col0;
-                    flush<uint8_t, 8>(buf, 0, p.codes[0] + to, p.cols, r8, rows, cols, lane);
-                    flush<uint8_t, 8>(buf, 8, p.codes[1] + to, p.cols, r8, rows, cols, lane);
+                    const int64_t to = static_cast<int64_t>(row0) * p.f + col0;
+                    flush<uint8_t, 8>(buf, 0, p.codes[0] + to, p.f, r8, rows, cols, lane);
+                    flush<uint8_t, 8>(buf, 8, p.codes[1] + to, p.f, r8, rows, cols, lane);
                     quarter_sync(quarter);
                 }
-            } else if (p.splits > 1) {                           // partial sums in 32 bits, 64 columns at a time
-                float* dst = p.sums + (static_cast<int64_t>(KIND == FK_DW ? 2 * share + sel : share) * p.rows + row0) * p.cols + col0;
+            } else if (p.shares[it.dw] > 1) {                    // partial sums in 32 bits, 64 columns at a time
+                float* dst = p.sums[it.dw] + (static_cast<int64_t>(it.dw ? 2 * it.share + it.sel : it.share) * all_rows + row0) * p.k + col0;
+                if (part == 0 && lane == 0) tma_store_wait_read<0>();     // the item before may have been stored by TMA
+                quarter_sync(quarter);
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     uint32_t v[16];
@@ -434,49 +493,53 @@ tb200_k_ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ F
 #pragma unroll
                     for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(staged(buf, lane, 4 * part + q)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
                     quarter_sync(quarter);
-                    flush<float, 16>(buf, 0, dst + c * 64, p.cols, r8, rows, cols - c * 64, lane);
+                    flush<float, 16>(buf, 0, dst + c * 64, p.k, r8, rows, cols - c * 64, lane);
                     quarter_sync(quarter);
                 }
             } else {
-                // By TMA, which leaves out what lies beyond the result: 32 rows x 64 columns a copy, in the 128-byte swizzle.  One half of
-                // the columns per staging area; the quarter's first lane, which issues the copies, waits for the area's last ones.
+                // By TMA, which leaves out what lies beyond the result: 32 rows x 64 columns a copy, in the 128-byte swizzle, from the
+                // places of the quarter's staging area in turn; its first lane, which issues the copies, waits for the place's last one.
                 // Rows that do not begin on 32-byte boundaries are written by the warps, 256 bytes of a row at once: copies of 128
                 // would leave twice as many sectors half written (6 rows of 7192 -> 28637: 221 us where this takes 182).
-                uint32_t v[2][32];
-                tmem_ld32(t_acc + part * 32, v[0]);
-                tmem_ld32(t_acc + kHalf + part * 32, v[1]);
-                tmem_wait_ld();
-                release();
-                const bool issuer = part == 0 && lane == 0, by_tma = p.cols % 16 == 0;
+                const int which = it.dw ? 1 + it.sel : 0;
+                if (p.k % 16 == 0) {
+                    const bool issuer = part == 0 && lane == 0;
+                    uint32_t v[4][16];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    if (!by_tma) {
+                    for (int c = 0; c < 4; ++c) tmem_ld16(t_acc + c * 64 + part * 16, v[c]);
+                    tmem_wait_ld();
+                    release();
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint8_t* area = buf + c % kPlaces * (kStagingBytes / 2);
+                        if (issuer) tma_store_wait_read<kPlaces - 1>();   // all but the other places'
+                        quarter_sync(quarter);
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) w[e] = ActType<T>::pack(__uint_as_float(v[c][8 * q + 2 * e]), __uint_as_float(v[c][8 * q + 2 * e + 1]));
+                            *reinterpret_cast<uint4*>(area + lane * 128 + (((2 * part + q) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                        fence_async_smem();
+                        quarter_sync(quarter);
+                        if (issuer) {
+                            if (rows > 0 && c * 64 < cols) tma_store_2d(&maps.out[which], area, col0 + c * 64, row0);
+                            tma_store_commit();
+                        }
+                    }
+                } else {
+                    uint32_t v[2][32];
+                    tmem_ld32(t_acc + part * 32, v[0]);
+                    tmem_ld32(t_acc + kHalf + part * 32, v[1]);
+                    tmem_wait_ld();
+                    release();
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
                         stage32<T>(buf, lane, 4 * part, v[c]);
                         quarter_sync(quarter);
-                        flush<T, 16>(buf, 0, static_cast<T*>(p.out[sel]) + static_cast<int64_t>(row0) * p.cols + col0 + c * kHalf, p.cols, r8, rows, cols - c * kHalf, lane);
+                        flush<T, 16>(buf, 0, static_cast<T*>(p.out[which]) + static_cast<int64_t>(row0) * p.k + col0 + c * kHalf, p.k, r8, rows, cols - c * kHalf, lane);
                         quarter_sync(quarter);
-                        continue;
-                    }
-                    uint8_t* area = staging + (c % kAreas * 4 + quarter) * kStagingBytes;
-                    if (issuer) tma_store_wait_read<kAreas - 1>();        // all but the other area's
-                    quarter_sync(quarter);
-                    uint8_t* box = area + (part >> 1) * (32 * 128) + lane * 128;
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = ActType<T>::pack(__uint_as_float(v[c][8 * q + 2 * e]), __uint_as_float(v[c][8 * q + 2 * e + 1]));
-                        *reinterpret_cast<uint4*>(box + ((((part & 1) * 4 + q) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                    fence_async_smem();
-                    quarter_sync(quarter);
-                    if (issuer) {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int x = col0 + c * kHalf + h * 64;
-                            if (rows > 0 && x < p.cols) tma_store_2d(&maps.out[sel], area + h * (32 * 128), x, row0);
-                        }
-                        tma_store_commit();
                     }
                 }
             }
@@ -1006,8 +1069,9 @@ int map_out(CUtensorMap* m, const void* base, int64_t rows, int64_t cols) {
     return encode_tmap_2d(m, base, tmap_type<T>(), 2, rows, cols, cols * 2, 32, 64, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// Pairs that the device holds at once.
 template <int KIND, typename T, int ACT, bool SAVE>
-int launch_pair(const FfnMaps& maps, const FfnArgs& args, cudaStream_t st) {
+int pairs_of(int* n) {
     auto kern = tb200_k_ffn_pair<KIND, T, ACT, SAVE>;
     static PerDeviceInt max_pairs_tab;
     int dev = 0;
@@ -1020,26 +1084,32 @@ int launch_pair(const FfnMaps& maps, const FfnArgs& args, cudaStream_t st) {
         cfg.gridDim = dim3(static_cast<unsigned>(num_sms() & ~1), 1, 1);
         cfg.blockDim = dim3(kThreads, 1, 1);
         cfg.dynamicSmemBytes = kSmemBytes;
-        int clusters = 0;
-        TB200_CUDA_TRY(cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg));
-        if (clusters < 1) return fail(TB200_ERR_UNSUPPORTED, "ffn_gated: no CTA pair fits on this device");
-        max_pairs = clusters;
-        max_pairs_tab.v[dev].store(clusters, std::memory_order_release);
+        TB200_CUDA_TRY(cudaOccupancyMaxActiveClusters(&max_pairs, kern, &cfg));
+        if (max_pairs < 1) return fail(TB200_ERR_UNSUPPORTED, "ffn_gated: no CTA pair fits on this device");
+        max_pairs_tab.v[dev].store(max_pairs, std::memory_order_release);
     }
-    const int64_t tile_cols = KIND == FK_FWD ? args.w : 2 * kHalf;
-    const int64_t tiles = (KIND == FK_DW ? 2 : 1) * (KIND == FK_FWD ? 1 : args.splits) * ((args.rows + 2 * kHalf - 1) / (2 * kHalf)) * ((args.cols + tile_cols - 1) / tile_cols);
-    if (tiles > 0x7fffffffll / kGroupM) return fail(TB200_ERR_UNSUPPORTED, "ffn_gated: too many tiles");
-    const int pairs = static_cast<int>(tiles < max_pairs ? tiles : max_pairs);
-    return launch_over_previous(kern, 2 * pairs, kThreads, kSmemBytes, 1, st, maps, args);
+    *n = max_pairs;
+    return TB200_OK;
+}
+
+template <int KIND, typename T, int ACT, bool SAVE>
+int launch_pair(const FfnMaps<KIND>& maps, const FfnArgs& args, int64_t items, cudaStream_t st) {
+    int max_pairs = 0;
+    const int rc = pairs_of<KIND, T, ACT, SAVE>(&max_pairs);
+    if (rc != TB200_OK) return rc;
+    if (items > 0x7fffffffll / kGroupM) return fail(TB200_ERR_UNSUPPORTED, "ffn_gated: too many tiles");
+    const int pairs = static_cast<int>(items < max_pairs ? items : max_pairs);
+    return launch_over_previous(tb200_k_ffn_pair<KIND, T, ACT, SAVE>, 2 * pairs, kThreads, kSmemBytes, 1, st, maps, args);
 }
 
 template <typename T, bool SAVE>
-int launch_fwd(const FfnMaps& maps, const FfnArgs& args, int act, cudaStream_t st) {
+int launch_fwd(const FfnMaps<FK_FWD>& maps, const FfnArgs& args, int act, cudaStream_t st) {
+    const int64_t items = static_cast<int64_t>(ceil_to(args.m, 2 * kHalf)) * ceil_to(args.f, args.w);
     switch (act) {
-        case TB200_ACT_SILU: return launch_pair<FK_FWD, T, TB200_ACT_SILU, SAVE>(maps, args, st);
-        case TB200_ACT_GELU: return launch_pair<FK_FWD, T, TB200_ACT_GELU, SAVE>(maps, args, st);
-        case TB200_ACT_GELU_TANH: return launch_pair<FK_FWD, T, TB200_ACT_GELU_TANH, SAVE>(maps, args, st);
-        default: return launch_pair<FK_FWD, T, TB200_ACT_RELU, SAVE>(maps, args, st);
+        case TB200_ACT_SILU: return launch_pair<FK_FWD, T, TB200_ACT_SILU, SAVE>(maps, args, items, st);
+        case TB200_ACT_GELU: return launch_pair<FK_FWD, T, TB200_ACT_GELU, SAVE>(maps, args, items, st);
+        case TB200_ACT_GELU_TANH: return launch_pair<FK_FWD, T, TB200_ACT_GELU_TANH, SAVE>(maps, args, items, st);
+        default: return launch_pair<FK_FWD, T, TB200_ACT_RELU, SAVE>(maps, args, items, st);
     }
 }
 
@@ -1188,7 +1258,7 @@ template <typename T>
 int ffn_forward(const void* x, const void* wg, const void* wu, void* h, void* gq, float* gs, void* uq, float* us, int64_t m, int64_t f,
                 int64_t k, int64_t ldx, int act, cudaStream_t st) {
     const int w = gq ? kHalf : pair_width(m, f);
-    FfnMaps maps;
+    FfnMaps<FK_FWD> maps;
     memset(&maps, 0, sizeof(maps));
     int rc = map_k<T>(&maps.a[0], x, m, k, ldx);
     if (rc == TB200_OK) rc = map_k<T>(&maps.b[0], wg, f, k, k, w);
@@ -1197,9 +1267,9 @@ int ffn_forward(const void* x, const void* wg, const void* wu, void* h, void* gq
     FfnArgs args = {};
     args.w = w;
     args.out[0] = h;
-    args.rows = static_cast<int>(m);
-    args.cols = static_cast<int>(f);
-    args.depth = static_cast<int>(k);
+    args.m = static_cast<int>(m);
+    args.f = static_cast<int>(f);
+    args.k = static_cast<int>(k);
     args.codes[0] = static_cast<uint8_t*>(gq);
     args.codes[1] = static_cast<uint8_t*>(uq);
     args.scales[0] = gs;
@@ -1207,21 +1277,22 @@ int ffn_forward(const void* x, const void* wg, const void* wu, void* h, void* gq
     return gq ? launch_fwd<T, true>(maps, args, act, st) : launch_fwd<T, false>(maps, args, act, st);
 }
 
-// Shares of dx's contraction: the number with the least time by a model in stages of 0.27 us.  A tile costs some 6 beside its
-// own; shares are written and added up in 32 bits, at 5 TB/s, by a kernel that costs some 10 more.  For few rows a
-// stage takes longer where it waits for the weights: 0.38 us at 148 CTAs.
-int dx_splits(int64_t m, int64_t f, int64_t k) {
-    const bool few = m <= kFewRows;
-    const int64_t places = few ? num_sms() : num_sms() / 2;
-    const int64_t tiles = few ? (k + kHalf - 1) / kHalf : ((m + 2 * kHalf - 1) / (2 * kHalf)) * ((k + 2 * kHalf - 1) / (2 * kHalf));
-    const int64_t steps = 2 * ((f + kBK - 1) / kBK);
+// ---- the backward pass's shares ----
+// A model of time in stages of 0.27 us.  An item of dx costs some 6 beside its own stages, one of dw 3; shares are written and
+// added up in 32 bits, at 5 TB/s, by a kernel that costs some 10 more.
+constexpr int kMostShares = 16, kLeastStages = 8;               // of a share
+constexpr double kStagesPerByte = 1.0 / (5e6 * 0.27);
+
+// dx for few rows, by a kernel of its own; a stage takes longer where it waits for the weights: 0.38 us at 148 CTAs.
+int dx_few_shares(int64_t m, int64_t f, int64_t k) {
+    const int64_t places = num_sms(), tiles = (k + kHalf - 1) / kHalf, steps = 2 * ((f + kBK - 1) / kBK);
     int best = 1;
     double least = 0.0;
-    for (int s = 1; s <= 16 && steps >= 8 * (s - 1); ++s) {
+    for (int s = 1; s <= kMostShares && steps >= kLeastStages * (s - 1); ++s) {
         const int64_t at_once = tiles * s < places ? tiles * s : places;
-        const double stage = few ? fmax(1.0, 1.4 * static_cast<double>(at_once) / static_cast<double>(places)) : 1.0;
+        const double stage = fmax(1.0, 1.4 * static_cast<double>(at_once) / static_cast<double>(places));
         const double cost = static_cast<double>((tiles * s + places - 1) / places) * (static_cast<double>((steps + s - 1) / s) * stage + 6.0) +
-                            (s > 1 ? 10.0 + static_cast<double>(m) * k * 8.0 * s / (5e6 * 0.27) : 0.0);
+                            (s > 1 ? 10.0 + static_cast<double>(m) * k * 8.0 * s * kStagesPerByte : 0.0);
         if (s == 1 || cost < least) {
             least = cost;
             best = s;
@@ -1230,58 +1301,78 @@ int dx_splits(int64_t m, int64_t f, int64_t k) {
     return best;
 }
 
-// The same for dw, whose tiles are too few where the model is small and the tokens are many.
-int dw_splits(int64_t m, int64_t f, int64_t k) {
-    const int64_t pairs = num_sms() / 2, tiles = 2 * ((f + 2 * kHalf - 1) / (2 * kHalf)) * ((k + 2 * kHalf - 1) / (2 * kHalf));
-    const int64_t steps = (m + kBK - 1) / kBK;
-    int best = 1;
+// Whether dx goes to that kernel: few rows, and weights beyond what L2 (126 MB) holds of both.  Smaller ones gain more from sharing
+// a launch with dw than from the kernel's narrower tiles: 50 rows of 512 x 28000 38 us against 52, 33 of 2048 x 5632 32 against 35,
+// but 6 of 7192 x 28637 444 against 381.
+bool dx_alone(int64_t m, int64_t f, int64_t k) { return m <= kFewRows && f * k > (24ll << 20); }
+
+struct BwdPlan { int dx, dw, early; bool apart; }; // shares; early: see item_at; dx and dw in launches of their own
+// Time of nx items of dx and nw of dw (cx and cw each) on the pairs, with the better number of early ones.
+double bwd_time(int64_t nx, double cx, int64_t nw, double cw, int64_t pairs, int* early) {
+    const int64_t rounds = nx / pairs, last = nx % pairs, idle = pairs - last;
     double least = 0.0;
-    for (int s = 1; s <= 16 && steps >= 8 * (s - 1); ++s) {
-        const double cost = static_cast<double>((tiles * s + pairs - 1) / pairs) * static_cast<double>((steps + s - 1) / s + 2) +
-                            (s > 1 ? 20.0 + static_cast<double>(f) * k * 16.0 * s / (5e6 * 0.27) : 0.0);
-        if (s == 1 || cost < least) {
-            least = cost;
-            best = s;
+    for (int64_t more = 0; more < 2; ++more) {
+        const int64_t most = nw / idle, e = last == 0 ? 0 : static_cast<int64_t>(cx / cw) + more < most ? static_cast<int64_t>(cx / cw) + more : most;
+        const int64_t rest = nw - e * idle, left = rest % pairs;
+        const double busy = static_cast<double>(rounds + (last > 0)) * cx + static_cast<double>(rest / pairs + (left > idle)) * cw;
+        const double other = static_cast<double>(rounds) * cx + static_cast<double>(e + rest / pairs + (left > 0)) * cw;
+        if (more == 0 || fmax(busy, other) < least) {
+            least = fmax(busy, other);
+            *early = static_cast<int>(e);
         }
     }
+    return least;
+}
+BwdPlan bwd_plan(int64_t m, int64_t f, int64_t k) {
+    const bool few = dx_alone(m, f, k);
+    const int64_t pairs = num_sms() / 2, tn = (k + 2 * kHalf - 1) / (2 * kHalf);
+    const int64_t tx = few ? 0 : (m + 2 * kHalf - 1) / (2 * kHalf) * tn, tw = 2 * ((f + 2 * kHalf - 1) / (2 * kHalf)) * tn;
+    const int64_t x_steps = 2 * ((f + kBK - 1) / kBK), w_steps = (m + kBK - 1) / kBK;
+    BwdPlan best = {1, 1, 0, false};
+    double least = 0.0;
+    // more shares than it takes to give every pair two items are not looked at
+    for (int sx = 1; sx <= kMostShares && x_steps >= kLeastStages * (sx - 1) && tx * (sx - 1) < 2 * pairs; ++sx) {
+        for (int sw = 1; sw <= kMostShares && w_steps >= kLeastStages * (sw - 1) && tw * (sw - 1) < 2 * pairs; ++sw) {
+            int early = 0;
+            const double cx = static_cast<double>((x_steps + sx - 1) / sx) + 6.0, cw = static_cast<double>((w_steps + sw - 1) / sw) + 3.0;
+            double cost = bwd_time(tx * sx, cx, tw * sw, cw, pairs, &early);
+            // Items of both kinds at once read more of memory, in no common order: where one launch saves less than 5 % there are two
+            // (16000 rows of 2048 x 8192: 1589 us against 1608; 4096 of 4096 x 14336, where it saves 9 %: 1368 against 1329).
+            const double two = static_cast<double>((tx * sx + pairs - 1) / pairs) * cx + static_cast<double>((tw * sw + pairs - 1) / pairs) * cw + 10.0;
+            const bool apart = cost > 0.95 * two;
+            if (sx > 1 || sw > 1) cost += 10.0;
+            if (sx > 1) cost += static_cast<double>(m) * k * 8.0 * sx * kStagesPerByte;
+            if (sw > 1) cost += static_cast<double>(f) * k * 16.0 * sw * kStagesPerByte;
+            if (least == 0.0 || cost < least) {
+                least = cost;
+                best = {sx, sw, early, apart};
+            }
+        }
+        if (few) break;
+    }
+    if (few) best.dx = dx_few_shares(m, f, k);
     return best;
 }
 
-// out = the sum of `splits` arrays of n numbers that lie `stride8` pieces of 8 apart, in order; 8 numbers per thread.
+// out = the sum of `splits` arrays of n8 pieces of 8 numbers that lie `stride8` pieces apart, in order; 8 numbers per thread.  One
+// result per row of the grid.
+struct SumJob { const float4* sums; uint4* out; int64_t n8, stride8; int splits; };
+struct SumJobs { SumJob job[3]; };
 template <typename T>
-__global__ void __launch_bounds__(256) tb200_k_ffn_sum_shares(const float4* __restrict__ sums, uint4* __restrict__ out, int64_t n8, int64_t stride8, int splits) {
+__global__ void __launch_bounds__(256) tb200_k_ffn_sum_shares(const __grid_constant__ SumJobs jobs) {
     let_next_begin();
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n8; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const SumJob& q = jobs.job[blockIdx.y];
+    const float4* const __restrict__ sums = q.sums;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < q.n8; i += static_cast<int64_t>(gridDim.x) * 256) {
         float4 a = sums[2 * i], b = sums[2 * i + 1];
 #pragma unroll 4
-        for (int s = 1; s < splits; ++s) {
-            const float4 c = sums[2 * (s * stride8 + i)], d = sums[2 * (s * stride8 + i) + 1];
+        for (int s = 1; s < q.splits; ++s) {
+            const float4 c = sums[2 * (s * q.stride8 + i)], d = sums[2 * (s * q.stride8 + i) + 1];
             a.x += c.x; a.y += c.y; a.z += c.z; a.w += c.w;
             b.x += d.x; b.y += d.y; b.z += d.z; b.w += d.w;
         }
-        out[i] = make_uint4(ActType<T>::pack(a.x, a.y), ActType<T>::pack(a.z, a.w), ActType<T>::pack(b.x, b.y), ActType<T>::pack(b.z, b.w));
+        q.out[i] = make_uint4(ActType<T>::pack(a.x, a.y), ActType<T>::pack(a.z, a.w), ActType<T>::pack(b.x, b.y), ActType<T>::pack(b.z, b.w));
     }
-}
-
-template <typename T>
-int dx_pair(const void* dg, const void* du, int64_t ldg, const void* wg, const void* wu, void* dx, float* sums, int splits, int64_t m, int64_t f,
-            int64_t k, cudaStream_t st) {
-    FfnMaps maps;
-    memset(&maps, 0, sizeof(maps));
-    int rc = map_k<T>(&maps.a[0], dg, m, f, ldg);
-    if (rc == TB200_OK) rc = map_k<T>(&maps.a[1], du, m, f, ldg);
-    if (rc == TB200_OK) rc = map_mn<T>(&maps.b[0], wg, f, k, k);
-    if (rc == TB200_OK) rc = map_mn<T>(&maps.b[1], wu, f, k, k);
-    if (rc == TB200_OK) rc = map_out<T>(&maps.out[0], dx, m, k);
-    if (rc != TB200_OK) return rc;
-    FfnArgs args = {};
-    args.rows = static_cast<int>(m);
-    args.cols = static_cast<int>(k);
-    args.depth = static_cast<int>(f);
-    args.splits = splits;
-    args.sums = sums;
-    args.out[0] = dx;
-    return launch_pair<FK_DX, T, 0, false>(maps, args, st);
 }
 
 template <typename T>
@@ -1312,46 +1403,70 @@ int dx_few(const void* dg, const void* du, int64_t ldg, const void* wg, const vo
     return launch_over_previous(kern, static_cast<int>(items < num_sms() ? items : num_sms()), kDxThreads, kDxSmemBytes, 1, st, maps, args);
 }
 
-template <typename T>
-int launch_sum(const float* sums, void* out, int64_t n, int64_t stride, int splits, cudaStream_t st) {
-    const int64_t ctas = (n / 8 + 255) / 256, cap = static_cast<int64_t>(num_sms()) * 8;
-    tb200_k_ffn_sum_shares<T><<<static_cast<unsigned>(ctas < cap ? ctas : cap), 256, 0, st>>>(reinterpret_cast<const float4*>(sums), static_cast<uint4*>(out), n / 8,
-                                                                                  stride / 8, splits);
-    TB200_CUDA_TRY(cudaGetLastError());
-    return TB200_OK;
-}
-
-// dg, du: [m, ldg]; x: [m, k]; sums: room for dx_splits() arrays of [m, k] and, later, for dw_splits() of [2, f, k], where those are
-// more than 1
+// dg, du: [m, ldg]; x: [m, k]; sums: room for the plan's arrays of dx [m, k], then for those of dw [2, f, k], where they are more than 1
 template <typename T>
 int ffn_products_bwd(const void* dg, const void* du, int64_t ldg, const void* x, int64_t ldx, const void* wg, const void* wu, void* dx, void* dwg,
                      void* dwu, float* sums, int64_t m, int64_t f, int64_t k, cudaStream_t st) {
-    int splits = dx_splits(m, f, k);
-    int rc = m <= kFewRows ? dx_few<T>(dg, du, ldg, wg, wu, dx, sums, splits, m, f, k, st) : dx_pair<T>(dg, du, ldg, wg, wu, dx, sums, splits, m, f, k, st);
-    if (rc == TB200_OK && splits > 1) rc = launch_sum<T>(sums, dx, m * k, m * k, splits, st);
+    const BwdPlan plan = bwd_plan(m, f, k);
+    const bool few = dx_alone(m, f, k);
+    float* const sums_w = sums + (plan.dx > 1 ? plan.dx * m * k : 0);
+    int rc = few ? dx_few<T>(dg, du, ldg, wg, wu, dx, sums, plan.dx, m, f, k, st) : TB200_OK;
+    FfnBwdMaps maps;
+    memset(&maps, 0, sizeof(maps));
+    const void* const grads[2] = {dg, du};
+    const void* const weights[2] = {wg, wu};
+    for (int i = 0; i < 2; ++i) {
+        if (rc == TB200_OK) rc = map_k<T>(&maps.a[i], grads[i], m, f, ldg);
+        if (rc == TB200_OK) rc = map_mn<T>(&maps.b[i], weights[i], f, k, k);
+        if (rc == TB200_OK) rc = map_mn<T>(&maps.at[i], grads[i], m, f, ldg);
+    }
+    if (rc == TB200_OK) rc = map_mn<T>(&maps.x, x, m, k, ldx);
+    if (rc == TB200_OK) rc = map_out<T>(&maps.out[0], dx, m, k);
+    if (rc == TB200_OK) rc = map_out<T>(&maps.out[1], dwg, f, k);
+    if (rc == TB200_OK) rc = map_out<T>(&maps.out[2], dwu, f, k);
+    if (rc != TB200_OK) return rc;
+    FfnArgs args = {};
+    args.out[0] = dx;
+    args.out[1] = dwg;
+    args.out[2] = dwu;
+    args.m = static_cast<int>(m);
+    args.f = static_cast<int>(f);
+    args.k = static_cast<int>(k);
+    args.sums[0] = sums;
+    args.sums[1] = sums_w;
+    args.shares[0] = plan.dx;
+    args.shares[1] = plan.dw;
+    args.early = plan.early;
+    const int64_t tn = (k + 2 * kHalf - 1) / (2 * kHalf);
+    const int64_t items_x = plan.dx * ((m + 2 * kHalf - 1) / (2 * kHalf)) * tn, items_w = plan.dw * 2 * ((f + 2 * kHalf - 1) / (2 * kHalf)) * tn;
+    if (few) {
+        rc = launch_pair<FK_DW, T, 0, false>({maps}, args, items_w, st);
+    } else if (plan.apart) {
+        FfnArgs first = args;
+        first.shares[1] = first.early = args.shares[0] = args.early = 0;
+        rc = launch_pair<FK_BWD, T, 0, false>({maps}, first, items_x, st);
+        if (rc == TB200_OK) rc = launch_pair<FK_BWD, T, 0, false>({maps}, args, items_w, st);
+    } else {
+        rc = launch_pair<FK_BWD, T, 0, false>({maps}, args, items_x + items_w, st);
+    }
     if (rc != TB200_OK) return rc;
 
-    FfnMaps maps;
-    memset(&maps, 0, sizeof(maps));
-    rc = map_mn<T>(&maps.a[0], dg, m, f, ldg);
-    if (rc == TB200_OK) rc = map_mn<T>(&maps.a[1], du, m, f, ldg);
-    if (rc == TB200_OK) rc = map_mn<T>(&maps.b[0], x, m, k, ldx);
-    if (rc == TB200_OK) rc = map_out<T>(&maps.out[0], dwg, f, k);
-    if (rc == TB200_OK) rc = map_out<T>(&maps.out[1], dwu, f, k);
-    if (rc != TB200_OK) return rc;
-    splits = dw_splits(m, f, k);
-    FfnArgs args = {};
-    args.out[0] = dwg;
-    args.out[1] = dwu;
-    args.sums = sums;
-    args.rows = static_cast<int>(f);
-    args.cols = static_cast<int>(k);
-    args.depth = static_cast<int>(m);
-    args.splits = splits;
-    rc = launch_pair<FK_DW, T, 0, false>(maps, args, st);
-    if (rc == TB200_OK && splits > 1) rc = launch_sum<T>(sums, dwg, f * k, 2 * f * k, splits, st);
-    if (rc == TB200_OK && splits > 1) rc = launch_sum<T>(sums + f * k, dwu, f * k, 2 * f * k, splits, st);
-    return rc;
+    SumJobs jobs = {};
+    int n = 0;
+    int64_t most = 0;
+    auto add = [&](const float* from, void* to, int64_t count, int64_t stride, int splits) {
+        jobs.job[n++] = {reinterpret_cast<const float4*>(from), static_cast<uint4*>(to), count / 8, stride / 8, splits};
+        most = count > most ? count : most;
+    };
+    if (plan.dx > 1) add(sums, dx, m * k, m * k, plan.dx);
+    if (plan.dw > 1) add(sums_w, dwg, f * k, 2 * f * k, plan.dw);
+    if (plan.dw > 1) add(sums_w + f * k, dwu, f * k, 2 * f * k, plan.dw);
+    if (n > 0) {
+        const int64_t ctas = (most / 8 + 255) / 256, cap = static_cast<int64_t>(num_sms()) * 8;
+        tb200_k_ffn_sum_shares<T><<<dim3(static_cast<unsigned>(ctas < cap ? ctas : cap), static_cast<unsigned>(n)), 256, 0, st>>>(jobs);
+        TB200_CUDA_TRY(cudaGetLastError());
+    }
+    return TB200_OK;
 }
 
 bool to_elements(const void* p, uintptr_t size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
@@ -1401,10 +1516,9 @@ extern "C" int tb200_ffn_gated(const void* x, const void* wg, const void* wu, vo
 
 extern "C" size_t tb200_ffn_gated_bwd_workspace_bytes(int64_t m, int64_t f, int64_t k, int x_codes) {
     if (m <= 0 || f <= 0 || k <= 0) return 0;
-    const int64_t dx = dx_splits(m, f, k), dw = dw_splits(m, f, k);
-    const int64_t dx_sums = dx > 1 ? dx * m * k * 4 : 0, dw_sums = dw > 1 ? dw * 2 * f * k * 4 : 0;
+    const BwdPlan plan = bwd_plan(m, f, k);
     return static_cast<size_t>(2 * round_up(m * pitch_of(f) * 2, 256) + (x_codes ? round_up(m * k * 2, 256) : 0) +
-                               (dx_sums > dw_sums ? dx_sums : dw_sums));
+                               (plan.dx > 1 ? plan.dx * m * k * 4 : 0) + (plan.dw > 1 ? plan.dw * 2 * f * k * 4 : 0));
 }
 
 extern "C" int tb200_ffn_gated_bwd(const void* dh, const void* wg, const void* wu, const void* x, const float* xs, const void* gq,
