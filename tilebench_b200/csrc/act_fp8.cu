@@ -455,7 +455,7 @@ __device__ __forceinline__ void gated_bwd8(const uint32_t (&d)[4], const uint32_
 template <typename T, int ACT, int U>
 __global__ void __launch_bounds__(kThreads) tb200_k_ffn_gated_bwd(const uint4* __restrict__ dh, const uint2* __restrict__ gq, const float* __restrict__ gs,
                                                         const uint2* __restrict__ uq, const float* __restrict__ us, uint4* __restrict__ dg,
-                                                        uint4* __restrict__ du, uint32_t total, uint32_t per_row, uint32_t nblk,
+                                                        uint4* __restrict__ du, uint32_t total, uint32_t per_row, uint32_t out_row, uint32_t nblk,
                                                         const RestoreJob job) {
     let_next_begin();
     const uint32_t ctas = gridDim.x - job.ctas, step = ctas * kThreads;
@@ -464,11 +464,13 @@ __global__ void __launch_bounds__(kThreads) tb200_k_ffn_gated_bwd(const uint4* _
         uint4 d[U];
         uint2 cg[U], cu[U];
         float sg[U], su[U];
+        uint32_t to[U];                                          // place in dg and du, whose rows lie out_row pieces apart
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             const uint64_t i = i0 + j * step;
             if (i < total) {
-                const uint32_t row = static_cast<uint32_t>(i) / per_row, blk = row * nblk + (static_cast<uint32_t>(i) - row * per_row) / 16;
+                const uint32_t row = static_cast<uint32_t>(i) / per_row, col = static_cast<uint32_t>(i) - row * per_row, blk = row * nblk + col / 16;
+                to[j] = row * out_row + col;
                 d[j] = __ldcs(dh + i);
                 cg[j] = __ldcs(gq + i);
                 cu[j] = __ldcs(uq + i);
@@ -483,8 +485,8 @@ __global__ void __launch_bounds__(kThreads) tb200_k_ffn_gated_bwd(const uint4* _
                 const uint32_t dw[4] = {d[j].x, d[j].y, d[j].z, d[j].w}, gw[2] = {cg[j].x, cg[j].y}, uw[2] = {cu[j].x, cu[j].y};
                 uint4 a, b;
                 gated_bwd8<T, ACT>(dw, gw, uw, sg[j], su[j], a, b);
-                dg[i] = a;
-                du[i] = b;
+                dg[to[j]] = a;
+                du[to[j]] = b;
             }
         }
     }
@@ -604,12 +606,12 @@ template <typename T, int ACT>
 int launch_gated(const void* dh, const void* gq, const float* gs, const void* uq, const float* us, void* dg, void* du, int64_t m, int64_t f,
                  int64_t ldg, const RestoreJob& job, cudaStream_t st) {
     const uint32_t nblk = static_cast<uint32_t>((f + kActBlock - 1) / kActBlock);
-    if (f % 8 == 0 && aligned_to(16, dh, 0) && aligned_to(8, gq, 0) && aligned_to(8, uq, 0) && m * (f / 8) <= 0xFFFFFFFFll) {
+    if (f % 8 == 0 && aligned_to(16, dh, 0) && aligned_to(8, gq, 0) && aligned_to(8, uq, 0) && m * (ldg / 8) <= 0xFFFFFFFFll) {
         const int64_t total = m * (f / 8);
         constexpr int U = 2;
         tb200_k_ffn_gated_bwd<T, ACT, U><<<capped((total + kThreads * U - 1) / (kThreads * U), 8) + job.ctas, kThreads, 0, st>>>(
             static_cast<const uint4*>(dh), static_cast<const uint2*>(gq), gs, static_cast<const uint2*>(uq), us, static_cast<uint4*>(dg),
-            static_cast<uint4*>(du), static_cast<uint32_t>(total), static_cast<uint32_t>(f / 8), nblk, job);
+            static_cast<uint4*>(du), static_cast<uint32_t>(total), static_cast<uint32_t>(f / 8), static_cast<uint32_t>(ldg / 8), nblk, job);
     } else {
         const Spans sp = spans_of(m, f, Part<T>::kCols);
         tb200_k_ffn_gated_bwd_any<T, ACT><<<capped((sp.count + 7) / 8, 8) + job.ctas, kThreads, 0, st>>>(
