@@ -179,8 +179,8 @@ def test_refusals_of_the_forward_block(lib):
 
 def test_refusals_of_the_backward_block(lib):
     need = lib.tb200_ffn_gated_bwd_workspace_bytes(4, 17, 64, 1)
-    assert need == 2 * 256 + 512                            # dg, du: 4 x 24 x 2 bytes rounded up; x: 4 x 64 x 2
-    assert lib.tb200_ffn_gated_bwd_workspace_bytes(4, 17, 64, 0) == 2 * 256
+    assert need == 2 * 512 + 512                            # dg, du: 4 rows of 128 bytes; x: the same
+    assert lib.tb200_ffn_gated_bwd_workspace_bytes(4, 17, 64, 0) == 2 * 512
     assert lib.tb200_ffn_gated_bwd_workspace_bytes(0, 17, 64, 1) == 0
 
     def call(dh=P, wg=P, wu=P, x=P, xs=P, gq=P, gs=P, uq=P, us=P, dx=P, dwg=P, dwu=P, m=4, f=17, k=64, ldx=64, act=0,

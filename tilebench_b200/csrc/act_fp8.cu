@@ -8,11 +8,18 @@ namespace {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ void load32(const void* p, uint32_t (&r)[8]) {        // 32 bytes, read once
+__device__ __forceinline__ void load_once(const void* p, uint32_t (&r)[8]) {     // 32 bytes, read once
     asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "l"(p));
 }
-__device__ __forceinline__ void store32(void* p, const uint32_t (&r)[8]) {
+// 32 bytes on a boundary of 16, the second half only where it is there; the halves share a sector, which L1 keeps between them
+__device__ __forceinline__ void load_halves(const void* p, bool both, uint32_t (&r)[8]) {
+    const uint4 a = __ldg(static_cast<const uint4*>(p)), b = both ? __ldg(static_cast<const uint4*>(p) + 1) : make_uint4(0, 0, 0, 0);
+    r[0] = a.x; r[1] = a.y; r[2] = a.z; r[3] = a.w;
+    r[4] = b.x; r[5] = b.y; r[6] = b.z; r[7] = b.w;
+}
+__device__ __forceinline__ void store_piece(void* p, const uint32_t (&r)[4]) { *static_cast<uint4*>(p) = make_uint4(r[0], r[1], r[2], r[3]); }
+__device__ __forceinline__ void store_piece(void* p, const uint32_t (&r)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
                  "r"(r[6]), "r"(r[7]) : "memory");
 }
@@ -82,12 +89,33 @@ __device__ __forceinline__ void decode(const uint32_t (&codes)[E / 4], float s, 
     }
 }
 
-// ---- rows on 32-byte boundaries: one 32-byte piece of x per lane and access ------------------------------------
+// N words of codes, on a boundary of their size
+template <int N>
+__device__ __forceinline__ void load_codes(const uint8_t* p, uint32_t (&c)[N]) {
+    if constexpr (N == 4) {
+        const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
+        c[0] = v.x; c[1] = v.y; c[2] = v.z; c[3] = v.w;
+    } else if constexpr (N == 2) {
+        const uint2 v = __ldcs(reinterpret_cast<const uint2*>(p));
+        c[0] = v.x; c[1] = v.y;
+    } else {
+        c[0] = __ldcs(reinterpret_cast<const uint32_t*>(p));
+    }
+}
+template <int N>
+__device__ __forceinline__ void store_codes(uint8_t* p, const uint32_t (&c)[N]) {
+    if constexpr (N == 4) *reinterpret_cast<uint4*>(p) = make_uint4(c[0], c[1], c[2], c[3]);
+    else if constexpr (N == 2) *reinterpret_cast<uint2*>(p) = make_uint2(c[0], c[1]);
+    else *reinterpret_cast<uint32_t*>(p) = c[0];
+}
 
-// Saving.  E numbers (32 bytes) per lane, 128 / E lanes per block, U pieces in flight.  per_row: pieces per row; a row
-// ends inside a block where cols is not a multiple of 128 (lanes past it hold zeros).  FLAT: rows are whole blocks and
-// adjacent, so the piece's number is its place.
-template <typename T, int U, bool FLAT>
+// ---- rows on 32- or 16-byte boundaries: one such piece of x per lane and access ---------------------------------
+
+// Saving.  E numbers (32 bytes) per lane, 128 / E lanes per block, U pieces in flight; a row ends inside a block where cols is not a
+// multiple of 128 (lanes past it hold zeros).  FLAT: rows are whole blocks and adjacent, so the piece's number is its place.
+// HALVES: rows begin on 16-byte boundaries and may end with half a piece.  (Pieces of 16 bytes instead, at twice the shuffles per
+// number: 33390 x 5464 in 163 us where this takes 0.)
+template <typename T, int U, bool FLAT, bool HALVES>
 __global__ void __launch_bounds__(kThreads) tb200_k_act_save(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales,
                                                    uint32_t blocks, uint32_t nblk, int64_t cols, int64_t ldx) {
     let_next_begin();
@@ -96,20 +124,28 @@ __global__ void __launch_bounds__(kThreads) tb200_k_act_save(const T* __restrict
     for (uint64_t i0 = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x; i0 - (threadIdx.x & 31) < total; i0 += U * step) {
         uint32_t w[U][8];
         int64_t at[U];                                           // place of the lane's codes, -1 where it has none
+        bool both[U];                                            // whether the piece is whole
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             const uint64_t i = i0 + j * step;
             at[j] = -1;
+            both[j] = true;
             if (i < total) {
                 if constexpr (FLAT) {
                     at[j] = static_cast<int64_t>(i) * E;
-                    load32(x + at[j], w[j]);
+                    load_once(x + at[j], w[j]);
                 } else {
                     const uint32_t blk = static_cast<uint32_t>(i / kLanes), row = blk / nblk;
                     const int64_t col = static_cast<int64_t>(blk - row * nblk) * kActBlock + (i % kLanes) * E;
                     if (col < cols) {
                         at[j] = static_cast<int64_t>(row) * cols + col;
-                        load32(x + static_cast<int64_t>(row) * ldx + col, w[j]);
+                        const T* from = x + static_cast<int64_t>(row) * ldx + col;
+                        if constexpr (HALVES) {
+                            both[j] = col + E <= cols;
+                            load_halves(from, both[j], w[j]);
+                        } else {
+                            load_once(from, w[j]);
+                        }
                     }
                 }
             }
@@ -126,58 +162,65 @@ __global__ void __launch_bounds__(kThreads) tb200_k_act_save(const T* __restrict
             numbers<T, 8>(w[j], v);
             const float s = encode<E>(v, c);
             if (at[j] >= 0) {
-                if constexpr (E == 16) *reinterpret_cast<uint4*>(q + at[j]) = make_uint4(c[0], c[1], c[2], c[3]);
-                else *reinterpret_cast<uint2*>(q + at[j]) = make_uint2(c[0], c[1]);
+                if constexpr (HALVES) {
+                    constexpr int H = E / 8;
+                    uint32_t c0[H], c1[H];
+#pragma unroll
+                    for (int e = 0; e < H; ++e) {
+                        c0[e] = c[e];
+                        c1[e] = c[H + e];
+                    }
+                    store_codes<H>(q + at[j], c0);
+                    if (both[j]) store_codes<H>(q + at[j] + E / 2, c1);
+                } else {
+                    store_codes<E / 4>(q + at[j], c);
+                }
                 if (i % kLanes == 0) scales[i / kLanes] = s;
             }
         }
     }
 }
 
-// Restoring: E codes per lane make one 32-byte piece.
-template <typename T, int U, bool FLAT>
+// Restoring: E codes per lane make one piece.  Rows of the result lie ldo apart.
+template <typename T, int E, int U, bool FLAT>
 __global__ void __launch_bounds__(kThreads) tb200_k_act_restore(const uint8_t* __restrict__ q, const float* __restrict__ scales, T* __restrict__ out,
-                                                      uint32_t blocks, uint32_t nblk, int64_t cols) {
+                                                      uint32_t blocks, uint32_t nblk, int64_t cols, int64_t ldo) {
     let_next_begin();
-    constexpr int E = 32 / sizeof(T), kLanes = kActBlock / E;
+    constexpr int kLanes = kActBlock / E, kWords = E * sizeof(T) / 4;
     const uint64_t total = static_cast<uint64_t>(blocks) * kLanes, step = static_cast<uint64_t>(gridDim.x) * kThreads;
     for (uint64_t i0 = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x; i0 < total; i0 += U * step) {
         uint32_t c[U][E / 4];
         float s[U];
-        int64_t at[U];
+        int64_t to[U];                                           // place of the lane's numbers, -1 where it has none
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             const uint64_t i = i0 + j * step;
-            at[j] = -1;
+            to[j] = -1;
             if (i < total) {
                 const uint32_t blk = static_cast<uint32_t>(i / kLanes);
+                int64_t from = static_cast<int64_t>(i) * E;
                 if constexpr (FLAT) {
-                    at[j] = static_cast<int64_t>(i) * E;
+                    to[j] = from;
                 } else {
                     const uint32_t row = blk / nblk;
                     const int64_t col = static_cast<int64_t>(blk - row * nblk) * kActBlock + (i % kLanes) * E;
-                    if (col < cols) at[j] = static_cast<int64_t>(row) * cols + col;
+                    from = static_cast<int64_t>(row) * cols + col;
+                    if (col < cols) to[j] = static_cast<int64_t>(row) * ldo + col;
                 }
-                if (at[j] >= 0) {
-                    if constexpr (E == 16) {
-                        const uint4 p = __ldcs(reinterpret_cast<const uint4*>(q + at[j]));
-                        c[j][0] = p.x; c[j][1] = p.y; c[j][2] = p.z; c[j][3] = p.w;
-                    } else {
-                        const uint2 p = __ldcs(reinterpret_cast<const uint2*>(q + at[j]));
-                        c[j][0] = p.x; c[j][1] = p.y;
-                    }
+                if (to[j] >= 0) {
+                    load_codes<E / 4>(q + from, c[j]);
                     s[j] = __ldg(scales + blk);
                 }
             }
         }
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            if (at[j] >= 0) {
+            if (to[j] >= 0) {
                 float v[E];
-                uint32_t w[8];
+                uint32_t w[kWords];
                 decode<E>(c[j], s[j], ActType<T>::kTop, v);
-                words<T, 8>(v, w);
-                store32(out + at[j], w);
+                words<T, kWords>(v, w);
+                store_piece(out + to[j], w);
             }
         }
     }
@@ -368,7 +411,7 @@ __global__ void __launch_bounds__(kThreads) tb200_k_act_restore_across(const uin
                 for (int e = 0; e < E; ++e) v[e] = act_held(v[e], ActType<T>::kTop);
             }
             words<T, 8>(v, w);
-            if (at + E <= total) store32(out + at, w);
+            if (at + E <= total) store_piece(out + at, w);
             else {
 #pragma unroll
                 for (int e = 0; e < E; ++e)
@@ -395,7 +438,7 @@ struct RestoreJob {
     const uint2* q;
     const float* scales;
     uint4* out;
-    uint32_t total, per_row, nblk;                               // pieces of 8, in all and per row; blocks per row
+    uint32_t total, per_row, out_row, nblk;                      // pieces of 8, in all, per row and from row to row of the result; blocks per row
     int ctas;                                                    // 0: nothing to restore
 };
 template <typename T>
@@ -405,13 +448,15 @@ __device__ __forceinline__ void restore_job(const RestoreJob& job, uint32_t cta)
     for (uint64_t i0 = static_cast<uint64_t>(cta) * kThreads + threadIdx.x; i0 < job.total; i0 += U * step) {
         uint2 c[U];
         float s[U];
+        uint32_t to[U];
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             const uint64_t i = i0 + j * step;
             if (i < job.total) {
-                const uint32_t row = static_cast<uint32_t>(i) / job.per_row;
+                const uint32_t row = static_cast<uint32_t>(i) / job.per_row, col = static_cast<uint32_t>(i) - row * job.per_row;
+                to[j] = row * job.out_row + col;
                 c[j] = __ldcs(job.q + i);
-                s[j] = __ldg(job.scales + static_cast<int64_t>(row) * job.nblk + (static_cast<uint32_t>(i) - row * job.per_row) / 16);
+                s[j] = __ldg(job.scales + static_cast<int64_t>(row) * job.nblk + col / 16);
             }
         }
 #pragma unroll
@@ -423,7 +468,7 @@ __device__ __forceinline__ void restore_job(const RestoreJob& job, uint32_t cta)
                 uint32_t w[4];
                 decode<8>(codes, s[j], ActType<T>::kTop, v);
                 words<T, 4>(v, w);
-                job.out[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                job.out[to[j]] = make_uint4(w[0], w[1], w[2], w[3]);
             }
         }
     }
@@ -563,17 +608,27 @@ constexpr uint64_t aligned_to(uintptr_t bytes, const void* p, uintptr_t pitch_by
     return ((reinterpret_cast<uintptr_t>(p) | pitch_bytes) & (bytes - 1)) == 0;
 }
 
+// Pieces of 32 bytes where rows begin on such boundaries and are whole numbers of them, of 16 where that holds, else none of these.
+// (bf16, 33390 x 5464, saved by pieces of 16 in 0 us, by shifted words 171; restored in 0, across the ends of rows 123.)
+int piece_bytes(const void* x, int64_t row_bytes, int64_t pitch_bytes, const void* codes, int size) {
+    const uintptr_t all = reinterpret_cast<uintptr_t>(x) | static_cast<uintptr_t>(row_bytes) | static_cast<uintptr_t>(pitch_bytes);
+    for (int b = 32; b >= 16; b /= 2)
+        if (all % b == 0 && reinterpret_cast<uintptr_t>(codes) % (b / size) == 0) return b;
+    return 0;
+}
+
 template <typename T>
 int launch_save(const T* x, uint8_t* q, float* scales, int64_t rows, int64_t cols, int64_t ldx, cudaStream_t st) {
-    constexpr int E = 32 / sizeof(T), U = 4;
+    constexpr int kSize = sizeof(T);
     const uint32_t nblk = static_cast<uint32_t>((cols + kActBlock - 1) / kActBlock);
-    if (cols % E == 0 && aligned_to(32, x, rows > 1 ? ldx * sizeof(T) : 0) && aligned_to(E, q, 0)) {
+    const int piece = piece_bytes(x, cols * kSize, rows > 1 ? ldx * kSize : 0, q, kSize);
+    if (piece > 0) {
+        constexpr int E = 32 / kSize, U = 4;
         const uint32_t blocks = static_cast<uint32_t>(rows * nblk);
         const int grid = capped((static_cast<int64_t>(blocks) * (kActBlock / E) + kThreads * U - 1) / (kThreads * U), 8);
-        if (cols % kActBlock == 0 && (ldx == cols || rows == 1))
-            tb200_k_act_save<T, U, true><<<grid, kThreads, 0, st>>>(x, q, scales, blocks, nblk, cols, ldx);
-        else
-            tb200_k_act_save<T, U, false><<<grid, kThreads, 0, st>>>(x, q, scales, blocks, nblk, cols, ldx);
+        if (piece == 16) tb200_k_act_save<T, U, false, true><<<grid, kThreads, 0, st>>>(x, q, scales, blocks, nblk, cols, ldx);
+        else if (cols % kActBlock == 0 && (ldx == cols || rows == 1)) tb200_k_act_save<T, U, true, false><<<grid, kThreads, 0, st>>>(x, q, scales, blocks, nblk, cols, ldx);
+        else tb200_k_act_save<T, U, false, false><<<grid, kThreads, 0, st>>>(x, q, scales, blocks, nblk, cols, ldx);
     } else {
         const Spans sp = spans_of(rows, cols, Part<T>::kCols);
         tb200_k_act_save_any<T><<<capped((sp.count + 7) / 8, 8), kThreads, 0, st>>>(x, q, scales, sp.count, sp.per_row, sp.width, nblk, rows, cols, ldx);
@@ -582,20 +637,28 @@ int launch_save(const T* x, uint8_t* q, float* scales, int64_t rows, int64_t col
     return TB200_OK;
 }
 
+template <typename T, int E>
+void launch_restore_pieces(const uint8_t* q, const float* scales, T* out, int64_t rows, int64_t cols, int64_t ldo, uint32_t nblk, cudaStream_t st) {
+    constexpr int U = 128 / (E * static_cast<int>(sizeof(T)));
+    const uint32_t blocks = static_cast<uint32_t>(rows * nblk);
+    const int grid = capped((static_cast<int64_t>(blocks) * (kActBlock / E) + kThreads * U - 1) / (kThreads * U), 8);
+    if (cols % kActBlock == 0 && ldo == cols) tb200_k_act_restore<T, E, U, true><<<grid, kThreads, 0, st>>>(q, scales, out, blocks, nblk, cols, ldo);
+    else tb200_k_act_restore<T, E, U, false><<<grid, kThreads, 0, st>>>(q, scales, out, blocks, nblk, cols, ldo);
+}
+
 template <typename T>
-int launch_restore(const uint8_t* q, const float* scales, T* out, int64_t rows, int64_t cols, cudaStream_t st) {
-    constexpr int E = 32 / sizeof(T), U = 4;
+int launch_restore(const uint8_t* q, const float* scales, T* out, int64_t rows, int64_t cols, int64_t ldo, cudaStream_t st) {
+    constexpr int kSize = sizeof(T), E = 32 / kSize, U = 4;
     const uint32_t nblk = static_cast<uint32_t>((cols + kActBlock - 1) / kActBlock);
-    if (cols % E == 0 && aligned_to(E, q, 0) && aligned_to(32, out, 0)) {
-        const uint32_t blocks = static_cast<uint32_t>(rows * nblk);
-        const int grid = capped((static_cast<int64_t>(blocks) * (kActBlock / E) + kThreads * U - 1) / (kThreads * U), 8);
-        if (cols % kActBlock == 0) tb200_k_act_restore<T, U, true><<<grid, kThreads, 0, st>>>(q, scales, out, blocks, nblk, cols);
-        else tb200_k_act_restore<T, U, false><<<grid, kThreads, 0, st>>>(q, scales, out, blocks, nblk, cols);
+    const int piece = piece_bytes(out, cols * kSize, ldo * kSize, q, kSize);
+    const int64_t total = rows * cols;
+    if (piece == 32) {
+        launch_restore_pieces<T, E>(q, scales, out, rows, cols, ldo, nblk, st);
+    } else if (piece == 16) {
+        launch_restore_pieces<T, E / 2>(q, scales, out, rows, cols, ldo, nblk, st);
     } else if (cols >= 16 && aligned_to(16, q, 0) && aligned_to(32, out, 0)) {
-        const int64_t total = rows * cols;
         tb200_k_act_restore_across<T, U><<<capped((total + kThreads * E * U - 1) / (kThreads * E * U), 8), kThreads, 0, st>>>(q, scales, out, total, nblk, cols);
     } else {
-        const int64_t total = rows * cols;
         tb200_k_act_restore_any<T><<<capped((total + kThreads - 1) / kThreads, 8), kThreads, 0, st>>>(q, scales, out, total, nblk, cols);
     }
     TB200_CUDA_TRY(cudaGetLastError());
@@ -644,17 +707,17 @@ int check_sizes(const char* what, int64_t rows, int64_t cols) {
 }  // namespace
 
 int launch_gated_act_bwd(const void* dh, const void* gq, const float* gs, const void* uq, const float* us, void* dg, void* du,
-                         int64_t m, int64_t f, int64_t ldg, const void* xq, const float* xs, void* x, int64_t k, int act, int dtype,
+                         int64_t m, int64_t f, int64_t ldg, const void* xq, const float* xs, void* x, int64_t k, int64_t ldx, int act, int dtype,
                          cudaStream_t st) {
     RestoreJob job = {};
     if (xq) {
         const int64_t total = m * (k / 8);
         // up to 4 M numbers (5 us by themselves); 12867 x 3616 took 52 us together with dg and du, 40 in two launches
         if ((reinterpret_cast<uintptr_t>(xq) & 7) == 0 && m * k <= (4ll << 20)) {
-            job = {static_cast<const uint2*>(xq), xs, static_cast<uint4*>(x), static_cast<uint32_t>(total), static_cast<uint32_t>(k / 8),
+            job = {static_cast<const uint2*>(xq), xs, static_cast<uint4*>(x), static_cast<uint32_t>(total), static_cast<uint32_t>(k / 8), static_cast<uint32_t>(ldx / 8),
                    static_cast<uint32_t>((k + kActBlock - 1) / kActBlock), capped((total + 2 * kThreads - 1) / (2 * kThreads), 8)};
         } else {
-            const int rc = launch_act_restore(xq, xs, x, dtype, m, k, st);
+            const int rc = launch_act_restore(xq, xs, x, dtype, m, k, ldx, st);
             if (rc != TB200_OK) return rc;
         }
     }
@@ -662,11 +725,11 @@ int launch_gated_act_bwd(const void* dh, const void* gq, const float* gs, const 
                                  : launch_gated_act<__nv_bfloat16>(dh, gq, gs, uq, us, dg, du, m, f, ldg, job, act, st);
 }
 
-int launch_act_restore(const void* q, const float* scales, void* out, int dtype, int64_t rows, int64_t cols, cudaStream_t st) {
+int launch_act_restore(const void* q, const float* scales, void* out, int dtype, int64_t rows, int64_t cols, int64_t ldo, cudaStream_t st) {
     const uint8_t* c = static_cast<const uint8_t*>(q);
-    if (dtype == TB200_DT_F32) return launch_restore<float>(c, scales, static_cast<float*>(out), rows, cols, st);
-    if (dtype == TB200_DT_F16) return launch_restore<__half>(c, scales, static_cast<__half*>(out), rows, cols, st);
-    return launch_restore<__nv_bfloat16>(c, scales, static_cast<__nv_bfloat16*>(out), rows, cols, st);
+    if (dtype == TB200_DT_F32) return launch_restore<float>(c, scales, static_cast<float*>(out), rows, cols, ldo, st);
+    if (dtype == TB200_DT_F16) return launch_restore<__half>(c, scales, static_cast<__half*>(out), rows, cols, ldo, st);
+    return launch_restore<__nv_bfloat16>(c, scales, static_cast<__nv_bfloat16*>(out), rows, cols, ldo, st);
 }
 
 }  // namespace tb200
@@ -704,5 +767,5 @@ extern "C" int tb200_act_restore_fp8(const void* q, const float* scales, void* o
     const int64_t size = dtype == TB200_DT_F32 ? 4 : 2;
     if (reinterpret_cast<uintptr_t>(out) % size || reinterpret_cast<uintptr_t>(scales) & 3)
         return fail(TB200_ERR_ALIGN, "act_restore_fp8: out and scales must be aligned to their elements");
-    return launch_act_restore(q, scales, out, dtype, rows, cols, static_cast<cudaStream_t>(stream));
+    return launch_act_restore(q, scales, out, dtype, rows, cols, cols, static_cast<cudaStream_t>(stream));
 }

@@ -188,10 +188,12 @@ int launch_over_previous(void (*kern)(Maps, Args), int grid, int block, int smem
 
 // ---- launchers shared between the files of the feed-forward block ----------------------------------------------
 // The backward pass's two intermediates, dg = dh * u * f'(g) and du = dh * f(g) with row pitch ldg; and, where xq is given, the
-// block's input [m, k] restored from its 8-bit form (k a multiple of 8).
+// block's input [m, k] restored from its 8-bit form with row pitch ldx (k and ldx multiples of 8; ldx = k unless xq lies on an 8-byte
+// boundary).
 int launch_gated_act_bwd(const void* dh, const void* gq, const float* gs, const void* uq, const float* us, void* dg, void* du,
-                         int64_t m, int64_t f, int64_t ldg, const void* xq, const float* xs, void* x, int64_t k, int act, int dtype,
+                         int64_t m, int64_t f, int64_t ldg, const void* xq, const float* xs, void* x, int64_t k, int64_t ldx, int act, int dtype,
                          cudaStream_t st);
-int launch_act_restore(const void* q, const float* scales, void* out, int dtype, int64_t rows, int64_t cols, cudaStream_t st);
+// ldo: row pitch of out, cols unless rows of out and of q are whole 16-byte and 8-byte pieces on such boundaries.
+int launch_act_restore(const void* q, const float* scales, void* out, int dtype, int64_t rows, int64_t cols, int64_t ldo, cudaStream_t st);
 
 }  // namespace tb200

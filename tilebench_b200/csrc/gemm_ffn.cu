@@ -1471,8 +1471,8 @@ int ffn_products_bwd(const void* dg, const void* du, int64_t ldg, const void* x,
 
 bool to_elements(const void* p, uintptr_t size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
 constexpr int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
-// Rows of dg and du begin on 128-byte boundaries: a copy of 128 bytes that begins elsewhere moves a fifth sector (12756 rows of
-// 1264 x 19937: 2450 us in rows of 39888 bytes, 0 so).
+// Rows of dg, du and a restored x begin on 128-byte boundaries: a copy of 128 bytes that begins elsewhere moves a fifth sector
+// (12756 rows of 1264 x 19937: 2547 us with rows of dg and du of 39888 bytes, 2282 so).
 int64_t pitch_of(int64_t f) { return round_up(f, 64); }
 
 int check_common(const char* what, int64_t m, int64_t f, int64_t k, int act, int dtype) {
@@ -1519,7 +1519,7 @@ extern "C" int tb200_ffn_gated(const void* x, const void* wg, const void* wu, vo
 extern "C" size_t tb200_ffn_gated_bwd_workspace_bytes(int64_t m, int64_t f, int64_t k, int x_codes) {
     if (m <= 0 || f <= 0 || k <= 0) return 0;
     const BwdPlan plan = bwd_plan(m, f, k);
-    return static_cast<size_t>(2 * round_up(m * pitch_of(f) * 2, 256) + (x_codes ? round_up(m * k * 2, 256) : 0) +
+    return static_cast<size_t>(2 * round_up(m * pitch_of(f) * 2, 256) + (x_codes ? round_up(m * pitch_of(k) * 2, 256) : 0) +
                                (plan.dx > 1 ? plan.dx * m * k * 4 : 0) + (plan.dw > 1 ? plan.dw * 2 * f * k * 4 : 0));
 }
 
@@ -1538,7 +1538,7 @@ extern "C" int tb200_ffn_gated_bwd(const void* dh, const void* wg, const void* w
     }
     if (!dh || !wg || !wu || !x || !gq || !gs || !uq || !us || !dx) return fail(TB200_ERR_ARG, "ffn_gated_bwd: null pointer");
     const bool codes = xs != nullptr;
-    if (codes || m == 1) ldx = k;
+    if (codes || m == 1) ldx = k;                                // no pitch of the caller's, or none that matters
     if (ldx < k || ldx % 8 != 0) return fail(TB200_ERR_ALIGN, "ffn_gated_bwd: row stride of x %lld must be a multiple of 8 and at least k", (long long)ldx);
     if (!aligned16(wg) || !aligned16(wu) || !aligned16(dx) || !aligned16(dwg) || !aligned16(dwu) || (!codes && !aligned16(x)))
         return fail(TB200_ERR_ALIGN, "ffn_gated_bwd: x, wg, wu, dx, dwg, dwu must be 16-byte aligned");
@@ -1553,8 +1553,9 @@ extern "C" int tb200_ffn_gated_bwd(const void* dh, const void* wg, const void* w
     void* dg = ws;
     void* du = ws + round_up(m * ldg * 2, 256);
     void* xr = ws + 2 * round_up(m * ldg * 2, 256);
-    float* sums = reinterpret_cast<float*>(static_cast<uint8_t*>(xr) + (codes ? round_up(m * k * 2, 256) : 0));
-    rc = launch_gated_act_bwd(dh, gq, gs, uq, us, dg, du, m, f, ldg, codes ? x : nullptr, xs, xr, k, act, dtype, st);
+    float* sums = reinterpret_cast<float*>(static_cast<uint8_t*>(xr) + (codes ? round_up(m * pitch_of(k) * 2, 256) : 0));
+    if (codes) ldx = reinterpret_cast<uintptr_t>(x) % 8 == 0 ? pitch_of(k) : k;
+    rc = launch_gated_act_bwd(dh, gq, gs, uq, us, dg, du, m, f, ldg, codes ? x : nullptr, xs, xr, k, ldx, act, dtype, st);
     if (rc != TB200_OK) return rc;
     if (codes) x = xr;
     return dtype == TB200_DT_F16 ? ffn_products_bwd<__half>(dg, du, ldg, x, ldx, wg, wu, dx, dwg, dwu, sums, m, f, k, st)
