@@ -72,6 +72,18 @@ def test_save_and_restore_are_exact(cuda_device, rows, cols, pad, dtype):
         assert torch.equal(restore.run(q, s, torch.bfloat16).float(), restore.run(q, s, torch.float32))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,cols,pad", [(5, 2060, 0), (5, 2060, 4), (40, 1032, 8), (3, 5464, 8), (70, 8, 8), (6, 140, 4), (3, 2049, 1), (900, 130, 3)])
+def test_save_and_restore_by_pieces_of_every_width(cuda_device, rows, cols, pad, dtype):
+    g = gen(rows + 17 * cols)
+    x = (normal(g, rows, cols + pad) * torch.exp(2 * normal(g, rows, 1))).to(dtype)[:, :cols]
+    x[0, -1], x[-1, 0] = float("inf"), float("nan")
+    q, s = save.run(x)
+    want_q, want_s = tensors.checkpoint_fp8(x)
+    assert torch.equal(s, want_s) and same_codes(q, want_q)
+    assert same_codes(restore.run(q, s, dtype), tensors.restore_fp8(want_q, want_s, dtype))
+
+
 @pytest.mark.parametrize("offset", [1, 3, 8])
 def test_save_and_restore_at_odd_addresses(cuda_device, offset):
     """Views that begin at any element, codes that begin at any byte; what lies around the outputs stays."""
@@ -195,6 +207,16 @@ def test_forward(cuda_device, m, k, f, dtype):
     check_held(uq, us, u, eu)
 
 
+@pytest.mark.parametrize("m,k,f", [(129, 64, 9), (200, 520, 136), (247, 2048, 1164), (513, 4096, 70), (1000, 1024, 264), (1024, 4104, 131), (1025, 512, 64)])
+def test_forward_of_rows_in_blocks(cuda_device, m, k, f):
+    """More than 128 rows and few hidden units: blocks of 128 rows on narrow tiles, with and without shares of the contraction."""
+    x, wg, wu = block_inputs(m, k, f, torch.bfloat16, pad=8)
+    h = torch.full((m + 2, f), 7.0, dtype=torch.bfloat16, device="cuda")
+    native.load().ffn_gated(x, wg, wu, h[1:-1], native.activation("silu"), None, None, None, None)
+    check_h(h[1:-1], x, wg, wu, "silu")
+    assert bool((h[0] == 7).all()) and bool((h[-1] == 7).all())
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("m", [3, 40, 200])
 def test_forward_gates_over_their_range(cuda_device, act, m):
@@ -307,6 +329,13 @@ def test_backward_of_very_large_projections(cuda_device, act):
     args = list(backward_inputs(40, 64, 40, torch.bfloat16))
     args[6] = torch.exp2(torch.arange(40, device="cuda") * 2.0 + 18)[:, None].contiguous()       # times codes of up to 448
     check_gradients(bwd.run(*args, act), args, act, torch.bfloat16)
+
+
+@pytest.mark.parametrize("m,k,f", [(512, 9472, 2820), (1100, 2056, 1900), (2000, 1024, 3000), (300, 520, 20000), (60, 4104, 6500)])
+def test_backward_over_many_tiles(cuda_device, m, k, f):
+    """Enough tiles for several rounds: dx and the weights' gradients in one launch, in two, and dx by the kernel for few rows."""
+    args = backward_inputs(m, k, f, torch.bfloat16, x_codes=True)
+    check_gradients(bwd.run(*args, "relu"), args, "relu", torch.bfloat16)
 
 
 @pytest.mark.parametrize("m,k,f", [(3000, 136, 140), (9000, 264, 24), (520, 72, 9000), (70, 2056, 5000)])

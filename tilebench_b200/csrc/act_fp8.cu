@@ -114,7 +114,7 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const uint32_t (&c)[N]) 
 // Saving.  E numbers (32 bytes) per lane, 128 / E lanes per block, U pieces in flight; a row ends inside a block where cols is not a
 // multiple of 128 (lanes past it hold zeros).  FLAT: rows are whole blocks and adjacent, so the piece's number is its place.
 // HALVES: rows begin on 16-byte boundaries and may end with half a piece.  (Pieces of 16 bytes instead, at twice the shuffles per
-// number: 33390 x 5464 in 163 us where this takes 0.)
+// number: 33390 x 5464 in 163 us where this takes 99.)
 template <typename T, int U, bool FLAT, bool HALVES>
 __global__ void __launch_bounds__(kThreads) tb200_k_act_save(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales,
                                                    uint32_t blocks, uint32_t nblk, int64_t cols, int64_t ldx) {
@@ -301,19 +301,15 @@ __device__ __forceinline__ void store_word(uint8_t* row, int b, int lo, int hi, 
             if (b + i >= lo && b + i < hi) row[b + i] = static_cast<uint8_t>(w >> (8 * i));
     }
 }
-template <typename T> struct Part {
-    static constexpr int E = 16 / sizeof(T);                     // numbers per lane
-    static constexpr int kCols = 32 * E;
-    static constexpr int kLanes = kActBlock / E;                 // lanes per block
-};
-
-// spans: warps' shares of the rows, per_row of them in a row, `width` columns each (a multiple of the part).
-template <typename T>
+// spans: warps' shares of the rows, per_row of them in a row, `width` columns each (a multiple of the part).  PIECE: bytes per lane.
+// 32 halve the shuffles per number (33390 x 5465 in bf16, with its restoring: 298 us with pieces of 16, 271 so), 16 leave fewer lanes
+// idle in narrow rows (100000 x 130: 48 us against 62).
+template <typename T, int PIECE>
 __global__ void __launch_bounds__(kThreads) tb200_k_act_save_any(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales,
                                                        int64_t spans, uint32_t per_row, int width, uint32_t nblk, int64_t rows, int64_t cols,
                                                        int64_t ldx) {
     let_next_begin();
-    constexpr int E = Part<T>::E, N = E / 4, kLanes = Part<T>::kLanes, kCols = Part<T>::kCols;
+    constexpr int E = PIECE / sizeof(T), N = E / 4, W = PIECE / 4, kLanes = kActBlock / E, kCols = 32 * E;
     const int lane = threadIdx.x & 31;
     const uint8_t *begin = reinterpret_cast<const uint8_t*>(x), *end = reinterpret_cast<const uint8_t*>(x + (rows - 1) * ldx + cols);
     for (int64_t s = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); s < spans; s += static_cast<int64_t>(gridDim.x) * (kThreads / 32)) {
@@ -324,20 +320,20 @@ __global__ void __launch_bounds__(kThreads) tb200_k_act_save_any(const T* __rest
         float* const sc = scales + row * nblk + first / kActBlock;
         const int mis = static_cast<int>(reinterpret_cast<uintptr_t>(to) & 3);
         uint32_t before = 0;                                     // lane 31's last word of the part before
-        uint32_t ahead[5];                                       // the next part's words, on the way while one is worked on
+        uint32_t ahead[W + 1];                                       // the next part's words, on the way while one is worked on
         auto fetch = [&](int col) {
             const uint8_t* p = from + static_cast<int64_t>(col) * sizeof(T);
-            load_words<4>(p + lane * 16, begin, end, part_inside<4>(p, begin, end), ahead);
+            load_words<W>(p + lane * PIECE, begin, end, part_inside<W>(p, begin, end), ahead);
         };
         fetch(0);
 #pragma unroll 2
         for (int col = 0; col < n; col += kCols) {
-            uint32_t r[4], c[N];
+            uint32_t r[W], c[N];
             float v[E];
             const int at = col + lane * E;                       // the lane's first column in the span
-            into_place<4>(ahead, from, r);
+            into_place<W>(ahead, from, r);
             if (col + kCols < n) fetch(col + kCols);
-            numbers<T, 4>(r, v);
+            numbers<T, W>(r, v);
             if (at + E > n) {
 #pragma unroll
                 for (int i = 0; i < E; ++i) v[i] = at + i < n ? v[i] : 0.0f;
@@ -347,7 +343,7 @@ __global__ void __launch_bounds__(kThreads) tb200_k_act_save_any(const T* __rest
             // aligned words: the last `mis` bytes of the codes before and the first of the lane's own
             const uint32_t last = c[N - 1], first_before = __shfl_sync(0xffffffffu, lane == 31 ? before : last, (lane + 31) & 31);
 #pragma unroll
-            for (int i = 0; i < N; ++i) store_word(to, at + 4 * i - mis, 0, n, __funnelshift_l(i == 0 ? first_before : c[0], c[i], 8 * mis));
+            for (int i = 0; i < N; ++i) store_word(to, at + 4 * i - mis, 0, n, __funnelshift_l(i == 0 ? first_before : c[i > 0 ? i - 1 : 0], c[i], 8 * mis));
             before = last;
         }
         const int end = (n + kCols - 1) / kCols * kCols;         // codes of lane 31 that belong to the word behind the last part's
@@ -547,7 +543,7 @@ __global__ void __launch_bounds__(kThreads) tb200_k_ffn_gated_bwd_any(const T* _
     const uint32_t ctas = gridDim.x - job.ctas;
     if (blockIdx.x >= ctas) return restore_job<T>(job, blockIdx.x - ctas);
     static_assert(sizeof(T) == 2, "8 numbers of 16 bits and 8 codes per lane");
-    constexpr int E = Part<T>::E, kCols = Part<T>::kCols;
+    constexpr int E = 8, kCols = 32 * E;
     const int lane = threadIdx.x & 31;
     const int64_t total = m * f;
     for (int64_t s = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); s < spans; s += static_cast<int64_t>(ctas) * (kThreads / 32)) {
@@ -609,7 +605,7 @@ constexpr uint64_t aligned_to(uintptr_t bytes, const void* p, uintptr_t pitch_by
 }
 
 // Pieces of 32 bytes where rows begin on such boundaries and are whole numbers of them, of 16 where that holds, else none of these.
-// (bf16, 33390 x 5464, saved by pieces of 16 in 0 us, by shifted words 171; restored in 0, across the ends of rows 123.)
+// (bf16, 33390 x 5464, saved in 99 us, by shifted words in 171; restored in 101, across the ends of rows 123.)
 int piece_bytes(const void* x, int64_t row_bytes, int64_t pitch_bytes, const void* codes, int size) {
     const uintptr_t all = reinterpret_cast<uintptr_t>(x) | static_cast<uintptr_t>(row_bytes) | static_cast<uintptr_t>(pitch_bytes);
     for (int b = 32; b >= 16; b /= 2)
@@ -630,8 +626,12 @@ int launch_save(const T* x, uint8_t* q, float* scales, int64_t rows, int64_t col
         else if (cols % kActBlock == 0 && (ldx == cols || rows == 1)) tb200_k_act_save<T, U, true, false><<<grid, kThreads, 0, st>>>(x, q, scales, blocks, nblk, cols, ldx);
         else tb200_k_act_save<T, U, false, false><<<grid, kThreads, 0, st>>>(x, q, scales, blocks, nblk, cols, ldx);
     } else {
-        const Spans sp = spans_of(rows, cols, Part<T>::kCols);
-        tb200_k_act_save_any<T><<<capped((sp.count + 7) / 8, 8), kThreads, 0, st>>>(x, q, scales, sp.count, sp.per_row, sp.width, nblk, rows, cols, ldx);
+        // the wider pieces where rows have some four parts of them and at most a tenth more idle lanes
+        const int64_t part = 32 * 32 / kSize, wide = (cols + part - 1) / part * part, narrow = (cols + part / 2 - 1) / (part / 2) * (part / 2);
+        const bool by32 = cols > 3 * part && 10 * wide <= 11 * narrow;
+        const Spans sp = spans_of(rows, cols, static_cast<int>(by32 ? part : part / 2));
+        (by32 ? tb200_k_act_save_any<T, 32> : tb200_k_act_save_any<T, 16>)<<<capped((sp.count + 7) / 8, 8), kThreads, 0, st>>>(
+            x, q, scales, sp.count, sp.per_row, sp.width, nblk, rows, cols, ldx);
     }
     TB200_CUDA_TRY(cudaGetLastError());
     return TB200_OK;
@@ -676,7 +676,7 @@ int launch_gated(const void* dh, const void* gq, const float* gs, const void* uq
             static_cast<const uint4*>(dh), static_cast<const uint2*>(gq), gs, static_cast<const uint2*>(uq), us, static_cast<uint4*>(dg),
             static_cast<uint4*>(du), static_cast<uint32_t>(total), static_cast<uint32_t>(f / 8), static_cast<uint32_t>(ldg / 8), nblk, job);
     } else {
-        const Spans sp = spans_of(m, f, Part<T>::kCols);
+        const Spans sp = spans_of(m, f, 256);
         tb200_k_ffn_gated_bwd_any<T, ACT><<<capped((sp.count + 7) / 8, 8) + job.ctas, kThreads, 0, st>>>(
             static_cast<const T*>(dh), static_cast<const uint8_t*>(gq), gs, static_cast<const uint8_t*>(uq), us, static_cast<T*>(dg),
             static_cast<T*>(du), sp.count, sp.per_row, sp.width, m, f, ldg, nblk, job);

@@ -559,9 +559,9 @@ tb200_k_ffn_pair(const __grid_constant__ FfnMaps<KIND> maps, const __grid_consta
 }
 
 // ------------------------------------------------------------------------------------------------
-// Forward block for a decoding batch (m <= 128 rows, no checkpoints): bound by reading the weights, so every SM has to
-// stream an equal share of them.  One CTA per tile of 128 rows x w hidden units (N = 2 w: w rows of Wg, w rows of Wu),
-// with w, a multiple of 8, chosen per call so that the tiles fill one wave (or whole waves) of SMs.  Where f is too
+// Forward block for a decoding batch (m <= 128 rows): bound by reading the weights, so every SM has to stream an equal share of
+// them.  One CTA per tile of 128 rows x w hidden units (N = 2 w: w rows of Wg, w rows of Wu), with w, a multiple of 8, chosen per
+// call so that the tiles fill one wave (or whole waves) of SMs.  More rows, in blocks of 128, where f is small.  Where f is too
 // small for that, the CTAs of a cluster share the contraction of a tile (SPLIT): each leaves its sums in its shared
 // memory, and each adds up a share of the columns in a fixed order, reading its peers' memory.
 constexpr int kMaxStages = 8;
@@ -671,7 +671,8 @@ __global__ void __launch_bounds__(kThreads, 1) tb200_k_ffn_mid(const __grid_cons
     constexpr bool SPLIT = SHARES > 1;
     const int share = SPLIT ? static_cast<int>(cluster_ctarank()) : 0;
     const int kb0 = KB * share / SHARES, kb1 = KB * (share + 1) / SHARES;
-    const int tiles = (p.f + w - 1) / w;
+    const int blocks = FEW ? 1 : (p.m + kHalf - 1) / kHalf;      // of 128 rows; a tile's are neighbours, so that they share its weights in L2
+    const int tiles = (p.f + w - 1) / w * blocks;
     const int t0 = static_cast<int>(blockIdx.x) / SHARES;
     const int t_step = SPLIT ? tiles : static_cast<int>(gridDim.x);                 // with SPLIT a CTA has one tile
     const bool vec = p.f % 4 == 0 && (reinterpret_cast<uintptr_t>(p.h) & 7) == 0 &&  // four of a row's results can be stored at once
@@ -712,8 +713,8 @@ __global__ void __launch_bounds__(kThreads, 1) tb200_k_ffn_mid(const __grid_cons
     if (warp == 0 && lane == 0 && t0 < tiles) {
         // the weights of the first stages, while the kernel before ends
         for (int kb = kb0; kb < min(kb1, kb0 + S); ++kb) {
-            prefetch_2d(&maps.wg, kb * kBK, t0 * w);
-            prefetch_2d(&maps.wu, kb * kBK, t0 * w);
+            prefetch_2d(&maps.wg, kb * kBK, t0 / blocks * w);
+            prefetch_2d(&maps.wu, kb * kBK, t0 / blocks * w);
         }
     }
     wait_for_previous();
@@ -721,16 +722,17 @@ __global__ void __launch_bounds__(kThreads, 1) tb200_k_ffn_mid(const __grid_cons
     if (warp == 0) {
         // ---------------- TMA producer ----------------
         if (lane == 0) {
-            uint32_t s = 0, ph = 1, it = 0;
+            uint32_t s = 0, ph = 1;
             bool ok = true;
             for (int t = t0; t < tiles && ok; t += t_step) {
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int unit = t / blocks * w, row = t % blocks * kHalf;
+                for (int kb = kb0; kb < kb1; ++kb) {
                     if (!mbar_wait(&bar_empty[s], ph, ST_WAIT_SMEM_EMPTY, kb)) { ok = false; break; }
                     uint8_t* stage = smem + s * stage_bytes;
                     mbar_expect_tx(&bar_full[s], stage_bytes);
-                    tma_load_2d(stage + x_bytes, &maps.wg, &bar_full[s], kb * kBK, t * w);
-                    tma_load_2d(stage + x_bytes + w * 128, &maps.wu, &bar_full[s], kb * kBK, t * w);
-                    tma_load_2d(stage, &maps.x, &bar_full[s], kb * kBK, 0);
+                    tma_load_2d(stage + x_bytes, &maps.wg, &bar_full[s], kb * kBK, unit);
+                    tma_load_2d(stage + x_bytes + w * 128, &maps.wu, &bar_full[s], kb * kBK, unit);
+                    tma_load_2d(stage, &maps.x, &bar_full[s], kb * kBK, row);
                     if (++s == static_cast<uint32_t>(S)) { s = 0; ph ^= 1; }
                 }
             }
@@ -791,6 +793,7 @@ __global__ void __launch_bounds__(kThreads, 1) tb200_k_ffn_mid(const __grid_cons
             ok = ok && mbar_wait(&bar_afull[acc], (cnt >> 1) & 1, ST_WAIT_TMEM_FULL, t);
             tc_fence_after();
             const uint32_t t_acc = t_lane + acc * (FEW ? kFewCols : 256);
+            const int first_row = t % blocks * kHalf, rows = p.m - first_row;         // of the tile (may be more than 128)
             if constexpr (FEW) {
                 // A lane has one row of the weights and 16 of the tokens at a time; the sums go token by token to where they are
                 // combined: the ring (SPLIT, as below) or a place of their own.
@@ -827,7 +830,7 @@ __global__ void __launch_bounds__(kThreads, 1) tb200_k_ffn_mid(const __grid_cons
                 // this CTA's sums, row by row.  A row pitch of 4 more than a multiple of 16 keeps eight lanes' (rows')
                 // 16-byte pieces on different banks.  Every copy into the ring has landed and been used by the time the
                 // accumulator is complete.
-                if (row0 < p.m) {
+                if (row0 < rows) {
                     const int at = part * ((w / 2 + 7) / 8 * 8), n = min((w / 2 + 7) / 8 * 8, 2 * w - at);
                     float* mine = reinterpret_cast<float*>(smem) + (row0 + lane) * (2 * w + 4) + at;
 #pragma unroll 1
@@ -835,7 +838,7 @@ __global__ void __launch_bounds__(kThreads, 1) tb200_k_ffn_mid(const __grid_cons
                         uint32_t v[16];
                         tmem_ld16(t_acc + at + c, v);
                         tmem_wait_ld();
-                        if (row0 + lane < p.m) {
+                        if (row0 + lane < rows) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
                                 if (c + 4 * i < n) *reinterpret_cast<uint4*>(mine + c + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
@@ -844,7 +847,7 @@ __global__ void __launch_bounds__(kThreads, 1) tb200_k_ffn_mid(const __grid_cons
                 }
             } else {
                 const int at = part * ((w / 4 + 7) / 8 * 8);
-                if (row0 < p.m && at < w) {
+                if (row0 < rows && at < w) {
                     uint32_t g[32], u[32];
                     tmem_ld32(t_acc + at, g);
                     tmem_ld32(t_acc + w + at, u);
@@ -856,7 +859,7 @@ __global__ void __launch_bounds__(kThreads, 1) tb200_k_ffn_mid(const __grid_cons
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar_aempty[acc]);
                 quarter_sync(quarter);
-                flush<T, 16>(buf, 0, static_cast<T*>(p.h) + static_cast<int64_t>(row0) * p.f + t * w, p.f, 8 * part, p.m - row0, min(w, p.f - t * w), lane);
+                flush<T, 16>(buf, 0, static_cast<T*>(p.h) + static_cast<int64_t>(first_row + row0) * p.f + t / blocks * w, p.f, 8 * part, rows - row0, min(w, p.f - t / blocks * w), lane);
                 quarter_sync(quarter);
             }
         }
@@ -872,11 +875,13 @@ __global__ void __launch_bounds__(kThreads, 1) tb200_k_ffn_mid(const __grid_cons
         if constexpr (SAVE) {
             for (int r = share + SHARES * warp; r < p.m; r += SHARES * (kThreads / 32)) save_row(base, 2 * w + 4, r, t0);
         } else {
-            for (int i = threadIdx.x; i < p.m * qn; i += kThreads) {
+            const int first_row = t0 % blocks * kHalf, rows = min(kHalf, p.m - first_row), unit = t0 / blocks * w;
+            T* const h = static_cast<T*>(p.h) + static_cast<int64_t>(first_row) * p.f;
+            for (int i = threadIdx.x; i < rows * qn; i += kThreads) {
                 const int r = i / qn, c = 4 * (q0 + i - r * qn);
                 float g[4], u[4];
                 gather4<SHARES>(base, 2 * w + 4, w, r, c, g, u);
-                store4<T, ACT>(g, u, static_cast<T*>(p.h), r, t0 * w + c, p.f, vec);
+                store4<T, ACT>(g, u, h, r, unit + c, p.f, vec);
             }
         }
         cluster_sync_all();                                      // no CTA leaves while a peer reads its memory
@@ -1114,7 +1119,7 @@ int launch_fwd(const FfnMaps<FK_FWD>& maps, const FfnArgs& args, int act, cudaSt
 }
 
 // ---- the decoding batch's tiles ----
-struct MidPlan { int w, shares; };
+struct MidPlan { int w, shares; float time; };
 
 template <int SHARES>
 int clusters_of(int* n) {                        // clusters of SHARES CTAs that the device holds at once
@@ -1154,22 +1159,23 @@ int mid_plan(int64_t m, int64_t f, int64_t k, int least_width, MidPlan* plan) {
     if (rc == TB200_OK) rc = clusters_of<4>(&clusters[2]);
     if (rc == TB200_OK) rc = clusters_of<8>(&clusters[3]);
     if (rc != TB200_OK) return rc;
-    const int KB = static_cast<int>((k + kBK - 1) / kBK), x_rows = static_cast<int>((m + 7) / 8 * 8);
+    const int KB = static_cast<int>((k + kBK - 1) / kBK), x_rows = static_cast<int>(m < kHalf ? (m + 7) / 8 * 8 : kHalf);
+    const int64_t blocks = (m + kHalf - 1) / kHalf;
     float best = 0.0f;
     for (int i = 0; i < 4; ++i) {
         const int shares = 1 << i;
-        if (shares > KB) break;                                  // every share has a stage
+        if (shares > KB || clusters[i] < 1) break;               // every share has a stage
         for (int w = least_width; w <= kHalf; w += 8) {
-            const int64_t tiles = (f + w - 1) / w;
-            if (shares > 1 && tiles > clusters[i]) continue;     // shared tiles run in one wave
+            const int64_t tiles = (f + w - 1) / w * blocks;
+            if (shares > 1 && tiles > clusters[i]) continue;     // shared tiles run in one wave: further ones, whose CTAs begin anew, gain nothing
             const int64_t waves = (tiles + clusters[i] - 1) / clusters[i], at_once = (tiles < clusters[i] ? tiles : clusters[i]) * shares;
-            const float link = static_cast<float>(x_rows + 2 * w) * (128.0f / 95e3f), hbm = static_cast<float>(at_once) * (2 * w) * (128.0f / 6.4e6f);
+            const float link = static_cast<float>(x_rows + 2 * w) * (128.0f / 95e3f), hbm = static_cast<float>(at_once) * (2 * w) * (128.0f / 6.4e6f) / static_cast<float>(blocks);
             const float stage = fmaxf(m <= kFewRows && 2 * w > kHalf ? 0.37f : 0.25f, fmaxf(link, hbm));
             const float t = static_cast<float>(waves) * static_cast<float>((KB + shares - 1) / shares) * stage +
-                            (shares > 1 ? 0.8f + static_cast<float>(m) * (8 * w) / 20e3f : 0.6f * static_cast<float>(waves) + 0.012f * w);
+                            (shares > 1 ? 0.8f + static_cast<float>(x_rows) * (8 * w) / 20e3f : 0.6f * static_cast<float>(waves) + 0.012f * w);
             if (best == 0.0f || t < best) {
                 best = t;
-                *plan = {w, shares};
+                *plan = {w, shares, t};
             }
         }
     }
@@ -1182,8 +1188,9 @@ int launch_mid(const MidMaps& maps, const MidArgs& args, cudaStream_t st) {
     static PerDeviceInt attr_set;
     const int rc = ensure_max_smem(attr_set, reinterpret_cast<const void*>(kern), kMidSmemBytes);
     if (rc != TB200_OK) return rc;
-    const int tiles = (args.f + args.w - 1) / args.w;
-    return launch_over_previous(kern, SHARES > 1 ? tiles * SHARES : tiles < num_sms() ? tiles : num_sms(), kThreads, kMidSmemBytes, SHARES, st, maps, args);
+    const int64_t tiles = static_cast<int64_t>((args.f + args.w - 1) / args.w) * ((args.m + kHalf - 1) / kHalf);
+    if (tiles > 0x7fffffffll / 8) return fail(TB200_ERR_UNSUPPORTED, "ffn_gated: too many tiles");
+    return launch_over_previous(kern, static_cast<int>(SHARES > 1 ? tiles * SHARES : tiles < num_sms() ? tiles : num_sms()), kThreads, kMidSmemBytes, SHARES, st, maps, args);
 }
 
 template <typename T, int ACT, bool FEW, bool SAVE>
@@ -1207,10 +1214,7 @@ int launch_mid_act(const MidMaps& maps, const MidArgs& args, int shares, int act
 
 template <typename T>
 int ffn_mid(const void* x, const void* wg, const void* wu, void* h, void* gq, float* gs, void* uq, float* us, int64_t m, int64_t f, int64_t k,
-            int64_t ldx, int act, cudaStream_t st) {
-    MidPlan plan = {kHalf, 1};
-    int rc = mid_plan(m, f, k, gq ? kHalf : 8, &plan);
-    if (rc != TB200_OK) return rc;
+            int64_t ldx, int act, const MidPlan& plan, cudaStream_t st) {
     MidArgs args = {};
     args.h = h;
     args.codes[0] = static_cast<uint8_t*>(gq);
@@ -1222,13 +1226,13 @@ int ffn_mid(const void* x, const void* wg, const void* wu, void* h, void* gq, fl
     args.depth = static_cast<int>(k);
     args.w = plan.w;
     const bool few = m <= kFewRows;
-    args.x_rows = static_cast<int>(few ? (m + 15) / 16 * 16 : (m + 7) / 8 * 8);
+    args.x_rows = static_cast<int>(few ? (m + 15) / 16 * 16 : m < kHalf ? (m + 7) / 8 * 8 : kHalf);
     const int stage = (args.x_rows + 2 * plan.w) * 128;
     const int ring = few ? kMidRing + 4 * kStagingBytes - kFewSums : kMidRing;
     args.stages = ring / stage < kMaxStages ? ring / stage : kMaxStages;
     MidMaps maps;
     memset(&maps, 0, sizeof(maps));
-    rc = map_k<T>(&maps.x, x, m, k, ldx, args.x_rows);
+    int rc = map_k<T>(&maps.x, x, m, k, ldx, args.x_rows);
     if (rc == TB200_OK) rc = map_k<T>(&maps.wg, wg, f, k, k, plan.w);
     if (rc == TB200_OK) rc = map_k<T>(&maps.wu, wu, f, k, k, plan.w);
     if (rc != TB200_OK) return rc;
@@ -1240,15 +1244,16 @@ int ffn_mid(const void* x, const void* wg, const void* wu, void* h, void* gq, fl
 // the least idle at the end.  A wave's time
 // hardly falls with its tiles' width, since a stage takes 0.27 us to issue whatever its width (measured at k = 2048: 12.1 us
 // a wave of 128-wide tiles, 9.8 of 64-wide ones): it goes as the width + 200.
-int pair_width(int64_t m, int64_t f) {
+int pair_width(int64_t m, int64_t f, int64_t* waves) {
     const int64_t pairs = num_sms() / 2, tm = (m + 2 * kHalf - 1) / (2 * kHalf);
     int best = kHalf;
     int64_t least = 0;
     for (int w = kHalf; w >= 64; w -= 16) {
-        const int64_t cost = (tm * ((f + w - 1) / w) + pairs - 1) / pairs * (w + 200);
+        const int64_t n = (tm * ((f + w - 1) / w) + pairs - 1) / pairs, cost = n * (w + 200);
         if (least == 0 || cost < least) {
             least = cost;
             best = w;
+            *waves = n;
         }
     }
     return best;
@@ -1256,8 +1261,7 @@ int pair_width(int64_t m, int64_t f) {
 
 template <typename T>
 int ffn_forward(const void* x, const void* wg, const void* wu, void* h, void* gq, float* gs, void* uq, float* us, int64_t m, int64_t f,
-                int64_t k, int64_t ldx, int act, cudaStream_t st) {
-    const int w = gq ? kHalf : pair_width(m, f);
+                int64_t k, int64_t ldx, int act, int w, cudaStream_t st) {
     FfnMaps<FK_FWD> maps;
     memset(&maps, 0, sizeof(maps));
     int rc = map_k<T>(&maps.a[0], x, m, k, ldx);
@@ -1275,6 +1279,25 @@ int ffn_forward(const void* x, const void* wg, const void* wu, void* h, void* gq
     args.scales[0] = gs;
     args.scales[1] = us;
     return gq ? launch_fwd<T, true>(maps, args, act, st) : launch_fwd<T, false>(maps, args, act, st);
+}
+
+// Up to 128 rows one CTA's accumulator holds them all and narrow tiles share the weights out evenly (1 row of 4096 -> 14336: 40 us
+// against the pair kernel's 70).  Beyond, two CTAs share each weight tile, unless that leaves most of them idle: up to 1024 rows
+// the shorter time by the two models decides (247 rows of 3960 -> 1164: 25 us in pairs, 17 so).  Checkpoints need whole 128-wide
+// blocks: tiles of that width for up to 64 rows, the pair kernel's beyond.
+template <typename T>
+int forward(const void* x, const void* wg, const void* wu, void* h, void* gq, float* gs, void* uq, float* us, int64_t m, int64_t f, int64_t k,
+            int64_t ldx, int act, cudaStream_t st) {
+    int64_t waves = 0;
+    const int w = gq ? kHalf : pair_width(m, f, &waves);
+    if (m <= (gq ? kFewRows : 8 * kHalf)) {
+        MidPlan plan = {kHalf, 1, 0.0f};
+        const int rc = mid_plan(m, f, k, gq ? kHalf : 8, &plan);
+        if (rc != TB200_OK) return rc;
+        const float pair = static_cast<float>(waves) * (static_cast<float>((k + kBK - 1) / kBK) * 0.27f * static_cast<float>(w + 200) / 328.0f + 0.5f) + 3.0f;
+        if (m <= kHalf || plan.time + 1.0f < pair) return ffn_mid<T>(x, wg, wu, h, gq, gs, uq, us, m, f, k, ldx, act, plan, st);
+    }
+    return ffn_forward<T>(x, wg, wu, h, gq, gs, uq, us, m, f, k, ldx, act, w, st);
 }
 
 // ---- the backward pass's shares ----
@@ -1506,14 +1529,8 @@ extern "C" int tb200_ffn_gated(const void* x, const void* wg, const void* wu, vo
     if (!aligned16(x) || !aligned16(wg) || !aligned16(wu)) return fail(TB200_ERR_ALIGN, "ffn_gated: x, wg, wu must be 16-byte aligned");
     if (!to_elements(h, 2) || !to_elements(gs, 4) || !to_elements(us, 4)) return fail(TB200_ERR_ALIGN, "ffn_gated: h, gs, us must be aligned to their elements");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // Up to 128 rows one CTA's accumulator holds them all and narrow tiles share the weights out evenly (1 row of 4096 ->
-    // 14336: 40 us against the pair kernel's 70); beyond, two CTAs share each weight tile.  Checkpoints need whole
-    // 128-wide blocks: tiles of that width for up to 64 rows, the pair kernel's beyond.
-    if (m <= (given ? kFewRows : kHalf))
-        return dtype == TB200_DT_F16 ? ffn_mid<__half>(x, wg, wu, h, gq, gs, uq, us, m, f, k, ldx, act, st)
-                                     : ffn_mid<__nv_bfloat16>(x, wg, wu, h, gq, gs, uq, us, m, f, k, ldx, act, st);
-    return dtype == TB200_DT_F16 ? ffn_forward<__half>(x, wg, wu, h, gq, gs, uq, us, m, f, k, ldx, act, st)
-                                 : ffn_forward<__nv_bfloat16>(x, wg, wu, h, gq, gs, uq, us, m, f, k, ldx, act, st);
+    return dtype == TB200_DT_F16 ? forward<__half>(x, wg, wu, h, gq, gs, uq, us, m, f, k, ldx, act, st)
+                                 : forward<__nv_bfloat16>(x, wg, wu, h, gq, gs, uq, us, m, f, k, ldx, act, st);
 }
 
 extern "C" size_t tb200_ffn_gated_bwd_workspace_bytes(int64_t m, int64_t f, int64_t k, int x_codes) {
