@@ -250,7 +250,7 @@ int tb200_allgather_cols(const void* local, int64_t ld_local, void* const* out_p
  * ------------------------------------------------------------------------------------------- */
 
 /* Codes and scales of x (dtype F32, F16 or BF16), rows ldx elements apart.  Any width, stride and alignment;
- * rows on 32-byte boundaries whose length is a multiple of 32 bytes, and codes on boundaries of 16 (8 for F32), are the faster path. */
+ * rows of whole 16-byte pieces on such boundaries, with codes on boundaries of 8 (4 for F32), are the faster path. */
 int tb200_act_checkpoint_fp8(const void* x, void* q, float* scales, int64_t rows, int64_t cols, int64_t ldx,
                              int dtype, void* stream);
 /* out[r, c] = code * scale in `dtype` (F32, F16 or BF16), [rows, cols] contiguous.  A product beyond the type's

@@ -1,5 +1,5 @@
 """cuda backend of ffn_gated_bwd (tb200_ffn_gated_bwd): one streaming kernel makes the gradients of both projections
-from the 8-bit checkpoints, one tcgen05 kernel the gradient of x, one those of both weights."""
+from the 8-bit checkpoints, one tcgen05 kernel the gradients of x and of both weights (few rows and large weights: two)."""
 import torch
 
 from tilebench_b200 import native
