@@ -233,29 +233,19 @@ __global__ void __launch_bounds__(kThreads) tb200_k_act_restore(const uint8_t* _
 // Stores of codes are of aligned words too, of the previous lane's last codes and the lane's own.  Loads that reach outside
 // the tensor and stores that reach outside the span are made byte by byte.
 
-// The piece at byte `off` behind base (base + off is aligned); bytes outside [lo, hi) come as zeros.
+// N words at p, on a boundary of their size, of which the first n bytes are there; the others come as zeros.
 template <int N>
-__device__ __forceinline__ void load_piece(const uint8_t* base, int off, int lo, int hi, uint32_t (&r)[N]) {
-    if (off >= lo && off + 4 * N <= hi) {
-        if constexpr (N == 4) {
-            const uint4 v = __ldcs(reinterpret_cast<const uint4*>(base + off));
-            r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
-        } else if constexpr (N == 2) {
-            const uint2 v = __ldcs(reinterpret_cast<const uint2*>(base + off));
-            r[0] = v.x; r[1] = v.y;
-        } else {
-            r[0] = __ldcs(reinterpret_cast<const uint32_t*>(base + off));
-        }
+__device__ __forceinline__ void load_piece(const uint8_t* p, int n, uint32_t (&r)[N]) {
+    if (n >= 4 * N) {
+        load_codes<N>(p, r);
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) r[i] = 0;
-        if (off + 4 * N > lo && off < hi) {
 #pragma unroll 1
-            for (int i = max(0, lo - off); i < 4 * N && off + i < hi; ++i) {
-                const uint32_t byte = static_cast<uint32_t>(base[off + i]) << (8 * (i & 3));
+        for (int i = 0; i < n; ++i) {
+            const uint32_t byte = static_cast<uint32_t>(p[i]) << (8 * (i & 3));
 #pragma unroll
-                for (int w = 0; w < N; ++w) r[w] |= i / 4 == w ? byte : 0;
-            }
+            for (int w = 0; w < N; ++w) r[w] |= i / 4 == w ? byte : 0;
         }
     }
 }
@@ -374,7 +364,7 @@ __global__ void __launch_bounds__(kThreads) tb200_k_act_restore_across(const uin
         for (int j = 0; j < U; ++j) {
             const int64_t at = w0 + (j * 32 + lane) * E;
             if (at >= total) continue;
-            load_piece<E / 4>(q + at, 0, 0, static_cast<int>(min(total - at, static_cast<int64_t>(E))), c[j]);
+            load_piece<E / 4>(q + at, static_cast<int>(min(total - at, static_cast<int64_t>(E))), c[j]);
             uint32_t col = col0 + (j * 32 + lane) * E, row = 0;
             if (col >= width) {
                 row = width >= kWarpCols ? 1 : col / width;      // 1: col0 < width, and the warp's share is no wider
@@ -696,6 +686,14 @@ int launch_gated_act(const void* dh, const void* gq, const float* gs, const void
     }
 }
 
+// ldo: row pitch of out, cols unless rows of out and of q are whole 16-byte and 8-byte pieces on such boundaries.
+int launch_act_restore(const void* q, const float* scales, void* out, int dtype, int64_t rows, int64_t cols, int64_t ldo, cudaStream_t st) {
+    const uint8_t* c = static_cast<const uint8_t*>(q);
+    if (dtype == TB200_DT_F32) return launch_restore<float>(c, scales, static_cast<float*>(out), rows, cols, ldo, st);
+    if (dtype == TB200_DT_F16) return launch_restore<__half>(c, scales, static_cast<__half*>(out), rows, cols, ldo, st);
+    return launch_restore<__nv_bfloat16>(c, scales, static_cast<__nv_bfloat16*>(out), rows, cols, ldo, st);
+}
+
 int check_sizes(const char* what, int64_t rows, int64_t cols) {
     if (rows < 0 || cols <= 0) return fail(TB200_ERR_ARG, "%s: rows=%lld cols=%lld (rows >= 0, cols > 0)", what, (long long)rows, (long long)cols);
     if (cols > (1ll << 31) || rows > (1ll << 40) / cols) return fail(TB200_ERR_UNSUPPORTED, "%s: rows=%lld cols=%lld is too large", what, (long long)rows, (long long)cols);
@@ -723,13 +721,6 @@ int launch_gated_act_bwd(const void* dh, const void* gq, const float* gs, const 
     }
     return dtype == TB200_DT_F16 ? launch_gated_act<__half>(dh, gq, gs, uq, us, dg, du, m, f, ldg, job, act, st)
                                  : launch_gated_act<__nv_bfloat16>(dh, gq, gs, uq, us, dg, du, m, f, ldg, job, act, st);
-}
-
-int launch_act_restore(const void* q, const float* scales, void* out, int dtype, int64_t rows, int64_t cols, int64_t ldo, cudaStream_t st) {
-    const uint8_t* c = static_cast<const uint8_t*>(q);
-    if (dtype == TB200_DT_F32) return launch_restore<float>(c, scales, static_cast<float*>(out), rows, cols, ldo, st);
-    if (dtype == TB200_DT_F16) return launch_restore<__half>(c, scales, static_cast<__half*>(out), rows, cols, ldo, st);
-    return launch_restore<__nv_bfloat16>(c, scales, static_cast<__nv_bfloat16*>(out), rows, cols, ldo, st);
 }
 
 }  // namespace tb200

@@ -60,12 +60,10 @@ __device__ __forceinline__ float act_held(float v, float top) {
 template <typename T> struct ActType;
 template <> struct ActType<float> {
     static constexpr float kTop = FLT_MAX;
-    static __device__ __forceinline__ float load(float v) { return v; }
     static __device__ __forceinline__ float store(float v) { return v; }
 };
 template <> struct ActType<__half> {
     static constexpr float kTop = 65504.0f;
-    static __device__ __forceinline__ float load(__half v) { return __half2float(v); }
     static __device__ __forceinline__ __half store(float v) { return __float2half_rn(v); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __half2 h = __floats2half2_rn(a, b);
@@ -75,7 +73,6 @@ template <> struct ActType<__half> {
 };
 template <> struct ActType<__nv_bfloat16> {
     static constexpr float kTop = 3.38953138925153547590470800371487866880e+38f;
-    static __device__ __forceinline__ float load(__nv_bfloat16 v) { return __bfloat162float(v); }
     static __device__ __forceinline__ __nv_bfloat16 store(float v) { return __float2bfloat16_rn(v); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
@@ -193,7 +190,5 @@ int launch_over_previous(void (*kern)(Maps, Args), int grid, int block, int smem
 int launch_gated_act_bwd(const void* dh, const void* gq, const float* gs, const void* uq, const float* us, void* dg, void* du,
                          int64_t m, int64_t f, int64_t ldg, const void* xq, const float* xs, void* x, int64_t k, int64_t ldx, int act, int dtype,
                          cudaStream_t st);
-// ldo: row pitch of out, cols unless rows of out and of q are whole 16-byte and 8-byte pieces on such boundaries.
-int launch_act_restore(const void* q, const float* scales, void* out, int dtype, int64_t rows, int64_t cols, int64_t ldo, cudaStream_t st);
 
 }  // namespace tb200

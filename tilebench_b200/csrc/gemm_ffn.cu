@@ -480,7 +480,7 @@ tb200_k_ffn_pair(const __grid_constant__ FfnMaps<KIND> maps, const __grid_consta
                     flush<uint8_t, 8>(buf, 8, p.codes[1] + to, p.f, r8, rows, cols, lane);
                     quarter_sync(quarter);
                 }
-            } else if (p.shares[it.dw] > 1) {                    // partial sums in 32 bits, 64 columns at a time
+            } else if (KIND == FK_BWD && p.shares[it.dw] > 1) {                    // partial sums in 32 bits, 64 columns at a time
                 float* dst = p.sums[it.dw] + (static_cast<int64_t>(it.dw ? 2 * it.share + it.sel : it.share) * all_rows + row0) * p.k + col0;
                 if (part == 0 && lane == 0) tma_store_wait_read<0>();     // the item before may have been stored by TMA
                 quarter_sync(quarter);
