@@ -271,7 +271,8 @@ int tb200_ffn_gated(const void* x, const void* wg, const void* wu, void* h, void
 size_t tb200_ffn_gated_bwd_workspace_bytes(int64_t m, int64_t f, int64_t k, int x_codes);
 /*
  * Gradients of that block from dh [m, f] and the 8-bit forms of g and u:
- *   dg = dh * u * f'(g), du = dh * f(g), rounded to dtype (a value beyond fp16's range becomes infinite there)
+ *   dg = dh * u * f'(g), du = dh * f(g), rounded to dtype; in F16 they are held times one power of two, taken from the largest
+ *                    finite |dh| and scale, so that none overflows and only what is 2^-27 of the bound or less loses bits
  *   dx = dg Wg + du Wu [m, k],  dWg = dg^T x [f, k],  dWu = du^T x [f, k], of dtype, written (not accumulated)
  * x is the block's input: of dtype with rows ldx elements apart (xs NULL), or its e4m3 codes with scales xs.
  * k and ldx must be multiples of 8; wg, wu, dx, dwg, dwu (and x unless in 8 bits) 16-byte aligned; any m and f.

@@ -7,6 +7,7 @@ namespace tb200 {
 namespace {
 
 constexpr int kThreads = 256;
+template <typename T> constexpr bool kRanged = ActType<T>::kTop < 1e5f;      // fp16, whose dg and du are held times a power of two
 
 __device__ __forceinline__ void load_once(const void* p, uint32_t (&r)[8]) {     // 32 bytes, read once
     asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -460,14 +461,98 @@ __device__ __forceinline__ void restore_job(const RestoreJob& job, uint32_t cta)
     }
 }
 
+// ---- the power of two of an fp16 backward pass ------------------------------------------------------------------------
+// Largest finite |dh| (its bits, in the upper half of a word) and largest finite |scale| (the upper half of its bits, in the lower) of a
+// CTA's share, written behind row blockIdx.x of du: there are at most m CTAs.  Bound by reading dh once, 2 bytes of the 16 or so that a
+// number of dh costs in all, and by a launch more: a captured backward pass in fp16 takes 5 us longer for it at 1023 rows of 1048 x 2731
+// (39 -> 45) and at 4 of 2048 x 5632 (33 -> 38), 7 at 64 of 4096 x 14336 (108 -> 115).  The launch overlaps with the end of the
+// kernel before, so nothing is read through the read-only path; the next kernel may begin once that one is complete.
+__device__ __forceinline__ void load_plain(const void* p, uint32_t (&r)[8]) {    // 32 bytes
+    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "l"(p) : "memory");
+}
+constexpr int kRangeThreads = 512, kMostMaxima = kThreads;       // one for each thread that reads them
+template <int WARPS>
+__device__ __forceinline__ uint32_t block_max2(uint32_t v, uint32_t* shared) {                   // of both halves, in all threads
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = __vmaxu2(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) v = __vmaxu2(v, shared[i]);
+    return v;
+}
+__global__ void __launch_bounds__(kRangeThreads) tb200_k_ffn_grad_range(const __half* dh, int64_t n, const float* gs, const float* us, int64_t blocks, uint32_t* maxima,
+                                                              int64_t pitch) {
+    wait_for_previous();
+    let_next_begin();
+    __shared__ uint32_t shared[kRangeThreads / 32];
+    constexpr int E = 16, U = 4;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kRangeThreads + threadIdx.x, step = static_cast<int64_t>(gridDim.x) * kRangeThreads;
+    // 32-byte pieces between the first such boundary and the last; up to 15 numbers before and 15 behind
+    const int64_t skip = static_cast<int64_t>((32 - (reinterpret_cast<uintptr_t>(dh) & 31)) & 31) / 2, head = skip < n ? skip : n;
+    const int64_t pieces = (n - head) / E, tail = head + pieces * E;
+    const uint16_t* const bits = reinterpret_cast<const uint16_t*>(dh);
+    uint32_t top = 0;                                            // of even and odd numbers
+    auto take = [&](uint32_t w) {
+        w &= 0x7FFF7FFFu;
+        const uint32_t most = 0x7BFF7BFFu;                       // infinities and NaN do not count
+        top = __vmaxu2(top, w & __hle2_mask(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(&most)));
+    };
+    // the first of each kind on the way together
+    const uint32_t before = first < head ? __ldcg(bits + first) : 0, behind = tail + first < n ? __ldcg(bits + tail + first) : 0;
+    const float g0 = first < blocks ? __ldcg(gs + first) : 0.0f, u0 = first < blocks ? __ldcg(us + first) : 0.0f;
+    for (int64_t i0 = first; i0 < pieces; i0 += U * step) {
+        uint32_t w[U][8];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            if (i0 + j * step < pieces) {
+                load_plain(dh + head + (i0 + j * step) * E, w[j]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[j][e] = 0;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) take(w[j][e]);
+    }
+    take(before);
+    take(behind);
+    float size = fmaxf(act_size(g0), act_size(u0));
+    for (int64_t i = first + step; i < blocks; i += step) size = fmaxf(size, fmaxf(act_size(__ldcg(gs + i)), act_size(__ldcg(us + i))));
+    top = max(top & 0xFFFFu, top >> 16);
+    const uint32_t all = block_max2<kRangeThreads / 32>(top << 16 | __float_as_uint(size) >> 16, shared);
+    if (threadIdx.x == 0) maxima[blockIdx.x * pitch] = all;
+}
+// The power of two from those maxima, the same in all threads; the inverse is left at `inverse` by CTA 0.
+struct GradRange { const uint32_t* maxima; float* inverse; int count; uint32_t pitch; };
+__device__ __forceinline__ float grad_power(const GradRange& r) {
+    __shared__ uint32_t shared[kThreads / 32];
+    wait_for_previous();                                         // for the maxima: this kernel's launch overlaps with that one's end
+    const int i = threadIdx.x;
+    const uint32_t v = block_max2<kThreads / 32>(i < r.count ? __ldcg(r.maxima + static_cast<int64_t>(i) * r.pitch) : 0, shared);
+    // 2^a <= |dh| < 2^(a + 1), 2^b <= scale < 2^(b + 1): the bound is below 2^(a + b + 11)
+    const float largest = __half2float(__ushort_as_half(static_cast<unsigned short>(v >> 16)));
+    const int a = static_cast<int>(__float_as_uint(largest) >> 23) - 127, b = static_cast<int>((v & 0xFFFFu) >> 7) - 127;
+    const int e = min(max(15 - (a + b + 11), -100), 100);        // both powers stay far within fp32's range
+    if (blockIdx.x == 0 && threadIdx.x == 0) *r.inverse = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    return __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+}
+
 // dg = dh * u * f'(g), du = dh * f(g) for 8 numbers of a lane, in fp32 and rounded once to T: they are operands of 16 bits in the
-// products that follow (half a step, 2^-9 of the value in bf16, which the products' sums average out).
+// products that follow (half a step, 2^-9 of the value in bf16, which the products' sums average out).  dh comes times `power` in fp16.
 template <typename T, int ACT>
-__device__ __forceinline__ void gated_bwd8(const uint32_t (&d)[4], const uint32_t (&cg)[2], const uint32_t (&cu)[2], float sg, float su,
+__device__ __forceinline__ void gated_bwd8(const uint32_t (&d)[4], const uint32_t (&cg)[2], const uint32_t (&cu)[2], float sg, float su, float power,
                                            uint4& dg, uint4& du) {
     float e[8], g[8], u[8];
     uint32_t og[4], ou[4];
     numbers<T, 4>(d, e);
+    if constexpr (kRanged<T>) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] *= power;
+    }
     decode<8>(cg, sg, FLT_MAX, g);
     decode<8>(cu, su, FLT_MAX, u);
 #pragma unroll
@@ -487,8 +572,10 @@ template <typename T, int ACT, int U>
 __global__ void __launch_bounds__(kThreads) tb200_k_ffn_gated_bwd(const uint4* __restrict__ dh, const uint2* __restrict__ gq, const float* __restrict__ gs,
                                                         const uint2* __restrict__ uq, const float* __restrict__ us, uint4* __restrict__ dg,
                                                         uint4* __restrict__ du, uint32_t total, uint32_t per_row, uint32_t out_row, uint32_t nblk,
-                                                        const RestoreJob job) {
+                                                        const RestoreJob job, const GradRange range) {
     let_next_begin();
+    float power = 1.0f;
+    if constexpr (kRanged<T>) power = grad_power(range);
     const uint32_t ctas = gridDim.x - job.ctas, step = ctas * kThreads;
     if (blockIdx.x >= ctas) return restore_job<T>(job, blockIdx.x - ctas);
     for (uint64_t i0 = blockIdx.x * kThreads + threadIdx.x; i0 < total; i0 += U * step) {
@@ -515,7 +602,7 @@ __global__ void __launch_bounds__(kThreads) tb200_k_ffn_gated_bwd(const uint4* _
             if (i < total) {
                 const uint32_t dw[4] = {d[j].x, d[j].y, d[j].z, d[j].w}, gw[2] = {cg[j].x, cg[j].y}, uw[2] = {cu[j].x, cu[j].y};
                 uint4 a, b;
-                gated_bwd8<T, ACT>(dw, gw, uw, sg[j], su[j], a, b);
+                gated_bwd8<T, ACT>(dw, gw, uw, sg[j], su[j], power, a, b);
                 dg[to[j]] = a;
                 du[to[j]] = b;
             }
@@ -528,8 +615,10 @@ template <typename T, int ACT>
 __global__ void __launch_bounds__(kThreads) tb200_k_ffn_gated_bwd_any(const T* __restrict__ dh, const uint8_t* __restrict__ gq, const float* __restrict__ gs,
                                                             const uint8_t* __restrict__ uq, const float* __restrict__ us, T* __restrict__ dg,
                                                             T* __restrict__ du, int64_t spans, uint32_t per_row, int width, int64_t m, int64_t f,
-                                                            int64_t ldg, uint32_t nblk, const RestoreJob job) {
+                                                            int64_t ldg, uint32_t nblk, const RestoreJob job, const GradRange range) {
     let_next_begin();
+    float power = 1.0f;
+    if constexpr (kRanged<T>) power = grad_power(range);
     const uint32_t ctas = gridDim.x - job.ctas;
     if (blockIdx.x >= ctas) return restore_job<T>(job, blockIdx.x - ctas);
     static_assert(sizeof(T) == 2, "8 numbers of 16 bits and 8 codes per lane");
@@ -567,7 +656,7 @@ __global__ void __launch_bounds__(kThreads) tb200_k_ffn_gated_bwd_any(const T* _
             if (col + kCols < n) fetch(col + kCols);
             if (here) {
                 uint4 a, b;
-                gated_bwd8<T, ACT>(d, cg, cu, sg, su, a, b);
+                gated_bwd8<T, ACT>(d, cg, cu, sg, su, power, a, b);
                 *reinterpret_cast<uint4*>(to_g + at) = a;        // the row's padding takes what is behind its last column
                 *reinterpret_cast<uint4*>(to_u + at) = b;
             }
@@ -655,24 +744,47 @@ int launch_restore(const uint8_t* q, const float* scales, T* out, int64_t rows, 
     return TB200_OK;
 }
 
+template <typename Kernel, typename... Args>
+int launch_over(bool over_previous, Kernel kern, int grid, int threads, cudaStream_t st, const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+    cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = over_previous ? 1 : 0;
+    TB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, args...));
+    return TB200_OK;
+}
+
 template <typename T, int ACT>
 int launch_gated(const void* dh, const void* gq, const float* gs, const void* uq, const float* us, void* dg, void* du, int64_t m, int64_t f,
                  int64_t ldg, const RestoreJob& job, cudaStream_t st) {
     const uint32_t nblk = static_cast<uint32_t>((f + kActBlock - 1) / kActBlock);
+    GradRange range = {};
+    if constexpr (kRanged<T>) {
+        // one piece per thread, as far as there are rows to leave the maxima behind and threads to read them
+        const int64_t wanted = (m * f + kRangeThreads * 16 - 1) / (kRangeThreads * 16), most = m < kMostMaxima ? m : kMostMaxima;
+        uint32_t* const maxima = behind_row<uint32_t>(du, ldg);
+        range = {maxima, behind_row<float>(dg, ldg), static_cast<int>(wanted < most ? wanted : most), static_cast<uint32_t>(ldg / 2)};
+        const int rc = launch_over(true, tb200_k_ffn_grad_range, range.count, kRangeThreads, st, static_cast<const __half*>(dh), m * f, gs, us,
+                                   m * static_cast<int64_t>(nblk), maxima, ldg / 2);
+        if (rc != TB200_OK) return rc;
+    }
     if (f % 8 == 0 && aligned_to(16, dh, 0) && aligned_to(8, gq, 0) && aligned_to(8, uq, 0) && m * (ldg / 8) <= 0xFFFFFFFFll) {
         const int64_t total = m * (f / 8);
         constexpr int U = 2;
-        tb200_k_ffn_gated_bwd<T, ACT, U><<<capped((total + kThreads * U - 1) / (kThreads * U), 8) + job.ctas, kThreads, 0, st>>>(
-            static_cast<const uint4*>(dh), static_cast<const uint2*>(gq), gs, static_cast<const uint2*>(uq), us, static_cast<uint4*>(dg),
-            static_cast<uint4*>(du), static_cast<uint32_t>(total), static_cast<uint32_t>(f / 8), static_cast<uint32_t>(ldg / 8), nblk, job);
-    } else {
-        const Spans sp = spans_of(m, f, 256);
-        tb200_k_ffn_gated_bwd_any<T, ACT><<<capped((sp.count + 7) / 8, 8) + job.ctas, kThreads, 0, st>>>(
-            static_cast<const T*>(dh), static_cast<const uint8_t*>(gq), gs, static_cast<const uint8_t*>(uq), us, static_cast<T*>(dg),
-            static_cast<T*>(du), sp.count, sp.per_row, sp.width, m, f, ldg, nblk, job);
+        return launch_over(kRanged<T>, tb200_k_ffn_gated_bwd<T, ACT, U>, capped((total + kThreads * U - 1) / (kThreads * U), 8) + job.ctas, kThreads, st,
+                           static_cast<const uint4*>(dh), static_cast<const uint2*>(gq), gs, static_cast<const uint2*>(uq), us,
+                           static_cast<uint4*>(dg), static_cast<uint4*>(du), static_cast<uint32_t>(total), static_cast<uint32_t>(f / 8),
+                           static_cast<uint32_t>(ldg / 8), nblk, job, range);
     }
-    TB200_CUDA_TRY(cudaGetLastError());
-    return TB200_OK;
+    const Spans sp = spans_of(m, f, 256);
+    return launch_over(kRanged<T>, tb200_k_ffn_gated_bwd_any<T, ACT>, capped((sp.count + 7) / 8, 8) + job.ctas, kThreads, st, static_cast<const T*>(dh),
+                       static_cast<const uint8_t*>(gq), gs, static_cast<const uint8_t*>(uq), us, static_cast<T*>(dg), static_cast<T*>(du),
+                       sp.count, sp.per_row, sp.width, m, f, ldg, nblk, job, range);
 }
 
 template <typename T>

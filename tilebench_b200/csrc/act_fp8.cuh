@@ -184,7 +184,23 @@ int launch_over_previous(void (*kern)(Maps, Args), int grid, int block, int smem
 #endif
 
 // ---- launchers shared between the files of the feed-forward block ----------------------------------------------
-// The backward pass's two intermediates, dg = dh * u * f'(g) and du = dh * f(g) with row pitch ldg; and, where xq is given, the
+// dg and du lie in rows of whole 128-byte lines: a copy of 128 bytes that begins elsewhere moves a fifth sector (12756 rows of
+// 1264 x 19937: 2547 us with rows of 39888 bytes, 2282 so).
+//
+// In fp16 they are held times a power of two, the same for all of them: dh times projections may be far below fp16's normal numbers
+// (with dh of 1e-6 half of the bits of the weights' gradients were lost, which are normal numbers themselves) or above its largest.  The
+// power brings the bound max|dh| * 512 * max(scale of g or u) to between 2^13 and 2^15 (|u| <= 448 s, |f(g)| <= |g|, |f'| <= 1.13, and
+// 448 * 1.13 < 512), over the finite values; what is within 2^-27 of the bound keeps all of its bits.  Products carry it exactly, and
+// the factor that takes it off again is applied to their 32-bit sums.  That factor lies in the last four bytes of dg's first row; behind du's rows lie the
+// maxima that it comes from.  So an fp16 row has room for four bytes behind its last whole piece of 8 numbers.
+constexpr int64_t grad_pitch(int64_t f, int dtype) {
+    return ((dtype == TB200_DT_F16 ? (f + 7) / 8 * 8 + 2 : f) + 63) / 64 * 64;
+}
+template <typename P>
+P* behind_row(void* grads, int64_t ldg) { return reinterpret_cast<P*>(static_cast<uint8_t*>(grads) + 2 * ldg - sizeof(P)); }
+
+// The backward pass's two intermediates, dg = dh * u * f'(g) and du = dh * f(g) with row pitch ldg = grad_pitch(f, dtype), in fp16 times
+// a power of two whose inverse is left at behind_row<float>(dg, ldg); and, where xq is given, the
 // block's input [m, k] restored from its 8-bit form with row pitch ldx (k and ldx multiples of 8; ldx = k unless xq lies on an 8-byte
 // boundary).
 int launch_gated_act_bwd(const void* dh, const void* gq, const float* gs, const void* uq, const float* us, void* dg, void* du,

@@ -62,6 +62,7 @@ struct FfnArgs {
     float* sums[2];                              // backward, in shares: partial sums of dx [shares, m, k], of dw [shares, 2, f, k]
     int shares[2];                               // of the contraction of dx, and of dw; 0: not in this launch
     int early;                                   // backward, see item_at
+    const float* factor;                         // backward in fp16: of the results, see grad_pitch
 };
 
 __device__ __forceinline__ uint64_t desc_mn(uint32_t smem_addr) {       // MN-major, 128-byte swizzle
@@ -194,6 +195,22 @@ template <int ACT>
 __device__ __forceinline__ void gated32(uint32_t (&g)[32], const uint32_t (&u)[32]) {       // h in the place of g
 #pragma unroll
     for (int i = 0; i < 32; ++i) g[i] = __float_as_uint(gate_value<ACT>(__uint_as_float(g[i])) * __uint_as_float(u[i]));
+}
+
+// The factor of an fp16 backward pass's results, which are then rounded; nothing in bf16.
+template <typename T>
+constexpr bool kFactor = ActType<T>::kTop < 1e5f;
+template <typename T>
+__device__ __forceinline__ float factor_of(const float* p) {
+    if constexpr (kFactor<T>) return __ldcg(p);
+    else return 1.0f;
+}
+template <typename T, int N>
+__device__ __forceinline__ void times(uint32_t (&v)[N], float factor) {
+    if constexpr (kFactor<T>) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * factor);
+    }
 }
 
 // First step of share i of n.  (At most 2^25 steps and 16 shares.)
@@ -397,6 +414,7 @@ tb200_k_ffn_pair(const __grid_constant__ FfnMaps<KIND> maps, const __grid_consta
         const int quarter = (warp - 4) & 3, part = (warp - 4) >> 2, r8 = 8 * part;
         uint8_t* buf = staging + quarter * kStaging;
         const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+        const float factor = KIND == FK_FWD ? 1.0f : factor_of<T>(p.factor);
         uint32_t cnt = 0;
         bool ok = true;
         for (;; ++cnt) {
@@ -511,6 +529,7 @@ tb200_k_ffn_pair(const __grid_constant__ FfnMaps<KIND> maps, const __grid_consta
                     release();
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
+                        times<T>(v[c], factor);
                         uint8_t* area = buf + c % kPlaces * (kStagingBytes / 2);
                         if (issuer) tma_store_wait_read<kPlaces - 1>();   // all but the other places'
                         quarter_sync(quarter);
@@ -536,6 +555,7 @@ tb200_k_ffn_pair(const __grid_constant__ FfnMaps<KIND> maps, const __grid_consta
                     release();
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
+                        times<T>(v[c], factor);
                         stage32<T>(buf, lane, 4 * part, v[c]);
                         quarter_sync(quarter);
                         flush<T, 16>(buf, 0, static_cast<T*>(p.out[which]) + static_cast<int64_t>(row0) * p.k + col0 + c * kHalf, p.k, r8, rows, cols - c * kHalf, lane);
@@ -903,6 +923,7 @@ struct DxFewArgs {
     float* sums;                                 // with more
     int m, k, depth, shares;
     int rows, stages;                            // of dg per copy: m rounded up to 16; in shared memory
+    const float* factor;                         // in fp16: of dx, where there is one share
 };
 constexpr int kDxCols = kFewRows;                     // columns of an accumulator
 constexpr int kDxRing = 192 * 1024;
@@ -1018,6 +1039,7 @@ __global__ void __launch_bounds__(kDxThreads, 1) tb200_k_ffn_dx_few(const __grid
         // ---------------- epilogue: a lane has one column of dx, a register one row ----------------
         const int quarter = warp - 4;
         const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+        const float factor = factor_of<T>(p.factor);
         uint32_t cnt = 0;
         bool ok = true;
         for (int t = blockIdx.x; t < items && ok; t += gridDim.x, ++cnt) {
@@ -1035,7 +1057,7 @@ __global__ void __launch_bounds__(kDxThreads, 1) tb200_k_ffn_dx_few(const __grid
                     for (int i = 0; i < 16; ++i) {
                         if (r0 + i < p.m) {
                             if (p.shares > 1) p.sums[(static_cast<int64_t>(share) * p.m + r0 + i) * p.k + col] = __uint_as_float(v[i]);
-                            else static_cast<T*>(p.dx)[static_cast<int64_t>(r0 + i) * p.k + col] = ActType<T>::store(__uint_as_float(v[i]));
+                            else static_cast<T*>(p.dx)[static_cast<int64_t>(r0 + i) * p.k + col] = ActType<T>::store(__uint_as_float(v[i]) * factor);
                         }
                     }
                 }
@@ -1380,12 +1402,13 @@ BwdPlan bwd_plan(int64_t m, int64_t f, int64_t k) {
 // out = the sum of `splits` arrays of n8 pieces of 8 numbers that lie `stride8` pieces apart, in order; 8 numbers per thread.  One
 // result per row of the grid.
 struct SumJob { const float4* sums; uint4* out; int64_t n8, stride8; int splits; };
-struct SumJobs { SumJob job[3]; };
+struct SumJobs { SumJob job[3]; const float* factor; };         // factor: in fp16, of the results
 template <typename T>
 __global__ void __launch_bounds__(256) tb200_k_ffn_sum_shares(const __grid_constant__ SumJobs jobs) {
     let_next_begin();
     const SumJob& q = jobs.job[blockIdx.y];
     const float4* const __restrict__ sums = q.sums;
+    const float factor = factor_of<T>(jobs.factor);
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < q.n8; i += static_cast<int64_t>(gridDim.x) * 256) {
         float4 a = sums[2 * i], b = sums[2 * i + 1];
 #pragma unroll 4
@@ -1394,13 +1417,17 @@ __global__ void __launch_bounds__(256) tb200_k_ffn_sum_shares(const __grid_const
             a.x += c.x; a.y += c.y; a.z += c.z; a.w += c.w;
             b.x += d.x; b.y += d.y; b.z += d.z; b.w += d.w;
         }
+        if constexpr (kFactor<T>) {
+            a.x *= factor; a.y *= factor; a.z *= factor; a.w *= factor;
+            b.x *= factor; b.y *= factor; b.z *= factor; b.w *= factor;
+        }
         q.out[i] = make_uint4(ActType<T>::pack(a.x, a.y), ActType<T>::pack(a.z, a.w), ActType<T>::pack(b.x, b.y), ActType<T>::pack(b.z, b.w));
     }
 }
 
 template <typename T>
-int dx_few(const void* dg, const void* du, int64_t ldg, const void* wg, const void* wu, void* dx, float* sums, int splits, int64_t m, int64_t f,
-           int64_t k, cudaStream_t st) {
+int dx_few(const void* dg, const void* du, int64_t ldg, const float* factor, const void* wg, const void* wu, void* dx, float* sums, int splits,
+           int64_t m, int64_t f, int64_t k, cudaStream_t st) {
     auto kern = tb200_k_ffn_dx_few<T>;
     static PerDeviceInt attr_set;
     int rc = ensure_max_smem(attr_set, reinterpret_cast<const void*>(kern), kDxSmemBytes);
@@ -1413,6 +1440,7 @@ int dx_few(const void* dg, const void* du, int64_t ldg, const void* wg, const vo
     args.depth = static_cast<int>(f);
     args.shares = splits;
     args.rows = static_cast<int>((m + 15) / 16 * 16);
+    args.factor = factor;
     const int stage = kOperandBytes + args.rows * 128;
     args.stages = kDxRing / stage < kMaxStages ? kDxRing / stage : kMaxStages;
     DxFewMaps maps;
@@ -1426,14 +1454,15 @@ int dx_few(const void* dg, const void* du, int64_t ldg, const void* wg, const vo
     return launch_over_previous(kern, static_cast<int>(items < num_sms() ? items : num_sms()), kDxThreads, kDxSmemBytes, 1, st, maps, args);
 }
 
-// dg, du: [m, ldg]; x: [m, k]; sums: room for the plan's arrays of dx [m, k], then for those of dw [2, f, k], where they are more than 1
+// dg, du: [m, ldg], in fp16 with the results' factor behind dg's first row; x: [m, k]; sums: room for the plan's arrays of dx [m, k], then for those of dw [2, f, k], where they are more than 1
 template <typename T>
-int ffn_products_bwd(const void* dg, const void* du, int64_t ldg, const void* x, int64_t ldx, const void* wg, const void* wu, void* dx, void* dwg,
+int ffn_products_bwd(void* dg, const void* du, int64_t ldg, const void* x, int64_t ldx, const void* wg, const void* wu, void* dx, void* dwg,
                      void* dwu, float* sums, int64_t m, int64_t f, int64_t k, cudaStream_t st) {
     const BwdPlan plan = bwd_plan(m, f, k);
     const bool few = dx_alone(m, f, k);
+    const float* const factor = kFactor<T> ? behind_row<float>(dg, ldg) : nullptr;
     float* const sums_w = sums + (plan.dx > 1 ? plan.dx * m * k : 0);
-    int rc = few ? dx_few<T>(dg, du, ldg, wg, wu, dx, sums, plan.dx, m, f, k, st) : TB200_OK;
+    int rc = few ? dx_few<T>(dg, du, ldg, factor, wg, wu, dx, sums, plan.dx, m, f, k, st) : TB200_OK;
     FfnBwdMaps maps;
     memset(&maps, 0, sizeof(maps));
     const void* const grads[2] = {dg, du};
@@ -1460,6 +1489,7 @@ int ffn_products_bwd(const void* dg, const void* du, int64_t ldg, const void* x,
     args.shares[0] = plan.dx;
     args.shares[1] = plan.dw;
     args.early = plan.early;
+    args.factor = factor;
     const int64_t tn = (k + 2 * kHalf - 1) / (2 * kHalf);
     const int64_t items_x = plan.dx * ((m + 2 * kHalf - 1) / (2 * kHalf)) * tn, items_w = plan.dw * 2 * ((f + 2 * kHalf - 1) / (2 * kHalf)) * tn;
     if (few) {
@@ -1475,6 +1505,7 @@ int ffn_products_bwd(const void* dg, const void* du, int64_t ldg, const void* x,
     if (rc != TB200_OK) return rc;
 
     SumJobs jobs = {};
+    jobs.factor = factor;
     int n = 0;
     int64_t most = 0;
     auto add = [&](const float* from, void* to, int64_t count, int64_t stride, int splits) {
@@ -1494,9 +1525,8 @@ int ffn_products_bwd(const void* dg, const void* du, int64_t ldg, const void* x,
 
 bool to_elements(const void* p, uintptr_t size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
 constexpr int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
-// Rows of dg, du and a restored x begin on 128-byte boundaries: a copy of 128 bytes that begins elsewhere moves a fifth sector
-// (12756 rows of 1264 x 19937: 2547 us with rows of dg and du of 39888 bytes, 2282 so).
-int64_t pitch_of(int64_t f) { return round_up(f, 64); }
+int64_t x_pitch(int64_t k) { return round_up(k, 64); }          // of a restored x: whole 128-byte lines, as for dg and du
+int64_t grad_bytes(int64_t m, int64_t f, int dtype) { return round_up(m * grad_pitch(f, dtype) * 2, 256); }
 
 int check_common(const char* what, int64_t m, int64_t f, int64_t k, int act, int dtype) {
     if (m < 0 || f <= 0 || k <= 0)
@@ -1536,7 +1566,7 @@ extern "C" int tb200_ffn_gated(const void* x, const void* wg, const void* wu, vo
 extern "C" size_t tb200_ffn_gated_bwd_workspace_bytes(int64_t m, int64_t f, int64_t k, int x_codes) {
     if (m <= 0 || f <= 0 || k <= 0) return 0;
     const BwdPlan plan = bwd_plan(m, f, k);
-    return static_cast<size_t>(2 * round_up(m * pitch_of(f) * 2, 256) + (x_codes ? round_up(m * pitch_of(k) * 2, 256) : 0) +
+    return static_cast<size_t>(2 * grad_bytes(m, f, TB200_DT_F16) + (x_codes ? round_up(m * x_pitch(k) * 2, 256) : 0) +     // no less than in bf16
                                (plan.dx > 1 ? plan.dx * m * k * 4 : 0) + (plan.dw > 1 ? plan.dw * 2 * f * k * 4 : 0));
 }
 
@@ -1565,13 +1595,13 @@ extern "C" int tb200_ffn_gated_bwd(const void* dh, const void* wg, const void* w
     const size_t need = tb200_ffn_gated_bwd_workspace_bytes(m, f, k, codes ? 1 : 0);
     if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
         return fail(TB200_ERR_WORKSPACE, "ffn_gated_bwd: needs a 256-byte aligned workspace of %zu bytes, got %zu", need, workspace ? workspace_bytes : size_t(0));
-    const int64_t ldg = pitch_of(f);
+    const int64_t ldg = grad_pitch(f, dtype);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     void* dg = ws;
-    void* du = ws + round_up(m * ldg * 2, 256);
-    void* xr = ws + 2 * round_up(m * ldg * 2, 256);
-    float* sums = reinterpret_cast<float*>(static_cast<uint8_t*>(xr) + (codes ? round_up(m * pitch_of(k) * 2, 256) : 0));
-    if (codes) ldx = reinterpret_cast<uintptr_t>(x) % 8 == 0 ? pitch_of(k) : k;
+    void* du = ws + grad_bytes(m, f, dtype);
+    void* xr = ws + 2 * grad_bytes(m, f, dtype);
+    float* sums = reinterpret_cast<float*>(static_cast<uint8_t*>(xr) + (codes ? round_up(m * x_pitch(k) * 2, 256) : 0));
+    if (codes) ldx = reinterpret_cast<uintptr_t>(x) % 8 == 0 ? x_pitch(k) : k;
     rc = launch_gated_act_bwd(dh, gq, gs, uq, us, dg, du, m, f, ldg, codes ? x : nullptr, xs, xr, k, ldx, act, dtype, st);
     if (rc != TB200_OK) return rc;
     if (codes) x = xr;
