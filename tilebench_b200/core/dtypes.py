@@ -1,6 +1,8 @@
 """dtype names used in operator configs (reference: tilebench/core/dtypes.py:6-47)."""
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 _SIZES = {
@@ -26,3 +28,15 @@ def resolve_dtype(dtype_name: str) -> torch.dtype:
     if isinstance(dt, torch.dtype):
         return dt
     raise ValueError(f"Unsupported dtype '{dtype_name}' for this environment.")
+
+
+@contextlib.contextmanager
+def full_fp32_matmul():
+    """fp32 products in full precision while it lasts.  The process's own setting comes back at the end: the fp32 reference of
+    matmul_fp32_fp16_fp8 runs with TF32 allowed, whichever operators ran before it."""
+    allowed = torch.backends.cuda.matmul.allow_tf32
+    torch.backends.cuda.matmul.allow_tf32 = False
+    try:
+        yield
+    finally:
+        torch.backends.cuda.matmul.allow_tf32 = allowed
