@@ -542,7 +542,7 @@ __device__ __forceinline__ float grad_power(const GradRange& r) {
 }
 
 // dg = dh * u * f'(g), du = dh * f(g) for 8 numbers of a lane, in fp32 and rounded once to T: they are operands of 16 bits in the
-// products that follow (half a step, 2^-9 of the value in bf16, which the products' sums average out).  dh comes times `power` in fp16.
+// products that follow (half a step, 2^-8 of the value in bf16 and 2^-11 in fp16, which the products' sums average out).  dh comes times `power` in fp16.
 template <typename T, int ACT>
 __device__ __forceinline__ void gated_bwd8(const uint32_t (&d)[4], const uint32_t (&cg)[2], const uint32_t (&cu)[2], float sg, float su, float power,
                                            uint4& dg, uint4& du) {
