@@ -1346,9 +1346,11 @@ int dx_few_shares(int64_t m, int64_t f, int64_t k) {
     return best;
 }
 
-// Whether dx goes to that kernel: few rows, and weights beyond what L2 (126 MB) holds of both.  Smaller ones gain more from sharing
-// a launch with dw than from the kernel's narrower tiles: 50 rows of 512 x 28000 38 us against 52, 33 of 2048 x 5632 32 against 35,
-// but 6 of 7192 x 28637 444 against 381.
+// Whether dx goes to that kernel: few rows, and weights of more than 100 MB in both, where its narrower tiles gain more than a launch
+// shared with dw does.  Captured calls with cold inputs, in a kernel of its own against together, at 1 / 16 / 64 rows: 57 MB (512 x 28000)
+// 47 / 49 / 57 us against 41 / 43 / 45; 84 MB (4096 x 5120) 49 / 51 / 55 against 53 / 53 / 53; 103 MB (3584 x 7168) 57 / 59 / 64 against
+// 57 / 59 / 61; 117 MB (4096 x 7168) 61 / 64 / 70 against 66 / 66 / 68; 180 MB (4096 x 11008) 84 / 86 / 92 against 92 / 92 / 94;
+// 235 MB (4096 x 14336) 104 / 107 / 113 against 115 / 117 / 119.  Between 80 and 150 MB it is a matter of 8 % either way, by rows and k.
 bool dx_alone(int64_t m, int64_t f, int64_t k) { return m <= kFewRows && f * k > (24ll << 20); }
 
 struct BwdPlan { int dx, dw, early; bool apart; }; // shares; early: see item_at; dx and dw in launches of their own
