@@ -139,3 +139,66 @@ def test_tensors_scaled_by_powers_of_two_give_the_same_bits(cuda_device):
     for a, b in zip(bwd.run(*args, "silu"), want):
         normal = b.abs() >= 2.0 ** -8
         assert torch.equal(a[normal].float() * 64, b[normal].float())
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_captured_behind_copies_fills_and_another_stream(cuda_device, m):
+    """The first kernel of a call begins over the end of what comes before it: a copy, a fill, another stream's work, a call of its own kind."""
+    k, f = 136, 200
+    dh, wg, wu, x, xs, *held = inputs(m, k, f, 1e-5)
+    source, weight = dh.clone(), wg.clone()
+    into, w, zeros = torch.empty_like(dh), torch.empty_like(wg), torch.ones_like(dh)
+    side = torch.cuda.Stream()
+
+    def step():
+        into.copy_(source)
+        first = bwd.run(into, wg, wu, x, xs, *held, "silu")
+        zeros.zero_()
+        none = bwd.run(zeros, wg, wu, x, xs, *held, "silu")
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            w.copy_(weight)
+            into.mul_(4096.0)
+        torch.cuda.current_stream().wait_stream(side)
+        return (*first, *none, *bwd.run(into, w, wu, x, xs, *held, "gelu"), *bwd.run(into, wg, w, x, xs, *held, "relu"))
+
+    def expected():
+        a, big, b = source.clone(), source * 4096.0, weight.clone()
+        torch.cuda.synchronize()
+        none = [torch.zeros_like(t) for t in bwd.run(a, wg, wu, x, xs, *held, "silu")]
+        return (*bwd.run(a, wg, wu, x, xs, *held, "silu"), *none, *bwd.run(big, b, wu, x, xs, *held, "gelu"), *bwd.run(big, wg, b, x, xs, *held, "relu"))
+    warm = torch.cuda.Stream()
+    warm.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(warm):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    g = torch.Generator(device="cuda").manual_seed(m)
+    for turn in range(4):
+        source.copy_(torch.randn(m, f, generator=g, device="cuda") * 10.0 ** -(2 + turn))
+        weight.copy_(torch.randn(f, k, generator=g, device="cuda") * 0.1)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, expected()))
+        assert all(torch.equal(a, b) for a, b in zip(step(), expected()))
+        torch.cuda.synchronize()
+
+
+def test_calls_of_different_size_on_two_streams_at_once(cuda_device):
+    sets = [inputs(64 + 200 * i, 512, 640, 10.0 ** -(1 + 4 * i), seed=i) for i in range(2)]
+    want = [bwd.run(*args, "silu") for args in sets]
+    for args, grads in zip(sets, want):
+        check(grads, args, "silu")
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(8):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(bwd.run(*sets[i], "silu"))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for grads in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(grads, want[i]))

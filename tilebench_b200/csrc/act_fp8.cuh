@@ -158,9 +158,10 @@ __device__ __forceinline__ float2 gate_both(float g) {
 // ---- launches that overlap their set-up with the end of the kernel before ----------------------------------------
 // Every kernel of the block lets the next one of its stream begin once all its CTAs have (let_next_begin), and the matrix
 // products are launched so that they may: their launch, barriers, tensor memory and tensor maps overlap with the end of
-// the kernel before, and they wait for it to be complete (wait_for_previous) before they touch global memory.  Only the
-// products are launched that way: what they read comes by TMA, from L2, whereas a load through L1 could meet a line that the
-// kernel before had left there.
+// the kernel before, and they wait for it to be complete (wait_for_previous) before they touch global memory.  So are the two
+// kernels that make fp16's power of two and use it.  The others, which stream, begin when the kernel before has ended (some 2 us later): they read
+// through the read-only path, which is for what nothing writes while the kernel is there, be it before it waits.  With ordinary loads
+// behind the wait they could overlap as well; that is not done.
 #ifdef __CUDACC__
 __device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
